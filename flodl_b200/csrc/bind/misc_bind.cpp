@@ -67,6 +67,130 @@ void rms_bwd(const Tensor& dy, const Tensor& x, const optional<Tensor>& w, const
                                    opt_ptr<float>(dw), rows, C, cur_stream()));
 }
 
+// Per-head RMS norm of queries and keys with the rotary embedding. Tensors are
+// [B, S, heads, D] with a contiguous last dimension, any other strides.
+int dtype_code(const Tensor& t) {
+  return t.scalar_type() == at::kFloat      ? 0
+         : t.scalar_type() == at::kBFloat16 ? 1
+         : t.scalar_type() == at::kHalf     ? 2
+                                            : -1;
+}
+
+flodl::QkNormRopeArgs qk_args(const Tensor& q, const Tensor& k, const optional<Tensor>& wq,
+                              const optional<Tensor>& wk, const optional<Tensor>& cos,
+                              const optional<Tensor>& sin, const optional<Tensor>& pos,
+                              int64_t offset, const Tensor& out_q, const Tensor& out_k,
+                              double eps) {
+  FL_CHECK_CUDA(q);
+  FL_CHECK(dtype_code(q) >= 0, "qk_norm_rope: f32, bf16 or f16 inputs");
+  const int64_t B = q.dim() == 4 ? q.size(0) : 0, S = q.dim() == 4 ? q.size(1) : 0;
+  auto heads = [&](const Tensor& t, const Tensor& like, const char* what) {
+    FL_CHECK(t.dim() == 4 && t.size(0) == B && t.size(1) == S && t.size(3) == q.size(3) &&
+                 t.size(2) == like.size(2) && t.scalar_type() == q.scalar_type() &&
+                 t.device() == q.device() && t.stride(3) == 1,
+             "qk_norm_rope: ", what, " must be [B, S, heads, D] of the queries' B, S, D, dtype and "
+             "device with a contiguous last dimension");
+  };
+  heads(q, q, "q");
+  heads(k, k, "k");
+  heads(out_q, q, "q output");
+  heads(out_k, k, "k output");
+  const int64_t D = q.size(3);
+  FL_CHECK(B > 0 && S > 0 && q.size(2) > 0 && k.size(2) > 0 && D > 0, "qk_norm_rope: empty input");
+  FL_CHECK(D <= flodl::kQkNormRopeMaxD, "qk_norm_rope: head size above ", flodl::kQkNormRopeMaxD);
+  FL_CHECK(B * S < (int64_t)1 << 31 && q.size(2) + k.size(2) < (int64_t)1 << 20,
+           "qk_norm_rope: too many rows");
+  flodl::QkNormRopeArgs a;
+  for (const optional<Tensor>* w : {&wq, &wk})
+    if (*w)
+      FL_CHECK((*w)->scalar_type() == at::kFloat && (*w)->is_contiguous() && (*w)->numel() == D &&
+                   (*w)->device() == q.device(), "qk_norm_rope: weights must be f32 [D]");
+  a.wq = opt_ptr<const float>(wq);
+  a.wk = opt_ptr<const float>(wk);
+  FL_CHECK(cos.has_value() == sin.has_value(), "qk_norm_rope: cos and sin come together");
+  if (cos) {
+    for (const Tensor* t : {&*cos, &*sin})
+      FL_CHECK(t->scalar_type() == at::kFloat && t->dim() == 2 && t->is_contiguous() &&
+                   t->device() == q.device() && t->sizes() == cos->sizes(),
+               "qk_norm_rope: cos and sin must be f32 [positions, R / 2]");
+    FL_CHECK(2 * cos->size(1) <= D, "qk_norm_rope: the tables rotate more than the head size");
+    a.cos = cos->data_ptr<float>();
+    a.sin = sin->data_ptr<float>();
+    a.R = (int)(2 * cos->size(1));
+    a.table_rows = cos->size(0);
+  }
+  if (a.R > 0 && pos) {
+    FL_CHECK(pos->scalar_type() == at::kLong && pos->is_contiguous() && pos->dim() == 2 &&
+                 pos->size(0) == B && pos->size(1) == S && pos->device() == q.device(),
+             "qk_norm_rope: positions must be int64 [B, S]");
+    a.pos = pos->data_ptr<int64_t>();
+  } else if (a.R > 0) {
+    FL_CHECK(offset >= 0 && offset <= a.table_rows - S, "qk_norm_rope: positions ", offset, " to ",
+             offset + S - 1, " outside the tables' ", a.table_rows, " rows");
+  }
+  a.offset = offset;
+  auto st = [](const Tensor& t, int64_t (&s)[3]) {
+    for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+  };
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.out_q = out_q.data_ptr();
+  a.out_k = out_k.data_ptr();
+  st(q, a.q_st);
+  st(k, a.k_st);
+  st(out_q, a.oq_st);
+  st(out_k, a.ok_st);
+  a.B = (int)B; a.S = (int)S; a.H = (int)q.size(2); a.Hk = (int)k.size(2); a.D = (int)D;
+  a.dtype = dtype_code(q);
+  a.eps = (float)eps;
+  return a;
+}
+
+void qk_norm_rope_fwd(const Tensor& q, const Tensor& k, const optional<Tensor>& wq,
+                      const optional<Tensor>& wk, const optional<Tensor>& cos,
+                      const optional<Tensor>& sin, const optional<Tensor>& pos, int64_t offset,
+                      Tensor& yq, Tensor& yk, double eps) {
+  const auto a = qk_args(q, k, wq, wk, cos, sin, pos, offset, yq, yk, eps);
+  c10::cuda::CUDAGuard guard(q.device());
+  FL_CUDA_OK(flodl::launch_qk_norm_rope_fwd(a, cur_stream()));
+}
+
+void qk_norm_rope_bwd(const Tensor& dyq, const Tensor& dyk, const Tensor& q, const Tensor& k,
+                      const optional<Tensor>& wq, const optional<Tensor>& wk,
+                      const optional<Tensor>& cos, const optional<Tensor>& sin,
+                      const optional<Tensor>& pos, int64_t offset, Tensor& dq, Tensor& dk,
+                      const optional<Tensor>& dwq, const optional<Tensor>& dwk, double eps) {
+  auto a = qk_args(q, k, wq, wk, cos, sin, pos, offset, dq, dk, eps);
+  for (const Tensor* t : {&dyq, &dyk})
+    FL_CHECK(t->scalar_type() == q.scalar_type() && t->device() == q.device() && t->dim() == 4 &&
+                 t->stride(3) == 1, "qk_norm_rope: output gradients of the inputs' dtype and device "
+             "with a contiguous last dimension");
+  FL_CHECK(dyq.sizes() == q.sizes() && dyk.sizes() == k.sizes(),
+           "qk_norm_rope: output gradients of the outputs' shapes");
+  a.dyq = dyq.data_ptr();
+  a.dyk = dyk.data_ptr();
+  for (int i = 0; i < 3; ++i) {
+    a.dyq_st[i] = dyq.size(i) > 1 ? dyq.stride(i) : 0;
+    a.dyk_st[i] = dyk.size(i) > 1 ? dyk.stride(i) : 0;
+  }
+  for (const optional<Tensor>* w : {&dwq, &dwk})
+    if (*w)
+      FL_CHECK((*w)->scalar_type() == at::kFloat && (*w)->is_contiguous() &&
+                   (*w)->numel() == q.size(3) && (*w)->device() == q.device(),
+               "qk_norm_rope: weight gradients must be f32 [D]");
+  a.dwq = opt_ptr<float>(dwq);
+  a.dwk = opt_ptr<float>(dwk);
+  FL_CHECK(!a.dwq || a.dwq != a.dwk, "qk_norm_rope: one buffer for both weight gradients");
+  c10::cuda::CUDAGuard guard(q.device());
+  Tensor partials;
+  if (a.dwq || a.dwk) {
+    a.partial_rows = flodl::qk_norm_rope_partial_rows(a);
+    partials = at::empty({a.partial_rows, 2, q.size(3)}, q.options().dtype(at::kFloat));
+    a.partials = partials.data_ptr<float>();
+  }
+  FL_CUDA_OK(flodl::launch_qk_norm_rope_bwd(a, cur_stream()));
+}
+
 // GroupNorm over x [N, C, *] contiguous (f32 or bf16), G groups.
 void gn_fwd(const Tensor& x, const optional<Tensor>& gamma, const optional<Tensor>& beta,
             Tensor& y, Tensor& mean, Tensor& rstd, int64_t G, double eps) {
@@ -404,6 +528,13 @@ void register_elementwise(py::module& m) {
         py::arg("eps"));
   m.def("rms_bwd", &rms_bwd, py::arg("dy"), py::arg("x"), py::arg("w"), py::arg("rstd"),
         py::arg("dx"), py::arg("dw"));
+  m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd, py::arg("q"), py::arg("k"), py::arg("wq"),
+        py::arg("wk"), py::arg("cos"), py::arg("sin"), py::arg("pos"), py::arg("offset"),
+        py::arg("yq"), py::arg("yk"), py::arg("eps"));
+  m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd, py::arg("dyq"), py::arg("dyk"), py::arg("q"),
+        py::arg("k"), py::arg("wq"), py::arg("wk"), py::arg("cos"), py::arg("sin"), py::arg("pos"),
+        py::arg("offset"), py::arg("dq"), py::arg("dk"), py::arg("dwq"), py::arg("dwk"),
+        py::arg("eps"));
   m.def("gn_fwd", &gn_fwd, py::arg("x"), py::arg("gamma"), py::arg("beta"), py::arg("y"),
         py::arg("mean"), py::arg("rstd"), py::arg("groups"), py::arg("eps"));
   m.def("gn_bwd", &gn_bwd, py::arg("dy"), py::arg("x"), py::arg("gamma"), py::arg("mean"),

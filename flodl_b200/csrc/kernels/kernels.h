@@ -49,6 +49,28 @@ cudaError_t launch_rms_fwd(const void* x, bool bf16, const float* w, void* y, fl
 cudaError_t launch_rms_bwd(const void* dy, const void* x, bool bf16, const float* w,
                            const float* rstd, void* dx, float* dw, int rows, int C,
                            cudaStream_t st);
+// Per-head RMS norm of queries and keys with the rotary embedding
+// (qk_norm_rope.cu). Strides in elements for (batch, position, head), the last
+// dimension contiguous; dtype 0 = f32, 1 = bf16, 2 = f16.
+constexpr int kQkNormRopeMaxD = 256;
+struct QkNormRopeArgs {
+  const void *q = nullptr, *k = nullptr;      // [B, S, H, D], [B, S, Hk, D]
+  const void *dyq = nullptr, *dyk = nullptr;  // backward: gradients of the outputs
+  void *out_q = nullptr, *out_k = nullptr;    // outputs (forward), input gradients (backward)
+  const float *wq = nullptr, *wk = nullptr;   // [D] (nullable: ones)
+  const float *cos = nullptr, *sin = nullptr; // [table_rows, R / 2] (R = 0: no rotation)
+  const int64_t* pos = nullptr;               // [B, S] table rows (nullable: offset + s)
+  int64_t q_st[3] = {}, k_st[3] = {}, dyq_st[3] = {}, dyk_st[3] = {}, oq_st[3] = {}, ok_st[3] = {};
+  int64_t offset = 0, table_rows = 0;
+  int B = 0, S = 0, H = 0, Hk = 0, D = 0, R = 0, dtype = 0;
+  float eps = 1e-5f;
+  float *dwq = nullptr, *dwk = nullptr;  // backward: += weight gradients (nullable, distinct)
+  float* partials = nullptr;             // backward with weight gradients: [partial_rows, 2, D]
+  int partial_rows = 0;
+};
+int qk_norm_rope_partial_rows(const QkNormRopeArgs& a);
+cudaError_t launch_qk_norm_rope_fwd(const QkNormRopeArgs& a, cudaStream_t st);
+cudaError_t launch_qk_norm_rope_bwd(const QkNormRopeArgs& a, cudaStream_t st);
 // Dropout (dropout.cu): y = x * keep / (1 - p), keep drawn from Philox-4x32-10
 // on (element, offset) with the key seed; the same seed and offset give the
 // same mask (the backward calls it on dy). x/y f32 or bf16, 0 <= p < 1.

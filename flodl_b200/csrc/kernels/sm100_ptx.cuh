@@ -49,6 +49,7 @@ enum KernelError : uint32_t {
   kErrPeerTimeout = 2,
   kErrBadArgs = 3,
   kErrBadLabel = 4,  // a class target outside [0, V) that is not ignore_index
+  kErrBadPosition = 5,  // a position outside the rotary tables
 };
 
 __device__ __forceinline__ void report_error(uint32_t* err, uint32_t code) {
