@@ -1,6 +1,10 @@
-// Torch bindings for the flash attention kernels.
+// Torch bindings for the attention kernels.
+#include <cmath>
+#include <tuple>
+
 #include "common.h"
 #include "../kernels/flash_attn.h"
+#include "../kernels/cross_attn.h"
 
 namespace {
 
@@ -65,6 +69,153 @@ void flash_bwd(const Tensor& dout, const Tensor& qkv, const Tensor& out, const T
   FL_CUDA_OK(flodl::launch_flash_bwd(a, cur_stream()));
 }
 
+// ---- attention with queries, keys and values in tensors of their own
+// [B, positions, heads, D], 16-bit, last dimension contiguous, strides of 16
+// bytes, 16-byte aligned.
+void cross_strides(const Tensor& t, const char* what, int64_t B, int64_t S, int64_t heads,
+                   int64_t D, const Tensor& like, int64_t (&st)[3]) {
+  FL_CHECK(t.dim() == 4 && t.size(0) == B && t.size(1) == S && t.size(2) == heads && t.size(3) == D,
+           "cross_attn: ", what, " must be [", B, ", ", S, ", ", heads, ", ", D, "] (got ", t.sizes(), ")");
+  FL_CHECK(t.scalar_type() == like.scalar_type() && t.device() == like.device(), "cross_attn: ", what,
+           " must have the queries' dtype and device");
+  FL_CHECK(t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "cross_attn: ",
+           what, " needs a contiguous last dimension and 16-byte alignment");
+  for (int i = 0; i < 3; ++i) {
+    st[i] = t.size(i) > 1 ? t.stride(i) : 0;
+    FL_CHECK(t.size(i) == 1 || (st[i] > 0 && st[i] % 8 == 0), "cross_attn: ", what,
+             " needs strides of 16 bytes (got ", t.strides(), ")");
+  }
+}
+
+flodl::CrossAttnArgs cross_args(const Tensor& q, const Tensor& k, const Tensor& v,
+                                const optional<Tensor>& key_pad, const optional<Tensor>& mask_bits,
+                                bool causal, double scale) {
+  FL_CHECK_CUDA(q);
+  FL_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf,
+           "cross_attn: bf16 or f16 inputs");
+  FL_CHECK(q.dim() == 4 && k.dim() == 4, "cross_attn: [B, positions, heads, D] inputs");
+  const int64_t B = q.size(0), Sq = q.size(1), H = q.size(2), D = q.size(3);
+  const int64_t Sk = k.size(1), Hk = k.size(2);
+  constexpr int64_t kMax = (int64_t)1 << 30;
+  FL_CHECK(B > 0 && Sq > 0 && Sk > 0 && H > 0 && Hk > 0 && H % Hk == 0 && B < kMax && Sq < kMax &&
+               Sk < kMax && H < kMax,
+           "cross_attn: sizes (positive, query heads a multiple of the memory heads)");
+  FL_CHECK(D > 0 && D <= 128 && D % 8 == 0, "cross_attn: head size a multiple of 8 up to 128");
+  FL_CHECK(!causal || Sq == Sk, "cross_attn: causal needs equal lengths");
+  FL_CHECK(scale > 0 && std::isfinite(scale), "cross_attn: scale must be positive");
+  flodl::CrossAttnArgs a;
+  cross_strides(q, "q", B, Sq, H, D, q, a.q_st);
+  cross_strides(k, "k", B, Sk, Hk, D, q, a.k_st);
+  cross_strides(v, "v", B, Sk, Hk, D, q, a.v_st);
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.B = (int)B; a.Sq = (int)Sq; a.Sk = (int)Sk; a.H = (int)H; a.Hk = (int)Hk; a.D = (int)D;
+  a.causal = causal;
+  a.half = q.scalar_type() == at::kHalf;
+  a.scale = (float)scale;
+  if (key_pad) {
+    FL_CHECK(key_pad->scalar_type() == at::kBool && key_pad->is_contiguous() && key_pad->dim() == 2 &&
+                 key_pad->size(0) == B && key_pad->size(1) == Sk && key_pad->device() == q.device(),
+             "cross_attn: key_pad must be bool [B, Sk]");
+    a.key_pad = reinterpret_cast<const uint8_t*>(key_pad->data_ptr());
+    if (mask_bits) {
+      FL_CHECK(mask_bits->scalar_type() == at::kInt && mask_bits->is_contiguous() &&
+                   mask_bits->numel() == B * ((Sk + 31) / 32 + 1) && mask_bits->device() == q.device(),
+               "cross_attn: mask_bits of another mask");
+      a.vis_end = mask_bits->data_ptr<int>();
+      a.words = reinterpret_cast<uint32_t*>(a.vis_end + B);
+    }
+  }
+  return a;
+}
+
+// The mask as [B] ends of the visible keys, then [B, ceil(Sk / 32)] words with
+// a bit per visible key.
+Tensor cross_attn_mask(const Tensor& key_pad) {
+  FL_CHECK_CUDA(key_pad);
+  FL_CHECK(key_pad.scalar_type() == at::kBool && key_pad.is_contiguous() && key_pad.dim() == 2 &&
+               key_pad.numel() > 0 && key_pad.size(0) < (int64_t)1 << 30 &&
+               key_pad.size(1) < (int64_t)1 << 30, "cross_attn: key_pad must be bool [B, Sk]");
+  const int64_t B = key_pad.size(0), Sk = key_pad.size(1);
+  c10::cuda::CUDAGuard guard(key_pad.device());
+  Tensor bits = at::empty({B * ((Sk + 31) / 32 + 1)}, key_pad.options().dtype(at::kInt));
+  flodl::CrossAttnArgs a;
+  a.key_pad = reinterpret_cast<const uint8_t*>(key_pad.data_ptr());
+  a.vis_end = bits.data_ptr<int>();
+  a.words = reinterpret_cast<uint32_t*>(a.vis_end + B);
+  a.B = (int)B;
+  a.Sk = (int)Sk;
+  FL_CUDA_OK(flodl::launch_cross_attn_pack_mask(a, cur_stream()));
+  return bits;
+}
+
+// -> (output [B, Sq, H, D], lse2 [B, H, Sq] f32 or none, mask bits or none)
+std::tuple<Tensor, optional<Tensor>, optional<Tensor>> cross_attn_fwd(
+    const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& key_pad, bool causal,
+    double scale, bool want_lse) {
+  auto a = cross_args(q, k, v, key_pad, c10::nullopt, causal, scale);
+  c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty({a.B, a.Sq, a.H, a.D}, q.options());
+  a.out = out.data_ptr();
+  optional<Tensor> lse, bits;
+  if (want_lse) {
+    lse = at::empty({a.B, a.H, a.Sq}, q.options().dtype(at::kFloat));
+    a.lse2 = lse->data_ptr<float>();
+  }
+  if (a.key_pad && !flodl::cross_attn_is_few(a)) {
+    bits = cross_attn_mask(*key_pad);
+    a.vis_end = bits->data_ptr<int>();
+    a.words = reinterpret_cast<uint32_t*>(a.vis_end + a.B);
+  }
+  Tensor part;
+  if (const int64_t n = flodl::cross_attn_fwd_partials(a)) {
+    part = at::empty({n}, q.options().dtype(at::kFloat));
+    a.partials = part.data_ptr<float>();
+  }
+  FL_CUDA_OK(flodl::launch_cross_attn_fwd(a, cur_stream()));
+  return {out, lse, bits};
+}
+
+// Gradients into dq, dk, dv (any strides of 16 bytes).
+void cross_attn_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v,
+                    const Tensor& out, const Tensor& lse2, const optional<Tensor>& key_pad,
+                    const optional<Tensor>& mask_bits, bool causal, double scale, Tensor& dq,
+                    Tensor& dk, Tensor& dv) {
+  auto a = cross_args(q, k, v, key_pad, mask_bits, causal, scale);
+  cross_strides(dout, "dout", a.B, a.Sq, a.H, a.D, q, a.do_st);
+  cross_strides(dq, "dq", a.B, a.Sq, a.H, a.D, q, a.dq_st);
+  cross_strides(dk, "dk", a.B, a.Sk, a.Hk, a.D, q, a.dk_st);
+  cross_strides(dv, "dv", a.B, a.Sk, a.Hk, a.D, q, a.dv_st);
+  FL_CHECK(out.sizes() == q.sizes() && out.is_contiguous() && out.scalar_type() == q.scalar_type() &&
+               out.device() == q.device(), "cross_attn: out must be the forward's");
+  FL_CHECK(lse2.scalar_type() == at::kFloat && lse2.is_contiguous() &&
+               lse2.numel() == (int64_t)a.B * a.H * a.Sq && lse2.device() == q.device(),
+           "cross_attn: lse2 must be the forward's");
+  c10::cuda::CUDAGuard guard(q.device());
+  a.dout = dout.data_ptr();
+  a.out = out.data_ptr();
+  a.lse2 = lse2.data_ptr<float>();
+  a.dq = dq.data_ptr();
+  a.dk = dk.data_ptr();
+  a.dv = dv.data_ptr();
+  Tensor bits;
+  if (a.key_pad && !a.words) {
+    bits = cross_attn_mask(*key_pad);
+    a.vis_end = bits.data_ptr<int>();
+    a.words = reinterpret_cast<uint32_t*>(a.vis_end + a.B);
+  }
+  auto f32 = q.options().dtype(at::kFloat);
+  Tensor stats = at::empty({flodl::cross_attn_stats_floats(a)}, f32);
+  a.stats = stats.data_ptr<float>();
+  Tensor part;
+  if (const int64_t n = flodl::cross_attn_bwd_partials(a)) {
+    part = at::empty({n}, f32);
+    a.partials = part.data_ptr<float>();
+  }
+  FL_CUDA_OK(flodl::launch_cross_attn_bwd(a, cur_stream()));
+}
+
 }  // namespace
 
 void register_attention(py::module& m) {
@@ -76,4 +227,10 @@ void register_attention(py::module& m) {
         py::arg("lse2"), py::arg("dqkv"), py::arg("B"), py::arg("S"), py::arg("H"), py::arg("D"),
         py::arg("causal"), py::arg("scale"), py::arg("key_pad") = py::none(),
         py::arg("dbias") = py::none());
+  m.def("cross_attn_mask", &cross_attn_mask, py::arg("key_pad"));
+  m.def("cross_attn_fwd", &cross_attn_fwd, py::arg("q"), py::arg("k"), py::arg("v"),
+        py::arg("key_pad"), py::arg("causal"), py::arg("scale"), py::arg("want_lse"));
+  m.def("cross_attn_bwd", &cross_attn_bwd, py::arg("dout"), py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("out"), py::arg("lse2"), py::arg("key_pad"), py::arg("mask_bits"),
+        py::arg("causal"), py::arg("scale"), py::arg("dq"), py::arg("dk"), py::arg("dv"));
 }

@@ -1,0 +1,1325 @@
+// Attention with queries, keys and values in tensors of their own, forward and
+// backward, on tcgen05 tensor cores: cross attention to an encoder's states of
+// another length, memory heads shared by several query heads, any strides.
+// The form for a few query rows is in cross_attn_few.cu.
+//
+//   S = Q K^T,  P = softmax(c S + mask),  O = P V
+//   backward, from the base-2 log-sum-exp and delta = rowsum(dO * O):
+//   P = 2^(c log2e S - lse2),  dS = P (dO V^T - delta),
+//   dQ = c dS K,  dK = c dS^T Q,  dV = P^T dO
+//
+// Tiles come by 4-D TMA maps {D, position, head, batch} straight from the
+// strided tensors: no copy for packed projections, rows past the end and
+// columns past D are zero-filled (D is rounded up to 64 or 128).
+//
+// All three kernels have one shape: 128 rows of the stationary side lie on the
+// TMEM lanes (a compute thread owns a row), tiles of the other side stream
+// through shared memory, the elementwise result is written back to TMEM as
+// 16-bit pairs and is the A operand of the next product, so no score touches
+// shared memory. Scores of one tile are computed by the tensor cores while the
+// compute warps are on another.
+//   forward  rows = queries, stream K, V:  S -> P, O += P V
+//   dQ       rows = queries, stream K, V:  S, dP -> dS, dQ += dS K
+//   dK/dV    rows = keys, stream Q, dO:    S^T, dP^T -> P^T, dS^T, dV += P^T dO, dK += dS^T Q
+// dQ has a kernel of its own, which recomputes S and dP (seven products instead
+// of five), so that no gradient is summed by atomics: results do not depend on
+// the order of execution. Where the items are fewer than the SMs, the streamed
+// axis is split and the pieces are added (the forward's joined by lse) in order
+// by a second kernel.
+//
+// Hidden keys: a packing kernel turns the padding mask into a bit per key and
+// the end of the visible keys of each sample; tiles past it are not visited.
+// Scores of hidden keys are replaced, not added to, and in a tile that mixes
+// hidden and visible keys the hidden rows of the B operand (V, or K for dQ) are
+// zeroed in shared memory, so that whatever a padded position holds (NaN too)
+// has no effect.
+//
+// All waits are bounded (see sm100_ptx.cuh).
+#include "sm100_ptx.cuh"
+#include "cross_attn.h"
+
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+#include <type_traits>
+
+namespace flodl {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRows = 128;  // stationary rows of a tile: the TMEM lanes
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units: P stays below 2^8
+
+template <typename T>
+struct Type;
+template <>
+struct Type<__nv_bfloat16> {
+  static constexpr uint32_t kIdesc = 1;  // tcgen05 kind::f16 operand format
+  static constexpr float kShift = 0.f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+};
+template <>
+struct Type<__half> {
+  static constexpr uint32_t kIdesc = 0;
+  // P of a long row lies below f16's normal range (2^-14): the backward's P^T
+  // is formed at 2^7 times its value and dV scaled back
+  static constexpr float kShift = 7.f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+__host__ __device__ constexpr uint32_t idesc(uint32_t fmt, uint32_t M, uint32_t N, uint32_t b_mn) {
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x,
+                                            int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// A tile of kN rows and kDP columns: kDP / 64 blocks of kN rows x 128 bytes in
+// 128-byte swizzle.
+template <int kN, int kDP>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar,
+                                          int row, int head, int batch) {
+#pragma unroll
+  for (int c = 0; c < kDP / 64; ++c)
+    tma_load_4d(dst + c * kN * 128, map, bar, c * 64, row, head, batch);
+}
+
+// D[128, n] (+)= A[128, kDP] B[n, kDP]^T, both tiles K-major in shared memory.
+template <int kNA, int kNB, int kDP>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t id) {
+#pragma unroll
+  for (int kk = 0; kk < kDP / 16; ++kk)
+    umma_bf16(d, make_sdesc_sw128(a + (kk / 4) * (kNA * 128) + (kk % 4) * 32, 16, 1024),
+              make_sdesc_sw128(b + (kk / 4) * (kNB * 128) + (kk % 4) * 32, 16, 1024), id, kk > 0);
+}
+// D[128, kDP] (+)= A[128, kK] B[kK, kDP], A 16-bit pairs in TMEM, B a streamed
+// tile read along its rows (MN-major).
+template <int kK, int kDP>
+__device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t id,
+                                         bool acc) {
+#pragma unroll
+  for (int kk = 0; kk < kK / 16; ++kk)
+    umma_bf16_tmem_a(d, a_tmem + kk * 8, make_sdesc_sw128(b + kk * 2048, kK * 128, 1024), id,
+                     (acc || kk > 0) ? 1u : 0u);
+}
+
+// Zero the rows of a streamed tile whose bit in words is clear (thread `tid` of
+// `nthreads`), before a product reads them as B.
+template <int kN, int kDP>
+__device__ __forceinline__ void zero_hidden_rows(uint8_t* tile, const uint32_t (&words)[kN / 32],
+                                                 int tid, int nthreads) {
+  for (int i = tid; i < kN * (kDP / 64); i += nthreads) {
+    const int row = i % kN;
+    uint32_t word = words[0];  // words stay in registers: no index at run time
+#pragma unroll
+    for (int w = 1; w < kN / 32; ++w) word = row / 32 == w ? words[w] : word;
+    if (!((word >> (row % 32)) & 1u)) {
+      uint4* r = reinterpret_cast<uint4*>(tile + (i / kN) * kN * 128 + row * 128);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) r[c] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  fence_proxy_async_shared();
+}
+
+struct Shape {
+  int B, Sq, Sk, H, Hk, G, D, causal;
+  int splits;
+  float scale;
+  const uint32_t* words;  // [B, nwords] or null
+  const int* vis_end;     // [B]
+  int nwords;
+  uint32_t* err;
+};
+
+__device__ __forceinline__ int visible_end(const Shape& s, int b) {
+  return s.vis_end ? __ldg(s.vis_end + b) : s.Sk;
+}
+
+struct Waiter {
+  volatile uint32_t* abort;
+  uint32_t* err;
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+    return mbar_wait_bounded(bar, parity, abort, err, kWaitNs);
+  }
+};
+
+// After a failed wait: the copies still in flight write this CTA's shared
+// memory, so give each issued load (bounded) time to land before leaving.
+__device__ __forceinline__ void settle(uint64_t* bar, uint32_t issued) {
+  if (issued == 0) return;
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, (issued - 1) & 1) && global_timer_ns() - t0 < 100000000ull) {
+  }
+}
+
+// ============================================================== forward
+// One item: 128 queries of a head, and a range of its key tiles. Warps: 0 TMA,
+// 1 MMA, 2..5 softmax (a row per thread). Two CTAs per SM (256 TMEM columns,
+// 97 KB of shared memory each) cover each other's waits.
+//   kDP =  64: tiles of 128 keys; S at 0 (128 columns), P at 128 (64), O at 192:
+//              the next S starts once this one has been read.
+//   kDP = 128: tiles of 64 keys; S double-buffered at 0 and 64 with P over its
+//              own scores, O at 128.
+template <int kDP>
+struct FwdGeo {
+  static constexpr int kN = kDP == 64 ? 128 : 64;
+  static constexpr int kQBufs = kDP == 64 ? 2 : 1;
+  static constexpr int kStages = 2;
+  static constexpr uint32_t kO = kDP == 64 ? 192 : 128;
+};
+constexpr int kFwdThreads = 192;
+
+template <int kDP>
+struct FwdSmem {
+  using G = FwdGeo<kDP>;
+  uint8_t q[G::kQBufs][kRows * kDP * 2];
+  uint8_t k[G::kStages][G::kN * kDP * 2];
+  uint8_t v[G::kStages][G::kN * kDP * 2];
+  uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], s_free, p_full, pv_done;
+  uint64_t drain;
+  uint32_t tmem_base, abort;
+};
+
+// Items run from the last query tile to the first (under a causal mask the
+// heaviest first), heads and batches fastest.
+struct FwdItem {
+  int qt, h, b, split, lo, hi;  // key tiles [lo, hi)
+};
+template <int kN>
+__device__ __forceinline__ FwdItem fwd_item(const Shape& s, int item, int n_qt) {
+  FwdItem it;
+  it.split = item % s.splits;
+  item /= s.splits;
+  const int n_bh = s.H * s.B;
+  it.qt = n_qt - 1 - item / n_bh;
+  const int bh = item % n_bh;
+  it.h = bh % s.H;
+  it.b = bh / s.H;
+  int end = visible_end(s, it.b);
+  if (s.causal) end = min(end, (it.qt + 1) * kRows);
+  const int nt = (end + kN - 1) / kN;
+  it.lo = (int)((int64_t)nt * it.split / s.splits);
+  it.hi = (int)((int64_t)nt * (it.split + 1) / s.splits);
+  return it;
+}
+
+// Visible-key words of the tile at key k0 (keys past Sk are clear).
+template <int kN>
+__device__ __forceinline__ void tile_words(const Shape& s, int b, int k0, uint32_t (&w)[kN / 32]) {
+#pragma unroll
+  for (int i = 0; i < kN / 32; ++i) {
+    const int at = k0 / 32 + i;
+    if (s.words) {
+      w[i] = at < s.nwords ? __ldg(s.words + (int64_t)b * s.nwords + at) : 0u;
+    } else {
+      const int left = s.Sk - at * 32;
+      w[i] = left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
+    }
+  }
+}
+
+template <typename T, int kDP>
+__global__ void __launch_bounds__(kFwdThreads, 2)
+    cross_fwd_kernel(const __grid_constant__ CUtensorMap tm_q,
+                     const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Shape sh,
+                     T* __restrict__ out, float* __restrict__ lse2, float* __restrict__ part_o,
+                     float* __restrict__ part_lse, int n_items, int n_qt) {
+  using Geo = FwdGeo<kDP>;
+  constexpr int kN = Geo::kN;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  FwdSmem<kDP>& sm = *reinterpret_cast<FwdSmem<kDP>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const Waiter wait{&sm.abort, sh.err};
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.q_full[i], 1);
+      mbar_init(&sm.q_empty[i], 1);
+      mbar_init(&sm.k_full[i], 1);
+      mbar_init(&sm.k_empty[i], 1);
+      mbar_init(&sm.v_full[i], 1);
+      mbar_init(&sm.v_empty[i], 1);
+      mbar_init(&sm.s_full[i], 1);
+    }
+    mbar_init(&sm.s_free, 4);
+    mbar_init(&sm.p_full, 4);
+    mbar_init(&sm.pv_done, 1);
+    mbar_init(&sm.drain, 1);
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc<256>(&sm.tmem_base);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (elect_one_sync()) {
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+      uint32_t n = 0, t = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+        const FwdItem it = fwd_item<kN>(sh, item, n_qt);
+        if (it.lo >= it.hi) continue;
+        const uint32_t qb = n % Geo::kQBufs;
+        if (!(ok = wait(&sm.q_empty[qb], ((n / Geo::kQBufs) & 1) ^ 1))) break;
+        mbar_arrive_expect_tx(&sm.q_full[qb], kRows * kDP * 2);
+        load_tile<kRows, kDP>(sm.q[qb], &tm_q, &sm.q_full[qb], it.qt * kRows, it.h, it.b);
+        ++n;
+        const int kh = it.h / sh.G;
+        for (int j = it.lo; j < it.hi; ++j, ++t) {
+          const uint32_t st = t & 1, par = ((t >> 1) & 1) ^ 1;
+          if (!(ok = wait(&sm.k_empty[st], par))) break;
+          mbar_arrive_expect_tx(&sm.k_full[st], kN * kDP * 2);
+          load_tile<kN, kDP>(sm.k[st], &tm_k, &sm.k_full[st], j * kN, kh, it.b);
+          if (!(ok = wait(&sm.v_empty[st], par))) break;
+          mbar_arrive_expect_tx(&sm.v_full[st], kN * kDP * 2);
+          load_tile<kN, kDP>(sm.v[st], &tm_v, &sm.v_full[st], j * kN, kh, it.b);
+        }
+      }
+      if (!ok) {
+        for (uint32_t i = 0; i < Geo::kQBufs; ++i)
+          settle(&sm.q_full[i], (n + Geo::kQBufs - 1 - i) / Geo::kQBufs);
+        for (uint32_t i = 0; i < 2; ++i) {
+          settle(&sm.k_full[i], (t + 2 - i) / 2);
+          settle(&sm.v_full[i], (t + 1 - i) / 2);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (elect_one_sync()) {
+      constexpr uint32_t id_s = idesc(Type<T>::kIdesc, kRows, kN, 0);
+      constexpr uint32_t id_o = idesc(Type<T>::kIdesc, kRows, kDP, 1);
+      const uint32_t t_o = tmem + Geo::kO;
+      uint32_t n = 0, t = 0;  // t: tile whose S is issued next
+      bool ok = true, issued = false;
+      // P V of tile u (the u-th of this CTA)
+      auto issue_pv = [&](uint32_t u, bool acc) -> bool {
+        if (!wait(&sm.v_full[u & 1], (u >> 1) & 1)) return false;
+        if (!wait(&sm.p_full, u & 1)) return false;
+        tc_fence_after();
+        const uint32_t t_p = tmem + (kDP == 64 ? 128u : (u & 1) * 64u);
+        mma_cols<kN, kDP>(t_o, t_p, smem_u32(sm.v[u & 1]), id_o, acc);
+        umma_commit(&sm.v_empty[u & 1]);
+        umma_commit(&sm.pv_done);
+        return true;
+      };
+      // P V of a tile is issued behind S of the next one, over item borders too
+      // where the next item's Q has a buffer of its own
+      bool behind = false, behind_acc = false;
+      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+        const FwdItem it = fwd_item<kN>(sh, item, n_qt);
+        if (it.lo >= it.hi) continue;
+        const uint32_t qb = n % Geo::kQBufs;
+        if (Geo::kQBufs == 1 && behind) {
+          if (!(ok = issue_pv(t - 1, behind_acc))) break;
+          behind = false;
+        }
+        if (!(ok = wait(&sm.q_full[qb], (n / Geo::kQBufs) & 1))) break;
+        ++n;
+        const uint32_t q_addr = smem_u32(sm.q[qb]);
+        for (int j = it.lo; j < it.hi; ++j, ++t) {
+          if (!(ok = wait(&sm.k_full[t & 1], (t >> 1) & 1))) break;
+          // the single S buffer has been read (kDP = 64); with two, S of tile
+          // t - 2 became P, whose product was issued before this one
+          if (kDP == 64 && !(ok = wait(&sm.s_free, (t & 1) ^ 1))) break;
+          tc_fence_after();
+          mma_rows<kRows, kN, kDP>(tmem + (kDP == 64 ? 0u : (t & 1) * 64u), q_addr,
+                                   smem_u32(sm.k[t & 1]), id_s);
+          issued = true;
+          umma_commit(&sm.k_empty[t & 1]);
+          umma_commit(&sm.s_full[t & 1]);
+          if (j == it.hi - 1) umma_commit(&sm.q_empty[qb]);
+          if (behind && !(ok = issue_pv(t - 1, behind_acc))) break;
+          behind = true;
+          behind_acc = j > it.lo;
+        }
+      }
+      if (ok && behind) ok = issue_pv(t - 1, behind_acc);
+      if (!ok && issued) {
+        umma_commit(&sm.drain);
+        settle(&sm.drain, 1);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int r = (warp & 3) * 32 + lane;  // query row within the tile
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_o = tmem + Geo::kO + lanes;
+    const float sl2 = sh.scale * kLog2e;
+    const uint64_t sl2x2 = f2_splat(sl2);
+    uint32_t t = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+      const FwdItem it = fwd_item<kN>(sh, item, n_qt);
+      const int qi = it.qt * kRows + r;
+      float m_ref = -INFINITY, l = 0.f;  // reference maximum (scaled, log2 units), row sum
+      for (int j = it.lo; j < it.hi; ++j, ++t) {
+        const int k0 = j * kN;
+        uint32_t words[kN / 32];
+        tile_words<kN>(sh, it.b, k0, words);
+        bool mixed = false;  // the tile holds hidden keys (not counting those past Sk)
+        if (sh.words) {
+#pragma unroll
+          for (int i = 0; i < kN / 32; ++i) {
+            const int left = sh.Sk - k0 - 32 * i;
+            const uint32_t whole = left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
+            mixed |= words[i] != whole;
+          }
+        }
+        const uint32_t t_s = tmem + lanes + (kDP == 64 ? 0u : (t & 1) * 64u);
+        const uint32_t t_p = kDP == 64 ? tmem + lanes + 128u : t_s;
+        const bool diag = sh.causal && k0 + kN - 1 > it.qt * kRows;
+        ok = wait(&sm.s_full[t & 1], (t >> 1) & 1);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc_fence_after();
+        // scores of 32 columns, hidden ones -inf
+        auto scores = [&](int c, const uint32_t (&raw)[32], float (&v)[32]) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
+          if (words[c] != 0xffffffffu) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = (words[c] >> i) & 1u ? v[i] : -INFINITY;
+          }
+          if (diag) {
+            const int lim = qi - (k0 + c * 32);  // last visible column
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = i <= lim ? v[i] : -INFINITY;
+          }
+        };
+        // pass 1: row maximum of the raw scores (the scale is positive)
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c2 = 0; c2 < kN / 64; ++c2) {
+          uint32_t raw[2][32];
+          tmem_ld_32cols(t_s + c2 * 64, raw[0]);
+          tmem_ld_32cols(t_s + c2 * 64 + 32, raw[1]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2) {
+            float v[32];
+            scores(c2 * 2 + h2, raw[h2], v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
+          }
+        }
+        const float mraw = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        const float mx = mraw == -INFINITY ? -INFINITY : mraw * sl2;
+        // the reference moves only when the maximum grew by more than the
+        // threshold, so O is seldom rescaled
+        const bool move = mx > m_ref + kRescaleThreshold;
+        const float m_new = move ? mx : m_ref;
+        const float corr = (move && m_ref != -INFINITY) ? ex2(m_ref - m_new) : 1.f;
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        m_ref = m_new;
+        // P V of the tile before reads P (kDP = 64) and writes O
+        if (j > it.lo) {
+          ok = wait(&sm.pv_done, (t - 1) & 1);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          tc_fence_after();
+        }
+        // pass 2: P = 2^(c s - m) as 16-bit pairs, row sum of the f32 values
+        const uint64_t neg_m = f2_splat(-m_use);
+        uint64_t la = f2_splat(0.f), lb = f2_splat(0.f);
+#pragma unroll
+        for (int c2 = 0; c2 < kN / 64; ++c2) {
+          uint32_t raw[2][32];
+          tmem_ld_32cols(t_s + c2 * 64, raw[0]);
+          tmem_ld_32cols(t_s + c2 * 64 + 32, raw[1]);
+          tmem_ld_wait();
+          if (kDP == 64 && c2 == kN / 64 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.s_free);
+          }
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2) {
+            const int c = c2 * 2 + h2;
+            float v[32];
+            scores(c, raw[h2], v);
+            uint32_t pw[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float a0, a1;
+              f2_unpack(f2_fma(f2_pack(v[i], v[i + 1]), sl2x2, neg_m), a0, a1);
+              const float p0 = ex2(a0), p1 = ex2(a1);
+              if (i & 2)
+                lb = f2_add(lb, f2_pack(p0, p1));
+              else
+                la = f2_add(la, f2_pack(p0, p1));
+              pw[i / 2] = Type<T>::pack(p0, p1);
+            }
+            tmem_st_16cols(t_p + c * 16, pw);
+          }
+        }
+        float la0, la1, lb0, lb1;
+        f2_unpack(la, la0, la1);
+        f2_unpack(lb, lb0, lb1);
+        l = l * corr + ((la0 + la1) + (lb0 + lb1));
+        if (j > it.lo && __any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll
+          for (int c = 0; c < kDP / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_16cols(t_o + c * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_st_16cols(t_o + c * 16, o);
+          }
+        }
+        if (mixed) {
+          ok = wait(&sm.v_full[t & 1], (t >> 1) & 1);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          zero_hidden_rows<kN, kDP>(sm.v[t & 1], words, threadIdx.x - 64, 128);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full);
+      }
+      if (!ok) break;
+      // ---- output: O / l and lse
+      const bool any = it.lo < it.hi;
+      if (any) {
+        ok = wait(&sm.pv_done, (t - 1) & 1);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc_fence_after();
+      }
+      const bool none = l == 0.f;  // (a NaN sum is not equal and passes through)
+      const float inv_l = none ? 0.f : 1.f / l;
+      const int64_t rows_all = (int64_t)sh.B * sh.Sq * sh.H;
+      const int64_t orow = ((int64_t)it.b * sh.Sq + qi) * sh.H + it.h;
+      const int64_t lrow = ((int64_t)it.b * sh.H + it.h) * sh.Sq + qi;
+#pragma unroll
+      for (int c = 0; c < kDP / 32; ++c) {
+        uint32_t o[32];
+        if (any) {
+          tmem_ld_32cols(t_o + c * 32, o);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          o[i] = any && !none ? __float_as_uint(__uint_as_float(o[i]) * inv_l) : 0u;
+        if (qi < sh.Sq) {
+          if (sh.splits == 1) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (c * 32 + q * 8 < sh.D)
+                *reinterpret_cast<uint4*>(out + orow * sh.D + c * 32 + q * 8) = make_uint4(
+                    Type<T>::pack(__uint_as_float(o[8 * q]), __uint_as_float(o[8 * q + 1])),
+                    Type<T>::pack(__uint_as_float(o[8 * q + 2]), __uint_as_float(o[8 * q + 3])),
+                    Type<T>::pack(__uint_as_float(o[8 * q + 4]), __uint_as_float(o[8 * q + 5])),
+                    Type<T>::pack(__uint_as_float(o[8 * q + 6]), __uint_as_float(o[8 * q + 7])));
+          } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (c * 32 + q * 4 < sh.D)
+                *reinterpret_cast<uint4*>(part_o + (it.split * rows_all + orow) * sh.D + c * 32 +
+                                          q * 4) =
+                    make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          }
+        }
+      }
+      if (qi < sh.Sq) {
+        if (sh.splits > 1)
+          part_lse[it.split * rows_all + lrow] = none ? -INFINITY : m_ref + log2f(l);
+        else if (lse2)
+          lse2[lrow] = none ? INFINITY : m_ref + log2f(l);
+      }
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<256>(tmem);
+  }
+}
+
+// ============================================================== mask packing
+// A CTA per sample: visible-key words and the end of the visible keys.
+__global__ void __launch_bounds__(256) pack_mask_kernel(const uint8_t* __restrict__ pad, int Sk,
+                                                        int nwords, uint32_t* __restrict__ words,
+                                                        int* __restrict__ vis_end) {
+  __shared__ int s_end[8];
+  pdl_wait();
+  pdl_trigger();
+  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int end = 0;
+#pragma unroll 4
+  for (int w = warp; w < nwords; w += 8) {
+    const int key = w * 32 + lane;
+    const uint32_t bits =
+        __ballot_sync(0xffffffffu, key < Sk && __ldg(pad + (int64_t)b * Sk + key) == 0);
+    if (lane == 0) words[(int64_t)b * nwords + w] = bits;
+    if (bits) end = w * 32 + 32 - __clz(bits);
+  }
+  if (lane == 0) s_end[warp] = end;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) end = max(end, s_end[w]);
+    vis_end[b] = end;
+  }
+}
+
+// ============================================================== backward
+// delta = rowsum(dO * O): kLanes lanes per row, 8 values each.
+template <typename T>
+__device__ __forceinline__ float dot8(uint4 a, uint4 b);
+template <>
+__device__ __forceinline__ float dot8<__nv_bfloat16>(uint4 a, uint4 b) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 u = unpack_bf16x2(x[i]), v = unpack_bf16x2(y[i]);
+    s = fmaf(u.x, v.x, fmaf(u.y, v.y, s));
+  }
+  return s;
+}
+template <>
+__device__ __forceinline__ float dot8<__half>(uint4 a, uint4 b) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&x[i]));
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&y[i]));
+    s = fmaf(u.x, v.x, fmaf(u.y, v.y, s));
+  }
+  return s;
+}
+struct Stride3 {
+  int64_t b, s, h;
+};
+// The backward's row statistics: {-lse2, -delta} of every query, [B, H, pitch]
+// with the pitch Sq rounded up to 64 so that a streamed tile's 64 pairs are one
+// aligned 512-byte copy. Rows past Sq hold {-inf, 0}: their P is 0.
+__host__ __device__ constexpr int stat_pitch(int Sq) { return (Sq + 63) / 64 * 64; }
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(256) cross_stats_kernel(const T* __restrict__ out,
+                                                          const T* __restrict__ dout, Stride3 ds,
+                                                          const float* __restrict__ lse2,
+                                                          float2* __restrict__ stats, int B, int Sq,
+                                                          int H, int D) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int kPer = 256 / kLanes;
+  const int part = threadIdx.x % kLanes, sub = threadIdx.x / kLanes;
+  const int pitch = stat_pitch(Sq);
+  const int64_t rows = (int64_t)B * pitch * H;
+  for (int64_t base = (int64_t)blockIdx.x * kPer; base < rows; base += (int64_t)gridDim.x * kPer) {
+    const int64_t row = base + sub;  // (b * pitch + i) * H + h
+    const int64_t bi = row / H;
+    const int h = (int)(row - bi * H);
+    const int64_t b = bi / pitch;
+    const int i = (int)(bi - b * pitch);
+    float s = 0.f;
+    if (row < rows && i < Sq && part * 8 < D)
+      s = dot8<T>(
+          __ldg(reinterpret_cast<const uint4*>(out + ((b * Sq + i) * H + h) * D + part * 8)),
+          __ldg(reinterpret_cast<const uint4*>(dout + b * ds.b + i * ds.s + h * ds.h + part * 8)));
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (row < rows && part == 0)
+      stats[(b * H + h) * pitch + i] =
+          make_float2(i < Sq ? -__ldg(lse2 + (b * H + h) * Sq + i) : -INFINITY, -s);
+  }
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// One kernel for both halves. kKeys false: rows are 128 queries (A1 = Q,
+// A2 = dO), the stream is K, V, acc1 = dS K. kKeys true: rows are 128 keys
+// (A1 = K, A2 = V), the stream is Q, dO of every query head that reads this
+// memory head, acc1 = dS^T Q, acc2 = P^T dO.
+// Warps: 0 TMA, 1 MMA, 2..5 and 6..9 two compute groups that take the streamed
+// tiles of 64 in turn: one group's exponentials run beside the tensor cores'
+// work for the other. TMEM: [S, dP] of two tiles at 0 and 128, acc1 at 256,
+// acc2 behind it; dS lies over S (kKeys: P over S, dS over dP).
+constexpr int kBN = 64;
+constexpr int kBwdThreads = 320;
+
+template <int kDP>
+struct BwdGeo {
+  static constexpr int kStages = kDP == 64 ? 4 : 3;
+  static constexpr int kABytes = kRows * kDP * 2;
+  static constexpr int kBBytes = kBN * kDP * 2;
+};
+template <int kDP>
+struct BwdSmem {
+  using G = BwdGeo<kDP>;
+  uint8_t a1[2][G::kABytes], a2[2][G::kABytes];
+  uint8_t b1[G::kStages][G::kBBytes], b2[G::kStages][G::kBBytes];
+  float2 stat[G::kStages][kBN];  // kKeys: the streamed queries' statistics
+  uint64_t a_full[2], a_empty[2], b_full[G::kStages], b_empty[G::kStages];
+  uint64_t s_full[2], ds_full[2], acc_full, acc_free, drain;
+  uint32_t tmem_base, abort;
+};
+struct BwdItem {
+  int row0, head, b, split, lo, hi;  // stream tiles [lo, hi); kKeys: tile index = group * n + tile
+  int first, n;                      // kKeys: first query tile, query tiles per head
+};
+template <bool kKeys>
+__device__ __forceinline__ BwdItem bwd_item(const Shape& s, int item, int n_rt) {
+  BwdItem it;
+  it.split = item % s.splits;
+  item /= s.splits;
+  const int heads = kKeys ? s.Hk : s.H;
+  const int n_bh = heads * s.B;
+  int rt = item / n_bh;
+  // heaviest first under a causal mask: the last queries, the first keys
+  if (!kKeys) rt = n_rt - 1 - rt;
+  const int bh = item % n_bh;
+  it.head = bh % heads;
+  it.b = bh / heads;
+  it.row0 = rt * kRows;
+  const int end = visible_end(s, it.b);
+  int nt;
+  it.first = 0;
+  it.n = 0;
+  if (kKeys) {
+    const int nq = (s.Sq + kBN - 1) / kBN;
+    it.first = s.causal ? min(it.row0 / kBN, nq) : 0;
+    it.n = nq - it.first;
+    nt = it.row0 < end ? s.G * it.n : 0;
+  } else {
+    nt = ((s.causal ? min(end, it.row0 + kRows) : end) + kBN - 1) / kBN;
+  }
+  it.lo = (int)((int64_t)nt * it.split / s.splits);
+  it.hi = (int)((int64_t)nt * (it.split + 1) / s.splits);
+  return it;
+}
+
+template <typename T>
+struct BwdOut {
+  T *o1, *o2;          // dQ, or dK and dV
+  Stride3 s1, s2;
+  float* part;         // [splits][1 or 2][rows][D] when splits > 1
+};
+
+template <typename T, int kDP, bool kKeys>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    cross_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1,
+                     const __grid_constant__ CUtensorMap tm_a2,
+                     const __grid_constant__ CUtensorMap tm_b1,
+                     const __grid_constant__ CUtensorMap tm_b2, const __grid_constant__ Shape sh,
+                     const float2* __restrict__ stats, const __grid_constant__ BwdOut<T> outs, int n_items, int n_rt) {
+  using Geo = BwdGeo<kDP>;
+  constexpr int kStages = Geo::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  BwdSmem<kDP>& sm = *reinterpret_cast<BwdSmem<kDP>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const Waiter wait{&sm.abort, sh.err};
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.a_full[i], 1);
+      mbar_init(&sm.a_empty[i], 1);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.ds_full[i], 4);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.b_full[i], 1);
+      mbar_init(&sm.b_empty[i], 1);
+    }
+    mbar_init(&sm.acc_full, 1);
+    mbar_init(&sm.acc_free, 8);
+    mbar_init(&sm.drain, 1);
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc<512>(&sm.tmem_base);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  const uint32_t t_acc1 = tmem + 256, t_acc2 = tmem + 256 + kDP;
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (elect_one_sync()) {
+      tma_prefetch_desc(&tm_a1);
+      tma_prefetch_desc(&tm_a2);
+      tma_prefetch_desc(&tm_b1);
+      tma_prefetch_desc(&tm_b2);
+      uint32_t n = 0, u = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+        const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
+        if (it.lo >= it.hi) continue;
+        if (!(ok = wait(&sm.a_empty[n & 1], ((n >> 1) & 1) ^ 1))) break;
+        mbar_arrive_expect_tx(&sm.a_full[n & 1], 2 * Geo::kABytes);
+        load_tile<kRows, kDP>(sm.a1[n & 1], &tm_a1, &sm.a_full[n & 1], it.row0, it.head, it.b);
+        load_tile<kRows, kDP>(sm.a2[n & 1], &tm_a2, &sm.a_full[n & 1], it.row0, it.head, it.b);
+        ++n;
+        for (int j = it.lo; j < it.hi; ++j, ++u) {
+          const uint32_t st = u % kStages;
+          if (!(ok = wait(&sm.b_empty[st], ((u / kStages) & 1) ^ 1))) break;
+          const int row = kKeys ? (it.first + j % it.n) * kBN : j * kBN;
+          const int head = kKeys ? it.head * sh.G + j / it.n : it.head / sh.G;
+          mbar_arrive_expect_tx(&sm.b_full[st],
+                                2 * Geo::kBBytes + (kKeys ? (uint32_t)sizeof(sm.stat[st]) : 0u));
+          if (kKeys)
+            bulk_load(sm.stat[st], stats + ((int64_t)it.b * sh.H + head) * stat_pitch(sh.Sq) + row,
+                      sizeof(sm.stat[st]), &sm.b_full[st]);
+          load_tile<kBN, kDP>(sm.b1[st], &tm_b1, &sm.b_full[st], row, head, it.b);
+          load_tile<kBN, kDP>(sm.b2[st], &tm_b2, &sm.b_full[st], row, head, it.b);
+        }
+      }
+      if (!ok) {
+        for (uint32_t i = 0; i < 2; ++i) settle(&sm.a_full[i], (n + 1 - i) / 2);
+        for (uint32_t i = 0; i < kStages; ++i)
+          settle(&sm.b_full[i], (u + kStages - 1 - i) / kStages);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (elect_one_sync()) {
+      constexpr uint32_t id_s = idesc(Type<T>::kIdesc, kRows, kBN, 0);
+      constexpr uint32_t id_acc = idesc(Type<T>::kIdesc, kRows, kDP, 1);
+      uint32_t n = 0, u = 0, m = 0;  // items started, tiles, items whose products began
+      bool ok = true, issued = false;
+      bool behind = false, behind_first = false, behind_last = false;
+      auto issue_acc = [&](uint32_t w, bool first, bool last) -> bool {
+        if (first) {  // the item before has been read out
+          if (!wait(&sm.acc_free, (m & 1) ^ 1)) return false;
+          ++m;
+        }
+        if (!wait(&sm.ds_full[w & 1], (w >> 1) & 1)) return false;
+        tc_fence_after();
+        const uint32_t t_s = tmem + (w & 1) * 128u, st = w % kStages;
+        if (kKeys) {
+          mma_cols<kBN, kDP>(t_acc2, t_s, smem_u32(sm.b2[st]), id_acc, !first);
+          mma_cols<kBN, kDP>(t_acc1, t_s + 64, smem_u32(sm.b1[st]), id_acc, !first);
+        } else {
+          mma_cols<kBN, kDP>(t_acc1, t_s, smem_u32(sm.b1[st]), id_acc, !first);
+        }
+        umma_commit(&sm.b_empty[st]);
+        if (last) umma_commit(&sm.acc_full);
+        return true;
+      };
+      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+        const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
+        if (it.lo >= it.hi) continue;
+        if (!(ok = wait(&sm.a_full[n & 1], (n >> 1) & 1))) break;
+        const uint32_t a1 = smem_u32(sm.a1[n & 1]), a2 = smem_u32(sm.a2[n & 1]);
+        for (int j = it.lo; j < it.hi; ++j, ++u) {
+          const uint32_t st = u % kStages;
+          if (!(ok = wait(&sm.b_full[st], (u / kStages) & 1))) break;
+          tc_fence_after();
+          // this buffer's last product (tile u - 2) was issued before: in order
+          const uint32_t t_s = tmem + (u & 1) * 128u;
+          mma_rows<kRows, kBN, kDP>(t_s, a1, smem_u32(sm.b1[st]), id_s);
+          mma_rows<kRows, kBN, kDP>(t_s + 64, a2, smem_u32(sm.b2[st]), id_s);
+          issued = true;
+          umma_commit(&sm.s_full[u & 1]);
+          if (j == it.hi - 1) umma_commit(&sm.a_empty[n & 1]);
+          if (behind && !(ok = issue_acc(u - 1, behind_first, behind_last))) break;
+          behind = true;
+          behind_first = j == it.lo;
+          behind_last = j == it.hi - 1;
+        }
+        ++n;
+      }
+      if (ok && behind) ok = issue_acc(u - 1, behind_first, behind_last);
+      if (!ok && issued) {
+        umma_commit(&sm.drain);
+        settle(&sm.drain, 1);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ compute
+    const int group = (warp - 2) >> 2;
+    const int r = (warp & 3) * 32 + lane;  // row within the tile
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + (uint32_t)group * 128u;
+    const uint64_t sl2x2 = f2_splat(sh.scale * kLog2e);
+    constexpr float kShift = kKeys ? Type<T>::kShift : 0.f;
+    const float unshift = exp2f(-kShift);
+    uint32_t u = 0, n = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+      const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
+      const int row = it.row0 + r;
+      const bool any = it.lo < it.hi;
+      // row statistics (queries), or the row's visibility (keys)
+      uint64_t row_lse = f2_splat(-INFINITY), row_delta = f2_splat(0.f);  // negated
+      bool row_ok = true;
+      if (!kKeys) {
+        if (any && row < sh.Sq) {
+          const float2 v =
+              __ldg(stats + ((int64_t)it.b * sh.H + it.head) * stat_pitch(sh.Sq) + row);
+          row_lse = f2_splat(v.x);
+          row_delta = f2_splat(v.y);
+        }
+      } else {
+        row_ok = row < sh.Sk;
+        if (row_ok && sh.words)
+          row_ok = (__ldg(sh.words + (int64_t)it.b * sh.nwords + row / 32) >> (row & 31)) & 1u;
+      }
+      const bool rows_ok = __all_sync(0xffffffffu, row_ok);
+      // tiles of this group: u counts the CTA's tiles
+      const uint32_t u0 = u;
+      for (int j = it.lo + (int)((u0 ^ (uint32_t)group) & 1u); j < it.hi; j += 2) {
+        const uint32_t w = u0 + (uint32_t)(j - it.lo), stage = w % kStages;
+        const int col0 = kKeys ? (it.first + j % it.n) * kBN : j * kBN;
+        uint32_t words[2] = {0xffffffffu, 0xffffffffu};
+        if (!kKeys) tile_words<kBN>(sh, it.b, col0, words);
+        const bool diag = sh.causal && (kKeys ? col0 < it.row0 + kRows - 1
+                                              : col0 + kBN - 1 > it.row0);
+        // the statistics came with the tile (already complete: S was computed)
+        ok = !kKeys || wait(&sm.b_full[stage], (w / kStages) & 1);
+        ok = ok && wait(&sm.s_full[group], (w >> 1) & 1);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc_fence_after();
+        // 32 columns: P and dS as 16-bit pairs. Hidden pairs are replaced by
+        // zero, whatever the products gave.
+        auto columns = [&](int c, auto masked) {
+          uint32_t rs[32], rd[32];
+          tmem_ld_32cols(t_s + c * 32, rs);
+          tmem_ld_32cols(t_s + 64 + c * 32, rd);
+          tmem_ld_wait();
+          uint32_t pk[16], dk[16];
+          const int lim = row - (col0 + c * 32);  // causal: key <= query
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            uint64_t nl = row_lse, nd = row_delta;
+            if (kKeys) {
+              const float4 v = *reinterpret_cast<const float4*>(&sm.stat[stage][c * 32 + i]);
+              nl = f2_pack(v.x, v.z);
+              nd = f2_pack(v.y, v.w);
+            }
+            uint64_t e = f2_fma(f2_pack(__uint_as_float(rs[i]), __uint_as_float(rs[i + 1])), sl2x2, nl);
+            if (kShift != 0.f) e = f2_add(e, f2_splat(kShift));
+            float p0, p1, d0, d1;
+            f2_unpack(e, p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            uint64_t d = f2_add(f2_pack(__uint_as_float(rd[i]), __uint_as_float(rd[i + 1])), nd);
+            if (kShift != 0.f) d = f2_mul(d, f2_splat(unshift));
+            f2_unpack(f2_mul(f2_pack(p0, p1), d), d0, d1);
+            if (decltype(masked)::value) {
+              bool v0 = row_ok && ((words[c] >> i) & 1u), v1 = row_ok && ((words[c] >> (i + 1)) & 1u);
+              if (diag) {
+                v0 = v0 && (kKeys ? i >= lim : i <= lim);
+                v1 = v1 && (kKeys ? i + 1 >= lim : i + 1 <= lim);
+              }
+              p0 = v0 ? p0 : 0.f;
+              p1 = v1 ? p1 : 0.f;
+              d0 = v0 ? d0 : 0.f;
+              d1 = v1 ? d1 : 0.f;
+            }
+            if (kKeys) pk[i / 2] = Type<T>::pack(p0, p1);
+            dk[i / 2] = Type<T>::pack(d0, d1);
+          }
+          if (kKeys) tmem_st_16cols(t_s + c * 16, pk);
+          tmem_st_16cols(t_s + (kKeys ? 64u : 0u) + c * 16, dk);
+        };
+        if (diag || !rows_ok || (words[0] & words[1]) != 0xffffffffu) {
+          columns(0, std::true_type{});
+          columns(1, std::true_type{});
+        } else {
+          columns(0, std::false_type{});
+          columns(1, std::false_type{});
+        }
+        if (!kKeys && sh.words && (words[0] & words[1]) != 0xffffffffu)
+          zero_hidden_rows<kBN, kDP>(sm.b1[stage], words, (warp & 3) * 32 + lane, 128);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.ds_full[group]);
+      }
+      if (!ok) break;
+      u = u0 + (uint32_t)max(0, it.hi - it.lo);
+      // ---- read the accumulators out
+      if (any) {
+        ok = wait(&sm.acc_full, n & 1);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc_fence_after();
+        ++n;
+      }
+      const int rows_n = kKeys ? sh.Sk : sh.Sq, heads = kKeys ? sh.Hk : sh.H;
+      const int64_t flat = ((int64_t)it.b * rows_n + row) * heads + it.head;
+      const int64_t rows_all = (int64_t)sh.B * rows_n * heads;
+      // queries: each group takes half of dQ's columns; keys: group 0 takes dV,
+      // group 1 dK
+      constexpr int kCols = kKeys ? kDP : kDP / 2;
+      const bool second = kKeys && group == 0;
+      const uint32_t t_a = (second ? t_acc2 : t_acc1) + lanes + (kKeys ? 0 : group * kCols);
+      const float f = second ? unshift : sh.scale;
+      T* dst = second ? outs.o2 : outs.o1;
+      const Stride3& st3 = second ? outs.s2 : outs.s1;
+      dst += it.b * st3.b + (int64_t)row * st3.s + it.head * st3.h;
+      float* part = outs.part + ((int64_t)it.split * (kKeys ? 2 : 1) + (second ? 1 : 0)) * rows_all * sh.D +
+                    flat * sh.D;
+#pragma unroll
+      for (int c = 0; c < kCols / 32; ++c) {
+        uint32_t o[32];
+        if (any) {
+          tmem_ld_32cols(t_a + c * 32, o);
+          tmem_ld_wait();
+        }
+        const int col0 = (kKeys ? 0 : group * kCols) + c * 32;
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = any ? __uint_as_float(o[i]) * f : 0.f;
+        if (row < rows_n) {
+          if (sh.splits == 1) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (col0 + q * 8 < sh.D)
+                *reinterpret_cast<uint4*>(dst + col0 + q * 8) =
+                    make_uint4(Type<T>::pack(v[8 * q], v[8 * q + 1]),
+                               Type<T>::pack(v[8 * q + 2], v[8 * q + 3]),
+                               Type<T>::pack(v[8 * q + 4], v[8 * q + 5]),
+                               Type<T>::pack(v[8 * q + 6], v[8 * q + 7]));
+          } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (col0 + q * 4 < sh.D)
+                *reinterpret_cast<float4*>(part + col0 + q * 4) =
+                    make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          }
+        }
+      }
+      if (any) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.acc_free);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<512>(tmem);
+  }
+}
+
+// out = the sum of the pieces, in order: part [splits][n_out][rows][D], rows
+// (b, i, h). Eight columns per thread.
+template <typename T>
+__global__ void __launch_bounds__(256) cross_sum_kernel(const __grid_constant__ BwdOut<T> outs,
+                                                        int splits, int n_out, int B, int S, int H,
+                                                        int D) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t rows = (int64_t)B * S * H, vec = D / 8, total = rows * vec * n_out;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t which = i / (rows * vec), rest = i - which * rows * vec;
+    const int64_t row = rest / vec;
+    const int col = (int)(rest - row * vec) * 8;
+    float a[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      const float4* p = reinterpret_cast<const float4*>(
+          outs.part + (((int64_t)s * n_out + which) * rows + row) * D + col);
+      const float4 x = p[0], y = p[1];
+      a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w;
+      a[4] += y.x; a[5] += y.y; a[6] += y.z; a[7] += y.w;
+    }
+    const int64_t bi = row / H, h = row - bi * H, b = bi / S, s = bi - b * S;
+    const Stride3& st = which ? outs.s2 : outs.s1;
+    *reinterpret_cast<uint4*>((which ? outs.o2 : outs.o1) + b * st.b + s * st.s + h * st.h + col) =
+        make_uint4(Type<T>::pack(a[0], a[1]), Type<T>::pack(a[2], a[3]), Type<T>::pack(a[4], a[5]),
+                   Type<T>::pack(a[6], a[7]));
+  }
+}
+
+// ============================================================== host
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// cuTensorMapEncodeTiled is a driver call: it needs a context current on the
+// calling thread (an autograd thread may not have one before its first launch).
+EncodeTiledFn encode_fn() {
+  thread_local int bound = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && bound != dev) {
+    cudaSetDevice(dev);
+    bound = dev;
+  }
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// Map {D, position, head, batch} of a strided 16-bit tensor; box = 64 columns x
+// `rows` positions. The stride of a dimension of one does not matter: any valid
+// value goes.
+bool make_map(CUtensorMap* m, const void* base, bool half, int D, int S, int heads, int B,
+              const int64_t (&st)[3], int rows) {
+  auto enc = encode_fn();
+  if (!enc) return false;
+  const int n[3] = {S, heads, B};
+  const int64_t e[3] = {st[1], st[2], st[0]};
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)heads, (cuuint64_t)B};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) {
+    const int64_t bytes = n[i] > 1 ? e[i] * 2 : 256;
+    if (bytes <= 0 || bytes % 16 || bytes >= ((int64_t)1 << 40)) return false;
+    strides[i] = (cuuint64_t)bytes;
+  }
+  cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  return enc(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+             const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Shared-memory opt-in, once per kernel and device.
+template <typename K>
+cudaError_t opt_in(K kernel, int smem, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                             cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess) done.fetch_or(bit);
+  return e;
+}
+
+Shape shape_of(const CrossAttnArgs& a, int splits) {
+  Shape s{};
+  s.B = a.B; s.Sq = a.Sq; s.Sk = a.Sk; s.H = a.H; s.Hk = a.Hk; s.G = a.H / a.Hk; s.D = a.D;
+  s.causal = a.causal;
+  s.splits = splits;
+  s.scale = a.scale;
+  s.words = a.key_pad ? a.words : nullptr;
+  s.vis_end = a.key_pad ? a.vis_end : nullptr;
+  s.nwords = (a.Sk + 31) / 32;
+  s.err = default_err_word();
+  return s;
+}
+
+bool bad_shape(const CrossAttnArgs& a) {
+  return a.B <= 0 || a.Sq <= 0 || a.Sk <= 0 || a.H <= 0 || a.Hk <= 0 || a.H % a.Hk || a.D <= 0 ||
+         a.D > 128 || a.D % 8 || (a.causal && a.Sq != a.Sk) || !(a.scale > 0.f) ||
+         (a.key_pad && !cross_attn_is_few(a) && (!a.words || !a.vis_end));
+}
+
+// Pieces of the streamed axis: fewer items than places take as many pieces as
+// fill them, as long as a piece keeps four tiles (the pieces cost a join).
+int pieces(int64_t items, int64_t places, int64_t tiles) {
+  if (items >= places) return 1;
+  return (int)std::max<int64_t>(1, std::min(places / items, tiles / 4));
+}
+int64_t row_tiles(int n) { return ((int64_t)n + kRows - 1) / kRows; }
+
+int fwd_splits(const CrossAttnArgs& a) {
+  const int kn = a.D <= 64 ? 128 : 64;
+  return pieces(row_tiles(a.Sq) * a.H * a.B, 2ll * num_sms(), ((int64_t)a.Sk + kn - 1) / kn);
+}
+int dq_splits(const CrossAttnArgs& a) {
+  return pieces(row_tiles(a.Sq) * a.H * a.B, num_sms(), ((int64_t)a.Sk + kBN - 1) / kBN);
+}
+int dkv_splits(const CrossAttnArgs& a) {
+  return pieces(row_tiles(a.Sk) * a.Hk * a.B, num_sms(),
+                ((int64_t)a.Sq + kBN - 1) / kBN * (a.H / a.Hk));
+}
+
+template <typename T, int kDP>
+cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
+  const int splits = fwd_splits(a);
+  const int64_t rows = (int64_t)a.B * a.Sq * a.H;
+  if (splits > 1 && !a.partials) return cudaErrorInvalidValue;
+  constexpr int kn = FwdGeo<kDP>::kN;
+  CUtensorMap mq, mk, mv;
+  if (!make_map(&mq, a.q, a.half, a.D, a.Sq, a.H, a.B, a.q_st, kRows) ||
+      !make_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kn) ||
+      !make_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kn))
+    return cudaErrorInvalidValue;
+  static std::atomic<uint64_t> done{0};
+  const int smem = (int)sizeof(FwdSmem<kDP>) + 1024;
+  auto kernel = cross_fwd_kernel<T, kDP>;
+  cudaError_t e = opt_in(kernel, smem, done);
+  if (e != cudaSuccess) return e;
+  const int n_qt = (int)row_tiles(a.Sq);
+  const int64_t items = (int64_t)n_qt * a.H * a.B * splits;
+  if (items > 0x7fffffff - 4096) return cudaErrorInvalidValue;
+  const int grid = (int)std::min<int64_t>(items, 2ll * num_sms());
+  e = launch_pdl(kernel, dim3(grid), dim3(kFwdThreads), smem, st, mq, mk, mv, shape_of(a, splits),
+                 (T*)a.out, a.lse2, a.partials, a.partials + splits * rows * a.D, (int)items, n_qt);
+  if (e != cudaSuccess) return e;
+  note_launch();
+  return splits > 1 ? launch_cross_attn_join(a, splits, st) : cudaGetLastError();
+}
+
+template <typename T, int kDP, bool kKeys>
+cudaError_t run_bwd_half(const CrossAttnArgs& a, cudaStream_t st) {
+  const int splits = kKeys ? dkv_splits(a) : dq_splits(a);
+  if (splits > 1 && !a.partials) return cudaErrorInvalidValue;
+  const int rb = kRows, cb = kBN;
+  CUtensorMap mq, mk, mv, mo;
+  if (!make_map(&mq, a.q, a.half, a.D, a.Sq, a.H, a.B, a.q_st, kKeys ? cb : rb) ||
+      !make_map(&mo, a.dout, a.half, a.D, a.Sq, a.H, a.B, a.do_st, kKeys ? cb : rb) ||
+      !make_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kKeys ? rb : cb) ||
+      !make_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kKeys ? rb : cb))
+    return cudaErrorInvalidValue;
+  static std::atomic<uint64_t> done{0};
+  constexpr int smem = (int)sizeof(BwdSmem<kDP>) + 1024;
+  static_assert(smem <= 227 * 1024, "shared memory");
+  auto kernel = cross_bwd_kernel<T, kDP, kKeys>;
+  cudaError_t e = opt_in(kernel, smem, done);
+  if (e != cudaSuccess) return e;
+  const int S = kKeys ? a.Sk : a.Sq, heads = kKeys ? a.Hk : a.H;
+  const int n_rt = (int)row_tiles(S);
+  const int64_t items = (int64_t)n_rt * heads * a.B * splits;
+  if (items > 0x7fffffff - 4096) return cudaErrorInvalidValue;
+  BwdOut<T> o{};
+  auto s3 = [](const int64_t (&v)[3]) { return Stride3{v[0], v[1], v[2]}; };
+  o.o1 = (T*)(kKeys ? a.dk : a.dq);
+  o.s1 = kKeys ? s3(a.dk_st) : s3(a.dq_st);
+  o.o2 = kKeys ? (T*)a.dv : o.o1;
+  o.s2 = kKeys ? s3(a.dv_st) : o.s1;
+  o.part = a.partials;
+  const int grid = (int)std::min<int64_t>(items, num_sms());
+  e = launch_pdl(kernel, dim3(grid), dim3(kBwdThreads), smem, st, kKeys ? mk : mq, kKeys ? mv : mo,
+                 kKeys ? mq : mk, kKeys ? mo : mv, shape_of(a, splits), (const float2*)a.stats, o, (int)items, n_rt);
+  if (e != cudaSuccess) return e;
+  note_launch();
+  if (splits > 1) {
+    const int n_out = kKeys ? 2 : 1;
+    const int64_t total = (int64_t)a.B * S * heads * (a.D / 8) * n_out;
+    e = launch_pdl(cross_sum_kernel<T>,
+                   dim3((unsigned)std::min<int64_t>((total + 255) / 256, num_sms() * 8ll)), dim3(256),
+                   0, st, o, splits, n_out, a.B, S, heads, a.D);
+    if (e != cudaSuccess) return e;
+    note_launch();
+  }
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t run_stats(const CrossAttnArgs& a, cudaStream_t st) {
+  const int64_t rows = (int64_t)a.B * stat_pitch(a.Sq) * a.H;
+  const int per = a.D <= 64 ? 32 : 16;
+  const dim3 grid((unsigned)std::min<int64_t>((rows + per - 1) / per, num_sms() * 16ll));
+  const Stride3 ds{a.do_st[0], a.do_st[1], a.do_st[2]};
+  auto k = a.D <= 64 ? cross_stats_kernel<T, 8> : cross_stats_kernel<T, 16>;
+  cudaError_t e = launch_pdl(k, grid, dim3(256), 0, st, (const T*)a.out, (const T*)a.dout, ds,
+                             (const float*)a.lse2, (float2*)a.stats, a.B, a.Sq, a.H, a.D);
+  if (e != cudaSuccess) return e;
+  note_launch();
+  return cudaGetLastError();
+}
+
+template <typename T, int kDP>
+cudaError_t run_bwd(const CrossAttnArgs& a, cudaStream_t st) {
+  cudaError_t e = run_stats<T>(a, st);
+  if (e == cudaSuccess) e = run_bwd_half<T, kDP, false>(a, st);
+  if (e == cudaSuccess) e = run_bwd_half<T, kDP, true>(a, st);
+  return e;
+}
+
+}  // namespace
+
+int64_t cross_attn_stats_floats(const CrossAttnArgs& a) {
+  return 2ll * a.B * a.H * stat_pitch(a.Sq);
+}
+int64_t cross_attn_fwd_partials(const CrossAttnArgs& a) {
+  const int splits = cross_attn_is_few(a) ? cross_attn_few_splits(a) : fwd_splits(a);
+  return splits > 1 ? (int64_t)splits * a.B * a.Sq * a.H * (a.D + 1) : 0;
+}
+// The two halves run one after the other and use the same scratch.
+int64_t cross_attn_bwd_partials(const CrossAttnArgs& a) {
+  const int sq = dq_splits(a), sk = dkv_splits(a);
+  const int64_t nq = sq > 1 ? (int64_t)sq * a.B * a.Sq * a.H * a.D : 0;
+  const int64_t nk = sk > 1 ? (int64_t)sk * 2 * a.B * a.Sk * a.Hk * a.D : 0;
+  return std::max(nq, nk);
+}
+
+cudaError_t launch_cross_attn_pack_mask(const CrossAttnArgs& a, cudaStream_t st) {
+  if (!a.key_pad || !a.words || !a.vis_end || a.B <= 0 || a.Sk <= 0) return cudaErrorInvalidValue;
+  cudaError_t e = launch_pdl(pack_mask_kernel, dim3(a.B), dim3(256), 0, st, a.key_pad, a.Sk,
+                             (a.Sk + 31) / 32, a.words, a.vis_end);
+  if (e != cudaSuccess) return e;
+  note_launch();
+  return cudaGetLastError();
+}
+
+cudaError_t launch_cross_attn_fwd(const CrossAttnArgs& a, cudaStream_t st) {
+  if (bad_shape(a)) return cudaErrorInvalidValue;
+  if (cross_attn_is_few(a)) return launch_cross_attn_few(a, st);
+  if (a.D <= 64) return a.half ? run_fwd<__half, 64>(a, st) : run_fwd<__nv_bfloat16, 64>(a, st);
+  return a.half ? run_fwd<__half, 128>(a, st) : run_fwd<__nv_bfloat16, 128>(a, st);
+}
+
+cudaError_t launch_cross_attn_bwd(const CrossAttnArgs& a, cudaStream_t st) {
+  if (bad_shape(a) || !a.lse2 || !a.stats || (a.key_pad && (!a.words || !a.vis_end)))
+    return cudaErrorInvalidValue;
+  if (a.D <= 64) return a.half ? run_bwd<__half, 64>(a, st) : run_bwd<__nv_bfloat16, 64>(a, st);
+  return a.half ? run_bwd<__half, 128>(a, st) : run_bwd<__nv_bfloat16, 128>(a, st);
+}
+
+}  // namespace flodl

@@ -1,0 +1,57 @@
+// Host interface of attention with queries, keys and values in tensors of
+// their own (cross_attn.cu, cross_attn_few.cu).
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "gemm_sm100.h"
+
+namespace flodl {
+
+// Queries [B, Sq, H, D], keys and values [B, Sk, Hk, D], output and its
+// gradient likewise; strides in elements for (batch, position, head), the last
+// dimension contiguous, every stride of a dimension longer than one a multiple
+// of 8 and every base address of 16 bytes. D is a multiple of 8 up to 128.
+struct CrossAttnArgs {
+  const void *q = nullptr, *k = nullptr, *v = nullptr;
+  int64_t q_st[3] = {}, k_st[3] = {}, v_st[3] = {};
+  void* out = nullptr;                 // [B, Sq, H, D] contiguous (backward: the forward's output)
+  float* lse2 = nullptr;               // [B, H, Sq] base-2 log-sum-exp, +inf for a row without a key
+  const uint8_t* key_pad = nullptr;    // [B, Sk] contiguous, nonzero = hidden (nullable)
+  // from cross_attn_pack_mask, only with key_pad and outside the few-row form
+  uint32_t* words = nullptr;           // [B, ceil(Sk / 32)] bit per visible key
+  int* vis_end = nullptr;              // [B] index past the last visible key
+  // backward
+  const void* dout = nullptr;
+  int64_t do_st[3] = {};
+  float* stats = nullptr;              // scratch of cross_attn_stats_floats
+  void *dq = nullptr, *dk = nullptr, *dv = nullptr;
+  int64_t dq_st[3] = {}, dk_st[3] = {}, dv_st[3] = {};
+  int B = 0, Sq = 0, Sk = 0, H = 0, Hk = 0, D = 0;
+  bool causal = false;                 // needs Sq == Sk
+  bool half = false;                   // f16 instead of bf16
+  float scale = 1.f;
+  float* partials = nullptr;           // scratch of the sizes below (nullable where 0)
+};
+
+constexpr int kCrossFewRows = 16;  // query rows per memory head of the few-row form
+
+// Whether the forward takes the few-row form: all query rows of a memory head
+// (Sq * H / Hk) fit one 16-row tensor-core tile.
+bool cross_attn_is_few(const CrossAttnArgs& a);
+// Floats of scratch that the forward / backward needs in `partials` (0: none).
+int64_t cross_attn_stats_floats(const CrossAttnArgs& a);
+int64_t cross_attn_fwd_partials(const CrossAttnArgs& a);
+int64_t cross_attn_bwd_partials(const CrossAttnArgs& a);
+
+cudaError_t launch_cross_attn_pack_mask(const CrossAttnArgs& a, cudaStream_t st);
+cudaError_t launch_cross_attn_fwd(const CrossAttnArgs& a, cudaStream_t st);
+cudaError_t launch_cross_attn_bwd(const CrossAttnArgs& a, cudaStream_t st);
+
+// Pieces shared by the two files.
+int cross_attn_few_splits(const CrossAttnArgs& a);
+cudaError_t launch_cross_attn_few(const CrossAttnArgs& a, cudaStream_t st);
+// out = the partial results of `splits` key ranges joined by their lse.
+cudaError_t launch_cross_attn_join(const CrossAttnArgs& a, int splits, cudaStream_t st);
+
+}  // namespace flodl

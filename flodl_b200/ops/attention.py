@@ -15,6 +15,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from ._common import C, use_kernels
 
@@ -114,3 +115,124 @@ def scaled_dot_product_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     if dropout_p > 0:
         p = F.dropout(p, dropout_p)
     return torch.matmul(p, v)
+
+
+# ----------------------------------------------------------------- separate q, k, v
+def _tma_ready(t: torch.Tensor) -> torch.Tensor:
+    """A [B, S, heads, D] tensor the tile loads can read in place - contiguous
+    last dimension, other strides positive multiples of 16 bytes, 16-byte
+    aligned - or a contiguous copy."""
+    s = t.stride()
+    if s[3] == 1 and t.data_ptr() % 16 == 0:
+        n = t.shape
+        for i in range(3):
+            if n[i] != 1 and (s[i] % 8 or s[i] <= 0):
+                break
+        else:
+            return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 and t.stride(3) == 1 else t.clone(
+        memory_format=torch.contiguous_format)
+
+
+class _CrossAttnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, key_padding, causal, scale):
+        q, k, v = _tma_ready(q), _tma_ready(k), _tma_ready(v)
+        out, lse, bits = C().cross_attn_fwd(q, k, v, key_padding, causal, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, key_padding, bits)
+        ctx.consts = (causal, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, key_padding, bits = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+        C().cross_attn_bwd(_tma_ready(dout.to(q.dtype)), q, k, v, out, lse, key_padding, bits,
+                           *ctx.consts, dq, dk, dv)
+        return dq, dk, dv, None, None, None
+
+
+def _cross_composed(q, k, v, key_padding, causal, scale):
+    """The explicit form in the inputs' precision, at least f32."""
+    B, Sq, H, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    work = torch.float64 if q.dtype == torch.float64 else torch.float32
+    qh, kh, vh = (t.to(work).transpose(1, 2) for t in (q, k, v))
+    if key_padding is not None:  # what a hidden position holds has no effect
+        hidden = key_padding[:, None, :, None]
+        kh, vh = kh.masked_fill(hidden, 0.0), vh.masked_fill(hidden, 0.0)
+    if Hk != H:
+        kh, vh = kh.repeat_interleave(H // Hk, 1), vh.repeat_interleave(H // Hk, 1)
+    s = torch.matmul(qh, kh.transpose(-1, -2)) * scale
+    if key_padding is not None:
+        s = s.masked_fill(key_padding[:, None, None, :], float("-inf"))
+    if causal:
+        i = torch.arange(Sq, device=q.device)
+        s = s.masked_fill(i[None, :] > i[:, None], float("-inf"))
+    if Sk:
+        m = s.detach().amax(-1, keepdim=True)
+        s = s - m.masked_fill(m == float("-inf"), 0.0)
+    e = torch.exp(s)
+    total = e.sum(-1, keepdim=True)
+    o = torch.matmul(e, vh) / total.masked_fill(total == 0, 1.0)
+    return o.transpose(1, 2).to(q.dtype).contiguous()
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                    key_padding: Optional[torch.Tensor] = None, causal: bool = False,
+                    scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of ``q [B, Sq, H, D]`` over a memory ``k, v [B, Sk, Hk, D]`` of
+    another length: ``softmax(scale * q k^T) v``, token-major like
+    :func:`attention_packed`, returned contiguous as ``[B, Sq, H, D]``.
+
+    * H is a multiple of Hk; query head h reads memory head ``h // (H // Hk)``.
+    * ``key_padding`` (bool ``[B, Sk]``, True = hidden key) hides positions of
+      the memory; what they hold, NaN included, has no effect. A query that
+      sees no key gives zeros, and no gradient.
+    * ``causal`` (equal lengths only) lets query i see keys 0..i.
+    * ``scale`` is positive, ``1 / sqrt(D)`` by default.
+
+    CUDA bf16 and f16 inputs with D a multiple of 8 up to 128 run the sm_100a
+    kernels: views with 16-byte strides (a packed key/value projection's halves,
+    head-major tensors transposed to this layout) are read in place, others are
+    copied. Up to 16 query rows per memory head (``Sq * H / Hk``; the single
+    tokens of serving) take a form that streams the memory once. Scores and
+    sums are f32, probabilities are rounded to the inputs' type for the
+    products. Gradients are the same from run to run. Other inputs run the
+    composed form in f32 or f64.
+    """
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"cross_attention takes [B, S, heads, D] tensors (got {tuple(q.shape)} and "
+                         f"{tuple(k.shape)})")
+    B, Sq, H, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape:
+        raise ValueError(f"keys {tuple(k.shape)} and values {tuple(v.shape)} differ")
+    if k.shape[0] != B or k.shape[3] != D or D == 0:
+        raise ValueError(f"queries {tuple(q.shape)} and keys {tuple(k.shape)} differ in batch or "
+                         "head size")
+    if H == 0 or Hk == 0 or H % Hk:
+        raise ValueError(f"{H} query heads are not a multiple of {Hk} memory heads")
+    if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device
+            and q.dtype.is_floating_point):
+        raise ValueError("queries, keys and values must be floating-point tensors of one dtype and "
+                         "device")
+    if key_padding is not None and (key_padding.dtype != torch.bool or key_padding.shape != (B, Sk)
+                                    or key_padding.device != q.device):
+        raise ValueError(f"key_padding must be bool [{B}, {Sk}] on {q.device}")
+    if causal and Sq != Sk:
+        raise ValueError(f"causal attention needs equal lengths (got {Sq} and {Sk})")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"scale must be positive and finite (got {scale})")
+    if not (use_kernels(q) and q.dtype in (torch.bfloat16, torch.float16) and D % 8 == 0 and D <= 128
+            and B and Sq and Sk):
+        return _cross_composed(q, k, v, key_padding, causal, scale)
+    if key_padding is not None:
+        key_padding = key_padding.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _CrossAttnFn.apply(q, k, v, key_padding, bool(causal), scale)
+    return C().cross_attn_fwd(_tma_ready(q), _tma_ready(k), _tma_ready(v), key_padding, bool(causal),
+                              scale, False)[0]
