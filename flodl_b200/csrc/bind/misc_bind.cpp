@@ -124,6 +124,7 @@ flodl::QkNormRopeArgs qk_args(const Tensor& q, const Tensor& k, const optional<T
                  pos->size(0) == B && pos->size(1) == S && pos->device() == q.device(),
              "qk_norm_rope: positions must be int64 [B, S]");
     a.pos = pos->data_ptr<int64_t>();
+    a.pos_stride = S;
   } else if (a.R > 0) {
     FL_CHECK(offset >= 0 && offset <= a.table_rows - S, "qk_norm_rope: positions ", offset, " to ",
              offset + S - 1, " outside the tables' ", a.table_rows, " rows");
@@ -185,7 +186,7 @@ void qk_norm_rope_bwd(const Tensor& dyq, const Tensor& dyk, const Tensor& q, con
   Tensor partials;
   if (a.dwq || a.dwk) {
     a.partial_rows = flodl::qk_norm_rope_partial_rows(a);
-    partials = at::empty({a.partial_rows, 2, q.size(3)}, q.options().dtype(at::kFloat));
+    partials = at::empty({a.partial_rows, q.size(3)}, q.options().dtype(at::kFloat));
     a.partials = partials.data_ptr<float>();
   }
   FL_CUDA_OK(flodl::launch_qk_norm_rope_bwd(a, cur_stream()));

@@ -60,12 +60,13 @@ struct QkNormRopeArgs {
   const float *wq = nullptr, *wk = nullptr;   // [D] (nullable: ones)
   const float *cos = nullptr, *sin = nullptr; // [table_rows, R / 2] (R = 0: no rotation)
   const int64_t* pos = nullptr;               // [B, S] table rows (nullable: offset + s)
+  int64_t pos_stride = 0;                     // elements between samples' positions
   int64_t q_st[3] = {}, k_st[3] = {}, dyq_st[3] = {}, dyk_st[3] = {}, oq_st[3] = {}, ok_st[3] = {};
   int64_t offset = 0, table_rows = 0;
   int B = 0, S = 0, H = 0, Hk = 0, D = 0, R = 0, dtype = 0;
   float eps = 1e-5f;
   float *dwq = nullptr, *dwk = nullptr;  // backward: += weight gradients (nullable, distinct)
-  float* partials = nullptr;             // backward with weight gradients: [partial_rows, 2, D]
+  float* partials = nullptr;             // backward with weight gradients: [partial_rows, D]
   int partial_rows = 0;
 };
 int qk_norm_rope_partial_rows(const QkNormRopeArgs& a);

@@ -294,3 +294,31 @@ def test_gpu_extreme_rows():
     y, _ = ops.qk_norm_rope(x, x, None, None)
     assert (y[0, 0] == 0).all()
     torch.testing.assert_close(y[0, 1], torch.ones_like(y[0, 1]), rtol=16 * U, atol=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [0, 1])
+def test_gpu_spans_beyond_32_bits(dim):
+    """A sample (or a position) more than 2^31 elements from the first."""
+    B, S, H, D = (3, 4, 2, 64) if dim == 0 else (1, 3, 2, 64)
+    far = 2 ** 30 + 64
+    strides = (far, H * D, D, 1) if dim == 0 else (far, far, D, 1)
+    buf = torch.empty(2 * far + S * H * D, device="cuda", dtype=torch.bfloat16)
+    x = buf.as_strided((B, S, H, D), strides)
+    q, _, qw, kw, dq, _ = inputs(B, S, H, H, D, torch.bfloat16, "cuda", packed=False)
+    x.copy_(q)
+    cos, sin = tables(S + 9, D, "cuda")
+    pos = torch.randint(0, S + 9, (B, S), device="cuda")
+    for kw_pos in (dict(offset=5), dict(positions=pos)):
+        res = []
+        for v in (x, q):
+            leaf = v.detach().requires_grad_()
+            a, b = qw.clone().requires_grad_(), kw.clone().requires_grad_()
+            y = ops.qk_norm_rope(leaf, leaf, a, b, cos, sin, **kw_pos)
+            g = torch.autograd.grad(y, leaf, (dq, dq))[0]
+            res.append((*[t.detach() for t in y], g, a.grad, b.grad))
+        for i, (u, w) in enumerate(zip(*res)):
+            if i < 3:
+                assert torch.equal(u, w)
+            else:  # other launches, other order of the rows' sum
+                torch.testing.assert_close(u, w, rtol=1e-4, atol=1e-4)
