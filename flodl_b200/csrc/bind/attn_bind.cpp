@@ -150,22 +150,22 @@ Tensor cross_attn_mask(const Tensor& key_pad) {
   return bits;
 }
 
-// -> (output [B, Sq, H, D], lse2 [B, H, Sq] f32 or none, mask bits or none)
-std::tuple<Tensor, optional<Tensor>, optional<Tensor>> cross_attn_fwd(
-    const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& key_pad, bool causal,
-    double scale, bool want_lse) {
+// -> (output [B, Sq, H, D], lse2 [B, H, Sq] f32 or undefined, mask bits or undefined)
+std::tuple<Tensor, Tensor, Tensor> cross_attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                  const optional<Tensor>& key_pad, bool causal,
+                                                  double scale, bool want_lse) {
   auto a = cross_args(q, k, v, key_pad, c10::nullopt, causal, scale);
   c10::cuda::CUDAGuard guard(q.device());
   Tensor out = at::empty({a.B, a.Sq, a.H, a.D}, q.options());
   a.out = out.data_ptr();
-  optional<Tensor> lse, bits;
+  Tensor lse, bits;
   if (want_lse) {
     lse = at::empty({a.B, a.H, a.Sq}, q.options().dtype(at::kFloat));
-    a.lse2 = lse->data_ptr<float>();
+    a.lse2 = lse.data_ptr<float>();
   }
   if (a.key_pad && !flodl::cross_attn_is_few(a)) {
     bits = cross_attn_mask(*key_pad);
-    a.vis_end = bits->data_ptr<int>();
+    a.vis_end = bits.data_ptr<int>();
     a.words = reinterpret_cast<uint32_t*>(a.vis_end + a.B);
   }
   Tensor part;
@@ -205,15 +205,82 @@ void cross_attn_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const 
     a.vis_end = bits.data_ptr<int>();
     a.words = reinterpret_cast<uint32_t*>(a.vis_end + a.B);
   }
-  auto f32 = q.options().dtype(at::kFloat);
-  Tensor stats = at::empty({flodl::cross_attn_stats_floats(a)}, f32);
-  a.stats = stats.data_ptr<float>();
-  Tensor part;
-  if (const int64_t n = flodl::cross_attn_bwd_partials(a)) {
-    part = at::empty({n}, f32);
-    a.partials = part.data_ptr<float>();
-  }
+  // one allocation: the row statistics, then the pieces of split axes
+  const int64_t n_stats = flodl::cross_attn_stats_floats(a), n_part = flodl::cross_attn_bwd_partials(a);
+  Tensor scratch = at::empty({n_stats + n_part}, q.options().dtype(at::kFloat));
+  a.stats = scratch.data_ptr<float>();
+  a.partials = n_part ? a.stats + n_stats : nullptr;
   FL_CUDA_OK(flodl::launch_cross_attn_bwd(a, cur_stream()));
+}
+
+// A tensor the tile loads can read in place, or a contiguous copy.
+Tensor tma_ready(const Tensor& t) {
+  bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+optional<Tensor> if_defined(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
+
+struct CrossAttn : public torch::autograd::Function<CrossAttn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q0, const Tensor& k0,
+                        const Tensor& v0, const optional<Tensor>& key_pad, bool causal,
+                        double scale) {
+    const Tensor q = tma_ready(q0), k = tma_ready(k0), v = tma_ready(v0);
+    auto [out, lse, bits] = cross_attn_fwd(q, k, v, key_pad, causal, scale, true);
+    ctx->save_for_backward({q, k, v, out, lse, key_pad ? *key_pad : Tensor(), bits});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &q = s[0], &k = s[1], &v = s[2];
+    torch::autograd::variable_list out(6);
+    if (!grads[0].defined()) return out;
+    Tensor dq, dk, dv;
+    {
+      at::NoGradGuard no_grad;
+      const Tensor dout = tma_ready(grads[0].to(q.scalar_type()));
+      dq = at::empty(q.sizes(), q.options());
+      dk = at::empty(k.sizes(), k.options());
+      dv = at::empty(v.sizes(), v.options());
+      cross_attn_bwd(dout, q, k, v, s[3], s[4], if_defined(s[5]), if_defined(s[6]),
+                     ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), dq, dk,
+                     dv);
+    }
+    return once_differentiable({dq, dk, dv, Tensor(), Tensor(), Tensor()}, "cross_attention");
+  }
+};
+
+// Attention over a memory: argument errors are ValueErrors. Nothing comes back
+// where the kernels do not apply (another dtype or head size, an empty
+// dimension); the caller then checks and composes.
+optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor& v,
+                                 const optional<Tensor>& key_pad, bool causal, optional<double> scale) {
+  if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || !q.is_cuda() ||
+      !(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) ||
+      k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() ||
+      k.device() != q.device() || v.device() != q.device() || k.sizes() != v.sizes())
+    return c10::nullopt;
+  const int64_t B = q.size(0), D = q.size(3);
+  if (k.size(0) != B || k.size(3) != D || D % 8 || D > 128 || q.numel() == 0 || k.numel() == 0 ||
+      q.size(2) % k.size(2))
+    return c10::nullopt;
+  TORCH_CHECK_VALUE(!key_pad || (key_pad->scalar_type() == at::kBool && key_pad->dim() == 2 &&
+                                 key_pad->size(0) == B && key_pad->size(1) == k.size(1) &&
+                                 key_pad->device() == q.device()),
+                    "key_padding must be bool [", B, ", ", k.size(1), "] on ", q.device());
+  TORCH_CHECK_VALUE(!causal || q.size(1) == k.size(1), "causal attention needs equal lengths (got ",
+                    q.size(1), " and ", k.size(1), ")");
+  const double c = scale ? *scale : 1.0 / std::sqrt((double)D);
+  TORCH_CHECK_VALUE(c > 0 && std::isfinite(c), "scale must be positive and finite (got ", c, ")");
+  optional<Tensor> pad = key_pad;
+  if (pad) pad = pad->contiguous();
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return CrossAttn::apply(q, k, v, pad, causal, c);
+  return std::get<0>(cross_attn_fwd(tma_ready(q), tma_ready(k), tma_ready(v), pad, causal, c, false));
 }
 
 }  // namespace
@@ -227,9 +294,17 @@ void register_attention(py::module& m) {
         py::arg("lse2"), py::arg("dqkv"), py::arg("B"), py::arg("S"), py::arg("H"), py::arg("D"),
         py::arg("causal"), py::arg("scale"), py::arg("key_pad") = py::none(),
         py::arg("dbias") = py::none());
+  m.def("cross_attention", &cross_attention, py::arg("q"), py::arg("k"), py::arg("v"),
+        py::arg("key_padding"), py::arg("causal"), py::arg("scale"));
   m.def("cross_attn_mask", &cross_attn_mask, py::arg("key_pad"));
-  m.def("cross_attn_fwd", &cross_attn_fwd, py::arg("q"), py::arg("k"), py::arg("v"),
-        py::arg("key_pad"), py::arg("causal"), py::arg("scale"), py::arg("want_lse"));
+  m.def("cross_attn_fwd",
+        [](const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& key_pad,
+           bool causal, double scale, bool want_lse) {
+          auto [out, lse, bits] = cross_attn_fwd(q, k, v, key_pad, causal, scale, want_lse);
+          return std::make_tuple(out, if_defined(lse), if_defined(bits));
+        },
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("key_pad"), py::arg("causal"),
+        py::arg("scale"), py::arg("want_lse"));
   m.def("cross_attn_bwd", &cross_attn_bwd, py::arg("dout"), py::arg("q"), py::arg("k"),
         py::arg("v"), py::arg("out"), py::arg("lse2"), py::arg("key_pad"), py::arg("mask_bits"),
         py::arg("causal"), py::arg("scale"), py::arg("dq"), py::arg("dk"), py::arg("dv"));

@@ -1,6 +1,7 @@
 // Shared helpers for the torch-facing bindings of the CUDA kernel library.
 #pragma once
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -36,6 +37,26 @@ inline cudaStream_t cur_stream() {
 template <typename T>
 inline T* opt_ptr(const c10::optional<at::Tensor>& t) {
   return (t.has_value() && t->defined()) ? reinterpret_cast<T*>(t->data_ptr()) : nullptr;
+}
+
+// Gradients of an operator that is differentiable once: where the backward
+// itself is being recorded (create_graph), differentiating them raises.
+inline torch::autograd::variable_list once_differentiable(torch::autograd::variable_list grads,
+                                                          const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::variable_list defined;
+  for (const auto& g : grads)
+    if (g.defined()) {
+      defined.push_back(g);
+      defined.back().set_requires_grad(true);
+    }
+  auto err = std::make_shared<torch::autograd::DelayedError>(
+      std::string(what) + " is differentiable once", (int)defined.size());
+  auto out = (*err)(std::move(defined));
+  size_t i = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = out[i++];
+  return grads;
 }
 
 namespace py = pybind11;

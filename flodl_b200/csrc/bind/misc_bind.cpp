@@ -160,7 +160,8 @@ void qk_norm_rope_bwd(const Tensor& dyq, const Tensor& dyk, const Tensor& q, con
                       const optional<Tensor>& wq, const optional<Tensor>& wk,
                       const optional<Tensor>& cos, const optional<Tensor>& sin,
                       const optional<Tensor>& pos, int64_t offset, Tensor& dq, Tensor& dk,
-                      const optional<Tensor>& dwq, const optional<Tensor>& dwk, double eps) {
+                      const optional<Tensor>& dwq, const optional<Tensor>& dwk, double eps,
+                      bool dwq_add = true, bool dwk_add = true) {
   auto a = qk_args(q, k, wq, wk, cos, sin, pos, offset, dq, dk, eps);
   for (const Tensor* t : {&dyq, &dyk})
     FL_CHECK(t->scalar_type() == q.scalar_type() && t->device() == q.device() && t->dim() == 4 &&
@@ -181,6 +182,8 @@ void qk_norm_rope_bwd(const Tensor& dyq, const Tensor& dyk, const Tensor& q, con
                "qk_norm_rope: weight gradients must be f32 [D]");
   a.dwq = opt_ptr<float>(dwq);
   a.dwk = opt_ptr<float>(dwk);
+  a.dwq_add = dwq_add;
+  a.dwk_add = dwk_add;
   FL_CHECK(!a.dwq || a.dwq != a.dwk, "qk_norm_rope: one buffer for both weight gradients");
   c10::cuda::CUDAGuard guard(q.device());
   Tensor partials;
@@ -190,6 +193,151 @@ void qk_norm_rope_bwd(const Tensor& dyq, const Tensor& dyk, const Tensor& q, con
     a.partials = partials.data_ptr<float>();
   }
   FL_CUDA_OK(flodl::launch_qk_norm_rope_bwd(a, cur_stream()));
+}
+
+// Gradient-ready listeners of a parameter live on its Python object.
+void notify_grad_ready(const Tensor& w) {
+  py::gil_scoped_acquire gil;
+  static py::object& fn =
+      *new py::object(py::module_::import("flodl_b200.ops._common").attr("grad_ready"));
+  fn(w);
+}
+
+Tensor rows_ready(const Tensor& t) {
+  return t.stride(-1) == 1 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+optional<Tensor> some(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
+
+// Input gradients into dq / dk, and the weight gradients: a leaf weight's is
+// added to its .grad and its listeners are notified, as the other fused norms
+// do; a computed weight's is returned for autograd.
+std::pair<Tensor, Tensor> qk_norm_rope_backward(const Tensor& dyq, const Tensor& dyk,
+                                                const Tensor& q, const Tensor& k, const Tensor& wq,
+                                                const Tensor& wk, const Tensor& cos,
+                                                const Tensor& sin, const Tensor& pos,
+                                                int64_t offset, double eps, Tensor& dq, Tensor& dk) {
+  at::NoGradGuard no_grad;
+  const Tensor* w[2] = {&wq, &wk};
+  Tensor buf[2], ret[2];
+  bool add[2] = {false, false};
+  const bool shared = wq.defined() && wk.defined() && wq.is_same(wk);
+  for (int i = 0; i < 2; ++i) {
+    if (!w[i]->defined() || !w[i]->requires_grad()) continue;
+    const bool leaf = w[i]->is_leaf() && !shared;
+    add[i] = leaf && w[i]->grad().defined();
+    buf[i] = add[i] ? w[i]->grad() : at::empty(w[i]->sizes(), q.options().dtype(at::kFloat));
+    if (leaf && !add[i]) w[i]->mutable_grad() = buf[i];
+    if (!w[i]->is_leaf()) ret[i] = buf[i];
+  }
+  qk_norm_rope_bwd(dyq, dyk, q, k, some(wq), some(wk), some(cos), some(sin), some(pos), offset, dq,
+                   dk, some(buf[0]), some(buf[1]), eps, add[0], add[1]);
+  if (shared && wq.requires_grad() && wq.is_leaf()) {
+    buf[0].add_(buf[1]);
+    if (wq.grad().defined())
+      wq.mutable_grad().add_(buf[0]);
+    else
+      wq.mutable_grad() = buf[0];
+  }
+  for (int i = 0; i < (shared ? 1 : 2); ++i)
+    if (w[i]->defined() && w[i]->requires_grad() && w[i]->is_leaf()) notify_grad_ready(*w[i]);
+  return {ret[0], ret[1]};
+}
+
+struct QkNormRope : public torch::autograd::Function<QkNormRope> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                const Tensor& q0, const Tensor& k0,
+                                                const optional<Tensor>& wq,
+                                                const optional<Tensor>& wk,
+                                                const optional<Tensor>& cos,
+                                                const optional<Tensor>& sin,
+                                                const optional<Tensor>& pos, int64_t offset,
+                                                double eps) {
+    const Tensor q = rows_ready(q0), k = rows_ready(k0);
+    Tensor yq = at::empty(q.sizes(), q.options()), yk = at::empty(k.sizes(), k.options());
+    qk_norm_rope_fwd(q, k, wq, wk, cos, sin, pos, offset, yq, yk, eps);
+    auto t = [](const optional<Tensor>& x) { return x ? *x : Tensor(); };
+    ctx->save_for_backward({q, k, t(wq), t(wk), t(cos), t(sin), t(pos)});
+    ctx->saved_data["offset"] = offset;
+    ctx->saved_data["eps"] = eps;
+    return {yq, yk};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &q = s[0], &k = s[1];
+    torch::autograd::variable_list out(9);
+    {
+      at::NoGradGuard no_grad;
+      Tensor dy[2];
+      for (int i = 0; i < 2; ++i)
+        dy[i] = grads[i].defined() ? rows_ready(grads[i].to(q.scalar_type()))
+                                   : at::zeros(s[i].sizes(), q.options());
+      out[0] = at::empty(q.sizes(), q.options());
+      out[1] = at::empty(k.sizes(), k.options());
+      std::tie(out[2], out[3]) = qk_norm_rope_backward(
+          dy[0], dy[1], q, k, s[2], s[3], s[4], s[5], s[6], ctx->saved_data["offset"].toInt(),
+          ctx->saved_data["eps"].toDouble(), out[0], out[1]);
+    }
+    return once_differentiable(out, "qk_norm_rope");
+  }
+};
+
+// The operator: argument errors are ValueErrors. Nothing comes back where the
+// kernels do not apply (another dtype or head size, an empty input); the caller
+// then checks and composes.
+optional<std::pair<Tensor, Tensor>> qk_norm_rope(const Tensor& q, const Tensor& k,
+                                                 const optional<Tensor>& q_weight,
+                                                 const optional<Tensor>& k_weight,
+                                                 const optional<Tensor>& cos,
+                                                 const optional<Tensor>& sin,
+                                                 const optional<Tensor>& positions, int64_t offset,
+                                                 double eps) {
+  if (!q.is_cuda() || dtype_code(q) < 0 || q.dim() != 4 || k.dim() != 4 || q.size(3) < 2 ||
+      q.size(3) > flodl::kQkNormRopeMaxD || q.numel() == 0 || k.numel() == 0)
+    return c10::nullopt;
+  const int64_t B = q.size(0), S = q.size(1), D = q.size(3);
+  TORCH_CHECK_VALUE(k.size(0) == B && k.size(1) == S && k.size(3) == D, "queries ", q.sizes(),
+                    " and keys ", k.sizes(), " differ in batch, positions or head size");
+  TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && k.device() == q.device(),
+                    "queries and keys must be floating-point tensors of one dtype and device");
+  for (const optional<Tensor>* w : {&q_weight, &k_weight}) {
+    TORCH_CHECK_VALUE(!*w || ((*w)->dim() == 1 && (*w)->numel() == D &&
+                              (*w)->scalar_type() == at::kFloat && (*w)->device() == q.device()),
+                      "weights must be f32 [", D, "] on ", q.device());
+  }
+  TORCH_CHECK_VALUE(cos.has_value() == sin.has_value(), "cos and sin come together");
+  TORCH_CHECK_VALUE(cos || !positions, "positions need the cos and sin tables");
+  const bool turn = cos && cos->dim() == 2 && cos->size(1) > 0;
+  if (cos) {
+    TORCH_CHECK_VALUE(cos->dim() == 2 && cos->sizes() == sin->sizes() && 2 * cos->size(1) <= D &&
+                          cos->scalar_type() == at::kFloat && sin->scalar_type() == at::kFloat &&
+                          cos->device() == q.device() && sin->device() == q.device(),
+                      "cos and sin must be f32 [positions, R / 2] with R <= ", D, " on ", q.device());
+    if (positions) {
+      TORCH_CHECK_VALUE(offset == 0 && positions->scalar_type() == at::kLong &&
+                            positions->dim() == 2 && positions->size(0) == B &&
+                            positions->size(1) == S && positions->device() == q.device(),
+                        "positions must be int64 [", B, ", ", S, "] on ", q.device(),
+                        ", without an offset");
+    } else {
+      TORCH_CHECK_VALUE(offset >= 0 && offset <= cos->size(0) - S, "positions ", offset, " to ",
+                        offset + S - 1, " are outside the tables' ", cos->size(0), " rows");
+    }
+  }
+  auto plain = [](const optional<Tensor>& t) {
+    return t ? optional<Tensor>(t->contiguous()) : c10::nullopt;
+  };
+  const auto wq = plain(q_weight), wk = plain(k_weight);
+  const auto c = turn ? plain(cos) : c10::nullopt, s = turn ? plain(sin) : c10::nullopt;
+  const auto pos = turn ? plain(positions) : c10::nullopt;
+  auto grad = [](const optional<Tensor>& t) { return t && t->requires_grad(); };
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || grad(wq) || grad(wk))) {
+    auto y = QkNormRope::apply(q, k, wq, wk, c, s, pos, offset, eps);
+    return std::make_pair(y[0], y[1]);
+  }
+  Tensor yq = at::empty(q.sizes(), q.options()), yk = at::empty(k.sizes(), k.options());
+  qk_norm_rope_fwd(rows_ready(q), rows_ready(k), wq, wk, c, s, pos, offset, yq, yk, eps);
+  return std::make_pair(yq, yk);
 }
 
 // GroupNorm over x [N, C, *] contiguous (f32 or bf16), G groups.
@@ -529,13 +677,24 @@ void register_elementwise(py::module& m) {
         py::arg("eps"));
   m.def("rms_bwd", &rms_bwd, py::arg("dy"), py::arg("x"), py::arg("w"), py::arg("rstd"),
         py::arg("dx"), py::arg("dw"));
+  m.def("qk_norm_rope", &qk_norm_rope, py::arg("q"), py::arg("k"), py::arg("q_weight"),
+        py::arg("k_weight"), py::arg("cos"), py::arg("sin"), py::arg("positions"),
+        py::arg("offset"), py::arg("eps"));
   m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd, py::arg("q"), py::arg("k"), py::arg("wq"),
         py::arg("wk"), py::arg("cos"), py::arg("sin"), py::arg("pos"), py::arg("offset"),
         py::arg("yq"), py::arg("yk"), py::arg("eps"));
-  m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd, py::arg("dyq"), py::arg("dyk"), py::arg("q"),
-        py::arg("k"), py::arg("wq"), py::arg("wk"), py::arg("cos"), py::arg("sin"), py::arg("pos"),
-        py::arg("offset"), py::arg("dq"), py::arg("dk"), py::arg("dwq"), py::arg("dwk"),
-        py::arg("eps"));
+  m.def("qk_norm_rope_backward", [](const Tensor& dyq, const Tensor& dyk, const Tensor& q,
+                                    const Tensor& k, const optional<Tensor>& wq,
+                                    const optional<Tensor>& wk, const optional<Tensor>& cos,
+                                    const optional<Tensor>& sin, const optional<Tensor>& pos,
+                                    int64_t offset, double eps, Tensor& dq, Tensor& dk) {
+    auto t = [](const optional<Tensor>& x) { return x ? *x : Tensor(); };
+    auto [a, b] = qk_norm_rope_backward(dyq, dyk, q, k, t(wq), t(wk), t(cos), t(sin), t(pos), offset,
+                                        eps, dq, dk);
+    return std::make_pair(some(a), some(b));
+  }, py::arg("dyq"), py::arg("dyk"), py::arg("q"), py::arg("k"), py::arg("q_weight"),
+        py::arg("k_weight"), py::arg("cos"), py::arg("sin"), py::arg("positions"),
+        py::arg("offset"), py::arg("eps"), py::arg("dq"), py::arg("dk"));
   m.def("gn_fwd", &gn_fwd, py::arg("x"), py::arg("gamma"), py::arg("beta"), py::arg("y"),
         py::arg("mean"), py::arg("rstd"), py::arg("groups"), py::arg("eps"));
   m.def("gn_bwd", &gn_bwd, py::arg("dy"), py::arg("x"), py::arg("gamma"), py::arg("mean"),

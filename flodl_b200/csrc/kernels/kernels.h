@@ -65,7 +65,8 @@ struct QkNormRopeArgs {
   int64_t offset = 0, table_rows = 0;
   int B = 0, S = 0, H = 0, Hk = 0, D = 0, R = 0, dtype = 0;
   float eps = 1e-5f;
-  float *dwq = nullptr, *dwk = nullptr;  // backward: += weight gradients (nullable, distinct)
+  float *dwq = nullptr, *dwk = nullptr;  // backward: weight gradients (nullable, distinct),
+  bool dwq_add = true, dwk_add = true;   // added to what is there, or written
   float* partials = nullptr;             // backward with weight gradients: [partial_rows, D]
   int partial_rows = 0;
 };

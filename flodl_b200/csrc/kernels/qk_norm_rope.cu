@@ -384,12 +384,13 @@ __global__ void __launch_bounds__(kThreads, kLanes ? ctas_per_sm(kBwd, sizeof(T)
   }
 }
 
-// dw += the column sums of the blocks' rows, queries' rows first: 32 columns of
+// dw (+)= the column sums of the blocks' rows, queries' rows first: 32 columns of
 // one weight per block, 32 rows at a time, then the 32 row sums in order.
 __global__ void __launch_bounds__(1024) qk_norm_rope_dw_kernel(const float* __restrict__ partials,
                                                                int q_rows, int rows, int D,
                                                                float* __restrict__ dwq,
-                                                               float* __restrict__ dwk) {
+                                                               float* __restrict__ dwk, int add_q,
+                                                               int add_k) {
   __shared__ float s[32][33];
   pdl_wait();
   pdl_trigger();
@@ -409,7 +410,8 @@ __global__ void __launch_bounds__(1024) qk_norm_rope_dw_kernel(const float* __re
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
   const int mine = blockIdx.x * 32 + warp;
-  if (lane == 0 && mine < D && out) out[mine] += t;
+  if (lane == 0 && mine < D && out)
+    out[mine] = (blockIdx.y == 0 ? add_q : add_k) ? out[mine] + t : t;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -523,7 +525,10 @@ cudaError_t run(const QkNormRopeArgs& a, bool bwd, cudaStream_t st) {
     const bool samples = a.B > 1;
     const int n = samples ? a.B : a.S;
     const cudaError_t e = run(part_of(a, samples, 0, n / 2), bwd, st);
-    return e != cudaSuccess ? e : run(part_of(a, samples, n / 2, n - n / 2), bwd, st);
+    if (e != cudaSuccess) return e;
+    QkNormRopeArgs rest = part_of(a, samples, n / 2, n - n / 2);
+    rest.dwq_add = rest.dwk_add = true;
+    return run(rest, bwd, st);
   }
   if (!narrow(a, bwd) || a.table_rows * (int64_t)(a.R / 2) >= kMaxFlatIndex || a.B <= 0 || a.S <= 0 || a.H <= 0 || a.Hk <= 0 || a.D <= 0 || a.D > kQkNormRopeMaxD ||
       a.R < 0 || a.R > a.D || a.R % 2 || a.dtype < 0 || a.dtype > 2)
@@ -560,7 +565,8 @@ cudaError_t run(const QkNormRopeArgs& a, bool bwd, cudaStream_t st) {
   note_launch();
   if (dw) {
     e = launch_pdl(qk_norm_rope_dw_kernel, dim3((a.D + 31) / 32, 2), dim3(1024), 0, st,
-                   (const float*)a.partials, plan.q_blocks, grid, a.D, a.dwq, a.dwk);
+                   (const float*)a.partials, plan.q_blocks, grid, a.D, a.dwq, a.dwk,
+                   (int)a.dwq_add, (int)a.dwk_add);
     if (e != cudaSuccess) return e;
     note_launch();
   }

@@ -15,7 +15,6 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from ._common import C, use_kernels
 
@@ -118,42 +117,6 @@ def scaled_dot_product_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
 
 
 # ----------------------------------------------------------------- separate q, k, v
-def _tma_ready(t: torch.Tensor) -> torch.Tensor:
-    """A [B, S, heads, D] tensor the tile loads can read in place - contiguous
-    last dimension, other strides positive multiples of 16 bytes, 16-byte
-    aligned - or a contiguous copy."""
-    s = t.stride()
-    if s[3] == 1 and t.data_ptr() % 16 == 0:
-        n = t.shape
-        for i in range(3):
-            if n[i] != 1 and (s[i] % 8 or s[i] <= 0):
-                break
-        else:
-            return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 and t.stride(3) == 1 else t.clone(
-        memory_format=torch.contiguous_format)
-
-
-class _CrossAttnFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, key_padding, causal, scale):
-        q, k, v = _tma_ready(q), _tma_ready(k), _tma_ready(v)
-        out, lse, bits = C().cross_attn_fwd(q, k, v, key_padding, causal, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, key_padding, bits)
-        ctx.consts = (causal, scale)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, lse, key_padding, bits = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
-        C().cross_attn_bwd(_tma_ready(dout.to(q.dtype)), q, k, v, out, lse, key_padding, bits,
-                           *ctx.consts, dq, dk, dv)
-        return dq, dk, dv, None, None, None
-
-
 def _cross_composed(q, k, v, key_padding, causal, scale):
     """The explicit form in the inputs' precision, at least f32."""
     B, Sq, H, D = q.shape
@@ -203,6 +166,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     products. Gradients are the same from run to run. Other inputs run the
     composed form in f32 or f64.
     """
+    if use_kernels(q):
+        out = C().cross_attention(q, k, v, key_padding, causal, scale)
+        if out is not None:
+            return out
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError(f"cross_attention takes [B, S, heads, D] tensors (got {tuple(q.shape)} and "
                          f"{tuple(k.shape)})")
@@ -227,12 +194,4 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite (got {scale})")
-    if not (use_kernels(q) and q.dtype in (torch.bfloat16, torch.float16) and D % 8 == 0 and D <= 128
-            and B and Sq and Sk):
-        return _cross_composed(q, k, v, key_padding, causal, scale)
-    if key_padding is not None:
-        key_padding = key_padding.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _CrossAttnFn.apply(q, k, v, key_padding, bool(causal), scale)
-    return C().cross_attn_fwd(_tma_ready(q), _tma_ready(k), _tma_ready(v), key_padding, bool(causal),
-                              scale, False)[0]
+    return _cross_composed(q, k, v, key_padding, causal, scale)

@@ -11,7 +11,6 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from ._common import C, grad_buffer, grad_ready, use_kernels, wants_grad
 
@@ -155,77 +154,6 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     return _GroupNormFn.apply(x, int(groups), weight, bias, float(eps))
 
 
-def _rows_ok(t: torch.Tensor) -> torch.Tensor:
-    """A tensor whose last dimension is contiguous (a copy where it is not)."""
-    return t if t.stride(-1) == 1 else t.contiguous()
-
-
-def qk_norm_rope_forward(q, k, q_weight, k_weight, cos, sin, positions, offset, eps):
-    """The forward kernel on checked CUDA arguments (no autograd)."""
-    yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    yk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-    if q.numel() == 0:
-        return yq, yk
-    C().qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, positions, offset, yq, yk, eps)
-    return yq, yk
-
-
-def qk_norm_rope_backward(dyq, dyk, q, k, q_weight, k_weight, cos, sin, positions, offset, eps,
-                          dq, dk):
-    """The backward kernels: input gradients into ``dq`` / ``dk`` (any strides
-    with a contiguous last dimension) and the weight gradients. A leaf weight's
-    gradient is added to its ``.grad`` and its listeners are notified, as the
-    other fused norms do; a computed weight's gradient is returned. Returns
-    ``(dq_weight, dk_weight)`` for autograd."""
-    if q.numel() == 0:
-        return (torch.zeros_like(q_weight) if wants_grad(q_weight) else None,
-                torch.zeros_like(k_weight) if wants_grad(k_weight) else None)
-    shared = q_weight is not None and q_weight is k_weight
-    bufs, returned = [], []
-    for w in (q_weight, k_weight):
-        if not wants_grad(w):
-            bufs.append(None)
-            returned.append(None)
-        elif w.is_leaf and not shared:
-            bufs.append(grad_buffer(w))
-            returned.append(None)
-        else:
-            bufs.append(torch.zeros(w.shape, device=q.device, dtype=torch.float32))
-            returned.append(bufs[-1])
-    det = (lambda w: w.detach() if w is not None else None)
-    C().qk_norm_rope_bwd(dyq, dyk, q, k, det(q_weight), det(k_weight), cos, sin, positions, offset,
-                         dq, dk, bufs[0], bufs[1], eps)
-    if shared and wants_grad(q_weight) and q_weight.is_leaf:
-        grad_buffer(q_weight).add_(bufs[0]).add_(bufs[1])
-        returned = [None, None]
-    for w in ((q_weight,) if shared else (q_weight, k_weight)):
-        if wants_grad(w) and w.is_leaf:
-            grad_ready(w)
-    return tuple(returned)
-
-
-class _QkNormRopeFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, offset, eps):
-        q, k = _rows_ok(q), _rows_ok(k)
-        det = (lambda w: w.detach() if w is not None else None)
-        yq, yk = qk_norm_rope_forward(q, k, det(q_weight), det(k_weight), cos, sin, positions,
-                                      offset, eps)
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.consts = (offset, eps)
-        return yq, yk
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dyq, dyk):
-        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-        dwq, dwk = qk_norm_rope_backward(_rows_ok(dyq.to(q.dtype)), _rows_ok(dyk.to(k.dtype)), q, k,
-                                         q_weight, k_weight, cos, sin, positions, *ctx.consts, dq, dk)
-        return dq, dk, dwq, dwk, None, None, None, None, None
-
-
 def _check_qk(q, k, q_weight, k_weight, cos, sin, positions, offset):
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError(f"qk_norm_rope takes [B, S, heads, D] queries and keys (got {tuple(q.shape)}"
@@ -298,28 +226,25 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     values of its heads and records code 5 in the kernel error word on CUDA;
     on the CPU it raises.
     """
+    if use_kernels(q):
+        y = C().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, offset, eps)
+        if y is not None:
+            return y
     _check_qk(q, k, q_weight, k_weight, cos, sin, positions, offset)
     if cos is not None and cos.shape[1] == 0:
         cos = sin = positions = None
-    if (not use_kernels(q) or q.dtype not in (torch.float32, torch.bfloat16, torch.float16)
-            or not 2 <= q.shape[3] <= 256):
-        c = s = None
-        if cos is not None:
-            at = positions if positions is not None else slice(offset, offset + q.shape[1])
-            if positions is not None and not q.is_cuda and positions.numel() and (
-                    int(positions.min()) < 0 or int(positions.max()) >= cos.shape[0]):
-                raise IndexError(f"a position is outside the tables' {cos.shape[0]} rows")
-            if positions is not None and q.is_cuda:
-                bad = (at < 0) | (at >= cos.shape[0])
-                at = at.clamp(0, max(cos.shape[0] - 1, 0))
-                c, s = (t[at].masked_fill(bad[..., None], float("nan")) for t in (cos, sin))
-            else:
-                c, s = cos[at], sin[at]
-        return (_qk_norm_rope_composed(q, q_weight, c, s, eps),
-                _qk_norm_rope_composed(k, k_weight, c, s, eps))
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight), ("cos", cos), ("sin", sin)):
-        if w is not None and w.dtype != torch.float32:
-            raise ValueError(f"{name} must be f32 (got {w.dtype})")
-    c = (lambda t: t.contiguous() if t is not None else None)
-    return _QkNormRopeFn.apply(q, k, c(q_weight), c(k_weight), c(cos), c(sin), c(positions),
-                               int(offset), float(eps))
+    c = s = None
+    if cos is not None and positions is None:
+        c, s = cos[offset:offset + q.shape[1]], sin[offset:offset + q.shape[1]]
+    elif cos is not None:
+        rows = cos.shape[0]
+        if not q.is_cuda:
+            if positions.numel() and (int(positions.min()) < 0 or int(positions.max()) >= rows):
+                raise IndexError(f"a position is outside the tables' {rows} rows")
+            c, s = cos[positions], sin[positions]
+        else:
+            bad = ((positions < 0) | (positions >= rows))[..., None]
+            at = positions.clamp(0, max(rows - 1, 0))
+            c, s = (t[at].masked_fill(bad, float("nan")) for t in (cos, sin))
+    return (_qk_norm_rope_composed(q, q_weight, c, s, eps),
+            _qk_norm_rope_composed(k, k_weight, c, s, eps))

@@ -389,3 +389,22 @@ def test_gpu_refusals_and_other_forms():
     with pytest.raises(RuntimeError):
         C.cross_attn_fwd(b(q), b(k), b(v), None, False, -1.0, False)
     assert cuda_ext().kernel_error() == 0
+
+
+@pytest.mark.gpu
+def test_gpu_differentiable_once_and_partial_gradients():
+    q, k, v, do = make(2, 40, 2, 1, 70, 64, torch.bfloat16, "cuda")
+    want = None
+    for need in itertools.product((False, True), repeat=3):
+        if not any(need):
+            continue
+        leaves = [x.clone().requires_grad_(n) for x, n in zip((q, k, v), need)]
+        ops.cross_attention(*leaves).backward(do)
+        grads = [x.grad for x in leaves]
+        if all(need):
+            want = grads
+        assert all((g is not None) == n for g, n in zip(grads, need))
+    g, = torch.autograd.grad(ops.cross_attention(*leaves), leaves[0], do, create_graph=True)
+    assert torch.equal(g.detach(), want[0])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), leaves[0])

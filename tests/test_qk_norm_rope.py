@@ -322,3 +322,17 @@ def test_gpu_spans_beyond_32_bits(dim):
                 assert torch.equal(u, w)
             else:  # other launches, other order of the rows' sum
                 torch.testing.assert_close(u, w, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.gpu
+def test_gpu_differentiable_once_and_partial_use():
+    q, k, qw, kw, dq, _ = inputs(1, 4, 2, 2, 64, torch.bfloat16, "cuda", packed=False)
+    q, k = q.requires_grad_(), k.requires_grad_()
+    y = ops.qk_norm_rope(q, k, qw, kw)[0]
+    g, = torch.autograd.grad(y, q, dq, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), q)
+    # only one of the two results used: the other has no gradient
+    y = ops.qk_norm_rope(q, k, qw, kw)[1]
+    a, b = torch.autograd.grad(y, (q, k), dq, allow_unused=True)
+    assert (a is None or (a == 0).all()) and torch.isfinite(b).all() and b.abs().max() > 0
