@@ -84,15 +84,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x,
-                                            int y, int z, int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
-
 // A tile of kN rows and kDP columns: kDP / 64 blocks of kN rows x 128 bytes in
 // 128-byte swizzle.
 template <int kN, int kDP>
@@ -1110,10 +1101,12 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
+}  // namespace
+
 // Map {D, position, head, batch} of a strided 16-bit tensor; box = 64 columns x
 // `rows` positions. The stride of a dimension of one does not matter: any valid
 // value goes.
-bool make_map(CUtensorMap* m, const void* base, bool half, int D, int S, int heads, int B,
+bool cross_attn_map(CUtensorMap* m, const void* base, bool half, int D, int S, int heads, int B,
               const int64_t (&st)[3], int rows) {
   auto enc = encode_fn();
   if (!enc) return false;
@@ -1134,20 +1127,21 @@ bool make_map(CUtensorMap* m, const void* base, bool half, int D, int S, int hea
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Shared-memory opt-in, once per kernel and device.
-template <typename K>
-cudaError_t opt_in(K kernel, int smem, std::atomic<uint64_t>& done) {
+cudaError_t cross_attn_opt_in(const void* kernel, size_t smem, std::atomic<uint64_t>& done) {
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                              cudaSharedmemCarveoutMaxShared);
   if (e == cudaSuccess) done.fetch_or(bit);
   return e;
 }
+
+namespace {
 
 Shape shape_of(const CrossAttnArgs& a, int splits) {
   Shape s{};
@@ -1195,14 +1189,14 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   if (splits > 1 && !a.partials) return cudaErrorInvalidValue;
   constexpr int kn = FwdGeo<kDP>::kN;
   CUtensorMap mq, mk, mv;
-  if (!make_map(&mq, a.q, a.half, a.D, a.Sq, a.H, a.B, a.q_st, kRows) ||
-      !make_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kn) ||
-      !make_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kn))
+  if (!cross_attn_map(&mq, a.q, a.half, a.D, a.Sq, a.H, a.B, a.q_st, kRows) ||
+      !cross_attn_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kn) ||
+      !cross_attn_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kn))
     return cudaErrorInvalidValue;
   static std::atomic<uint64_t> done{0};
   const int smem = (int)sizeof(FwdSmem<kDP>) + 1024;
   auto kernel = cross_fwd_kernel<T, kDP>;
-  cudaError_t e = opt_in(kernel, smem, done);
+  cudaError_t e = cross_attn_opt_in((const void*)kernel, smem, done);
   if (e != cudaSuccess) return e;
   const int n_qt = (int)row_tiles(a.Sq);
   const int64_t items = (int64_t)n_qt * a.H * a.B * splits;
@@ -1221,16 +1215,16 @@ cudaError_t run_bwd_half(const CrossAttnArgs& a, cudaStream_t st) {
   if (splits > 1 && !a.partials) return cudaErrorInvalidValue;
   const int rb = kRows, cb = kBN;
   CUtensorMap mq, mk, mv, mo;
-  if (!make_map(&mq, a.q, a.half, a.D, a.Sq, a.H, a.B, a.q_st, kKeys ? cb : rb) ||
-      !make_map(&mo, a.dout, a.half, a.D, a.Sq, a.H, a.B, a.do_st, kKeys ? cb : rb) ||
-      !make_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kKeys ? rb : cb) ||
-      !make_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kKeys ? rb : cb))
+  if (!cross_attn_map(&mq, a.q, a.half, a.D, a.Sq, a.H, a.B, a.q_st, kKeys ? cb : rb) ||
+      !cross_attn_map(&mo, a.dout, a.half, a.D, a.Sq, a.H, a.B, a.do_st, kKeys ? cb : rb) ||
+      !cross_attn_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kKeys ? rb : cb) ||
+      !cross_attn_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kKeys ? rb : cb))
     return cudaErrorInvalidValue;
   static std::atomic<uint64_t> done{0};
   constexpr int smem = (int)sizeof(BwdSmem<kDP>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory");
   auto kernel = cross_bwd_kernel<T, kDP, kKeys>;
-  cudaError_t e = opt_in(kernel, smem, done);
+  cudaError_t e = cross_attn_opt_in((const void*)kernel, smem, done);
   if (e != cudaSuccess) return e;
   const int S = kKeys ? a.Sk : a.Sq, heads = kKeys ? a.Hk : a.H;
   const int n_rt = (int)row_tiles(S);

@@ -1,8 +1,11 @@
 // Host interface of attention with queries, keys and values in tensors of
 // their own (cross_attn.cu, cross_attn_few.cu).
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <atomic>
 
 #include "gemm_sm100.h"
 
@@ -49,6 +52,12 @@ cudaError_t launch_cross_attn_fwd(const CrossAttnArgs& a, cudaStream_t st);
 cudaError_t launch_cross_attn_bwd(const CrossAttnArgs& a, cudaStream_t st);
 
 // Pieces shared by the two files.
+// Map {D, position, head, batch} of a strided 16-bit tensor; box = 64 columns x
+// `rows` positions.
+bool cross_attn_map(CUtensorMap* m, const void* base, bool half, int D, int S, int heads, int B,
+                    const int64_t (&st)[3], int rows);
+// Shared-memory opt-in of a kernel, once per device.
+cudaError_t cross_attn_opt_in(const void* kernel, size_t smem, std::atomic<uint64_t>& done);
 int cross_attn_few_splits(const CrossAttnArgs& a);
 cudaError_t launch_cross_attn_few(const CrossAttnArgs& a, cudaStream_t st);
 // out = the partial results of `splits` key ranges joined by their lse.

@@ -8,44 +8,59 @@
 //   l = sum p,  o = sum p v,  out = o / l,  lse2 = m + log2 l.
 //
 // What bounds it: the bytes of K and V (1 multiply-add per byte and row), so
-// the kernel is built around loads in flight, not around the tensor pipe. A
-// warp takes 32 keys at a time and loads K and V straight into the registers
-// of mma.m16n8k16 fragments with 16-byte loads, without shared memory:
-//  * S = Q K^T: the contraction index may be permuted as long as Q and K agree,
-//    so lane t of a quad takes 8 consecutive values of a key (one 16-byte load
-//    is two k-steps' B fragments).
-//  * O += P V: the output column index may be permuted, so lane group g takes
-//    D / 8 consecutive columns of the four keys its fragment needs and pairs
-//    them with byte permutes. P's accumulator layout is the A fragment's.
-// (tcgen05 would need 128 rows and a shared-memory stage for the same bytes.)
-// K is reloaded for the warp's next keys as soon as its fragments are used,
-// V likewise, so one of the two is always in flight. The key axis is split
-// over CTAs until the SMs are covered; the pieces are joined by their lse in
-// a second kernel, in a fixed order.
+// the kernel is built around loads in flight. Tiles of 64 keys come by TMA from
+// the strided tensors into a ring of shared-memory stages (64 KB per CTA, three
+// CTAs per SM: loads in flight need no registers), four consumer warps take 16
+// keys of every tile each, with a running maximum, sum and output of their own,
+// and read the fragments of mma.m16n8k16 with ldmatrix: the 16 rows of that
+// shape are what a serving batch's token has (tcgen05 would compute 128), and
+// the tensor pipe is not the limit. (A first version loaded the fragments
+// straight from global memory: 680 instructions per 16 keys, 2.5 TB/s.)
+// The key axis is split over CTAs until the SMs are covered; the pieces are
+// joined by their lse in a second kernel, in a fixed order.
 #include "sm100_ptx.cuh"
 #include "cross_attn.h"
 
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 namespace flodl {
 
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kKeys = 32;               // keys per warp step and per mask word
-constexpr int kMaxWords = 4096;         // mask words a CTA holds: 131072 keys of a split
+constexpr int kKeys = 64;               // keys of a tile: two mask words
+constexpr int kWarps = 4;               // consumer warps, 16 keys of a tile each
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kStageBytes = 64 * 1024;  // of all stages
+constexpr int kMaxWords = 2048;         // mask words a CTA holds: 65536 keys of a split
+constexpr uint64_t kWaitNs = 2000000000ull;
 
 struct FewParams {
-  const void *q, *k, *v;
+  const void* q;
   void* out;
   float *lse2, *part_o, *part_lse;
   const uint8_t* key_pad;
-  int64_t qb, qs, qh, kb, ks, kh, vb, vs, vh;
+  int64_t qb, qs, qh;
   int B, Sq, Sk, H, Hk, D, G, rows, splits;
   int causal;
   float sl2;
+  uint32_t* err;
+};
+
+template <int kDP>
+struct FewSmem {
+  static constexpr int kTile = kKeys * kDP * 2;
+  static constexpr int kStages = kStageBytes / (2 * kTile);
+  uint8_t k[kStages][kTile], v[kStages][kTile];  // the warps' outputs once all are read
+  uint8_t q[16 * kDP * 2];
+  float m[kWarps][16], l[kWarps][16];
+  uint64_t full[kStages], empty[kStages];
+  uint32_t abort;
+  int vis_end;  // of this CTA's words
+  // uint32_t words[] behind it, only with a mask
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -88,258 +103,259 @@ __device__ __forceinline__ uint32_t pack<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ uint4 ldg_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
 }
 
-// kDP: the head size rounded up to 64 or 128; kSub: 16-key groups per step (a
-// step's K and V take 64 registers either way).
-template <typename T, int kDP, int kSub, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32) few_kernel(const __grid_constant__ FewParams p) {
-  constexpr int kB32 = kDP / 32;        // 32-column blocks of a key
-  constexpr int kNT = kDP / 8;          // output column tiles, and columns per lane group
-  constexpr int kVL = kNT / 8;          // 16-byte loads of a value row per lane
-  constexpr int kStep = 16 * kSub;
-  extern __shared__ __align__(16) float smem[];  // [kWarps][16][kDP] o, [kWarps][16] m, l; words
-  float* s_o = smem;
-  float* s_m = s_o + kWarps * 16 * kDP;
-  float* s_l = s_m + kWarps * 16;
-  uint32_t* s_words = reinterpret_cast<uint32_t*>(s_l + kWarps * 16);
+// Byte offset of 16-byte chunk `c` of row r in a tile of kN rows: 64-column
+// blocks of kN rows x 128 bytes in the TMA's 128-byte swizzle.
+template <int kN>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return (uint32_t)((c >> 3) * (kN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+template <typename T, int kDP>
+__global__ void __launch_bounds__(kThreads, 3)
+    few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+               const __grid_constant__ FewParams p) {
+  using Smem = FewSmem<kDP>;
+  constexpr int kStages = Smem::kStages, kSteps = kDP / 16, kBlocks = kDP / 64;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                      ~uintptr_t(1023));
+  uint32_t* words = reinterpret_cast<uint32_t*>(&sm + 1);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, t = lane & 3;
   const int unit = blockIdx.x / p.splits, split = blockIdx.x - unit * p.splits;
   const int b = unit / p.Hk, kh = unit - b * p.Hk;
-  // this CTA's words (32 keys each)
-  const int n_words = (p.Sk + kKeys - 1) / kKeys;
-  const int w0 = (int)((int64_t)n_words * split / p.splits);
-  const int w1 = (int)((int64_t)n_words * (split + 1) / p.splits);
+  const int n_tiles = (p.Sk + kKeys - 1) / kKeys;
+  const int t0 = (int)((int64_t)n_tiles * split / p.splits);
+  const int t1 = (int)((int64_t)n_tiles * (split + 1) / p.splits);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], kWarps);
+    }
+    sm.abort = 0;
+    sm.vis_end = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
   pdl_wait();
   pdl_trigger();
 
-  // visible keys, a bit each (only with a mask; keys past Sk count as hidden)
+  // the first tiles are on their way while the queries and the mask are read;
+  // with a mask only one: the keys behind may all be hidden
+  const int ahead = std::min(t1 - t0, p.key_pad ? 1 : kStages);
+  auto load = [&](int i) {
+    const int st = i % kStages;
+    mbar_arrive_expect_tx(&sm.full[st], 2 * Smem::kTile);
+#pragma unroll
+    for (int c = 0; c < kBlocks; ++c) {
+      tma_load_4d(sm.k[st] + c * kKeys * 128, &tm_k, &sm.full[st], c * 64, (t0 + i) * kKeys, kh, b);
+      tma_load_4d(sm.v[st] + c * kKeys * 128, &tm_v, &sm.full[st], c * 64, (t0 + i) * kKeys, kh, b);
+    }
+  };
+  if (warp == kWarps && lane == 0)
+    for (int i = 0; i < ahead; ++i) load(i);
+
+  // queries, rows (head, position) of the group; rows past the end are zero
+  for (int i = threadIdx.x; i < 16 * kDP / 8; i += kThreads) {
+    const int r = i / (kDP / 8), c = i - r * (kDP / 8);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < p.rows && c * 8 < p.D)
+      v = *reinterpret_cast<const uint4*>((const T*)p.q + b * p.qb + (int64_t)(r % p.Sq) * p.qs +
+                                          (int64_t)(kh * p.G + r / p.Sq) * p.qh + c * 8);
+    *reinterpret_cast<uint4*>(sm.q + chunk_at<16>(r, c)) = v;
+  }
+  // visible keys, a bit each (keys past Sk count as hidden), and their end
+  int n_load = t1 - t0;
   if (p.key_pad) {
     const uint8_t* kp = p.key_pad + (int64_t)b * p.Sk;
+    int end = 0;
 #pragma unroll 4
-    for (int w = w0 + warp; w < w1; w += kWarps) {
-      const int key = w * kKeys + lane;
+    for (int w = warp; w < 2 * (t1 - t0); w += kWarps + 1) {
+      const int key = t0 * kKeys + w * 32 + lane;
       const uint32_t bits = __ballot_sync(0xffffffffu, key < p.Sk && __ldg(kp + key) == 0);
-      if (lane == 0) s_words[w - w0] = bits;
+      if (lane == 0) words[w] = bits;
+      if (bits) end = w + 1;
     }
+    if (lane == 0 && end) atomicMax(&sm.vis_end, end);
+    __syncthreads();
+    n_load = std::max(ahead, (sm.vis_end + 1) / 2);
+  } else {
     __syncthreads();
   }
-  auto bits_of = [&](int step) -> uint32_t {  // visible keys of a step, low kStep bits
-    const int key = step * kStep, w = key / kKeys;
-    uint32_t bits;
-    if (p.key_pad)
-      bits = s_words[w - w0];
-    else {
-      const int left = p.Sk - w * kKeys;
-      bits = left >= kKeys ? 0xffffffffu : (1u << left) - 1u;
-    }
-    return kStep == 32 ? bits : (bits >> (key & 31)) & 0xffffu;
-  };
 
-  // query fragments: rows g and g + 8 of the tile, 8 columns per 32-column block
-  uint32_t qa[kB32][2][4];
-  int row_q[2];  // position of the lane's two rows
+  float o[kDP / 8][4];
 #pragma unroll
-  for (int r2 = 0; r2 < 2; ++r2) {
-    const int r = g + 8 * r2;
-    row_q[r2] = r % p.Sq;
-    const T* qr = (const T*)p.q + b * p.qb + (int64_t)row_q[r2] * p.qs +
-                  (int64_t)(kh * p.G + r / p.Sq) * p.qh;
-#pragma unroll
-    for (int c = 0; c < kB32; ++c) {
-      const int col = c * 32 + t * 8;
-      const uint4 v = (r < p.rows && col < p.D) ? *reinterpret_cast<const uint4*>(qr + col)
-                                                : make_uint4(0, 0, 0, 0);
-      qa[c][r2][0] = v.x; qa[c][r2][1] = v.y; qa[c][r2][2] = v.z; qa[c][r2][3] = v.w;
-    }
-  }
-
-  const T* kbase = (const T*)p.k + b * p.kb + kh * p.kh;
-  const T* vbase = (const T*)p.v + b * p.vb + kh * p.vh;
-  uint4 kr[kSub][2][kB32];   // key 8 n + g of a group, columns 32 c + 8 t ..
-  uint4 vr[kSub][4][kVL];    // keys 2t, 2t+1, 2t+8, 2t+9, columns g * kNT ..
-  auto load_k = [&](int step) {
-#pragma unroll
-    for (int s = 0; s < kSub; ++s)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int key = step * kStep + s * 16 + n * 8 + g;
-        const T* row = kbase + (int64_t)key * p.ks;
-#pragma unroll
-        for (int c = 0; c < kB32; ++c) {
-          const int col = c * 32 + t * 8;
-          kr[s][n][c] = (key < p.Sk && col < p.D) ? ldg_stream(row + col) : make_uint4(0, 0, 0, 0);
-        }
-      }
-  };
-  auto load_v = [&](int step) {
-#pragma unroll
-    for (int s = 0; s < kSub; ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = step * kStep + s * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
-        const T* row = vbase + (int64_t)key * p.vs;
-#pragma unroll
-        for (int c = 0; c < kVL; ++c) {
-          const int col = g * kNT + c * 8;
-          vr[s][i][c] = (key < p.Sk && col < p.D) ? ldg_stream(row + col) : make_uint4(0, 0, 0, 0);
-        }
-      }
-  };
-
-  constexpr int kPerWord = kKeys / kStep;
-  const int end = std::min(w1 * kPerWord, (p.Sk + kStep - 1) / kStep);
-  auto visible_from = [&](int step) {
-    while (step < end && bits_of(step) == 0) step += kWarps;
-    return step;
-  };
-
-  float o[kNT][4];
-#pragma unroll
-  for (int n = 0; n < kNT; ++n)
+  for (int n = 0; n < kDP / 8; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const int g = lane >> 2, t = lane & 3;
 
-  int step = visible_from(w0 * kPerWord + warp);
-  if (step < end) {
-    load_k(step);
-    load_v(step);
-  }
-  while (step < end) {
-    const uint32_t bits = bits_of(step);
-    const int next = visible_from(step + kWarps);
-    float s[kSub][2][4];
+  if (warp == kWarps) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      int i = ahead;
+      bool ok = true;
+      for (; i < n_load; ++i) {
+        ok = mbar_wait_bounded(&sm.empty[i % kStages], ((i / kStages) & 1) ^ 1, &sm.abort, p.err,
+                               kWaitNs);
+        if (!ok) break;
+        load(i);
+      }
+      if (!ok) {  // copies in flight land (bounded) before the CTA leaves
+        const uint64_t from = global_timer_ns();
+        for (int j = std::max(0, i - kStages); j < i; ++j)
+          while (!mbar_try_wait(&sm.full[j % kStages], (j / kStages) & 1) &&
+                 global_timer_ns() - from < 100000000ull) {
+          }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ consumers
+    uint32_t qa[kSteps][4];
 #pragma unroll
-    for (int u = 0; u < kSub; ++u)
+    for (int s = 0; s < kSteps; ++s)
+      ldsm4(qa[s], smem_u32(sm.q) + chunk_at<16>((lane & 7) + ((lane >> 3) & 1) * 8, 2 * s + (lane >> 4)));
+    const int row_q[2] = {g % p.Sq, (g + 8) % p.Sq};
+    const int key0 = warp * 16;  // this warp's keys in a tile
+    for (int i = 0; i < n_load; ++i) {
+      const int st = i % kStages;
+      const int first = (t0 + i) * kKeys + key0;  // its first key
+      uint32_t bits = 0xffffu;                    // visible keys among the 16
+      if (p.key_pad)
+        bits = (words[2 * i + (warp >> 1)] >> ((warp & 1) * 16)) & 0xffffu;
+      else if (first + 16 > p.Sk)
+        bits = first < p.Sk ? (1u << (p.Sk - first)) - 1u : 0u;
+      bool ok = mbar_wait_bounded(&sm.full[st], (i / kStages) & 1, &sm.abort, p.err, kWaitNs);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (bits != 0) {
+        const uint32_t kt = smem_u32(sm.k[st]), vt = smem_u32(sm.v[st]);
+        // S = Q K^T: 8 keys per column tile
+        float s[2][4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[u][n][i] = 0.f;
+          for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
-        for (int c = 0; c < kB32; ++c) {
-          const uint32_t a0[4] = {qa[c][0][0], qa[c][1][0], qa[c][0][1], qa[c][1][1]};
-          mma16816<T>(s[u][n], a0, kr[u][n][c].x, kr[u][n][c].y);
-          const uint32_t a1[4] = {qa[c][0][2], qa[c][1][2], qa[c][0][3], qa[c][1][3]};
-          mma16816<T>(s[u][n], a1, kr[u][n][c].z, kr[u][n][c].w);
+        for (int c = 0; c < kSteps; ++c) {
+          uint32_t kf[4];
+          ldsm4(kf, kt + chunk_at<kKeys>(key0 + (lane & 7) + (lane >> 4) * 8, 2 * c + ((lane >> 3) & 1)));
+          mma16816<T>(s[0], qa[c], kf[0], kf[1]);
+          mma16816<T>(s[1], qa[c], kf[2], kf[3]);
+        }
+        // s[n][2 * r2 + j]: row g + 8 r2, key 8 n + 2 t + j
+        const bool all = bits == 0xffffu && !p.causal;
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[n][e] *= p.sl2;
+            if (!all) {
+              const int kk = n * 8 + 2 * t + (e & 1);
+              if (!((bits >> kk) & 1u) || (p.causal && first + kk > row_q[e >> 1])) s[n][e] = -INFINITY;
+            }
+            mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+          }
+        float corr[2], base[2];
+#pragma unroll
+        for (int r2 = 0; r2 < 2; ++r2) {
+          mx[r2] = fmaxf(mx[r2], __shfl_xor_sync(0xffffffffu, mx[r2], 1));
+          mx[r2] = fmaxf(mx[r2], __shfl_xor_sync(0xffffffffu, mx[r2], 2));
+          const float mn = fmaxf(m[r2], mx[r2]);
+          base[r2] = mn == -INFINITY ? 0.f : mn;
+          corr[r2] = ex2(m[r2] - base[r2]);
+          m[r2] = mn;
+        }
+        if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+          l[0] *= corr[0];
+          l[1] *= corr[1];
+#pragma unroll
+          for (int n = 0; n < kDP / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] *= corr[e >> 1];
+        }
+        uint32_t pa[4];  // P as the A fragment, rounded to 16 bits for the product
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float p0 = ex2(s[n][0] - base[0]), p1 = ex2(s[n][1] - base[0]);
+          const float p2 = ex2(s[n][2] - base[1]), p3 = ex2(s[n][3] - base[1]);
+          l[0] += p0 + p1;
+          l[1] += p2 + p3;
+          pa[2 * n] = pack<T>(p0, p1);
+          pa[2 * n + 1] = pack<T>(p2, p3);
+        }
+        // hidden keys' values may hold anything: zero them (0 * NaN is NaN)
+        if (bits != 0xffffu && p.key_pad) {
+          const int r = lane & 15;
+          if (!((bits >> r) & 1u))
+#pragma unroll
+            for (int c = 0; c < kDP / 16; ++c)
+              *reinterpret_cast<uint4*>(sm.v[st] + chunk_at<kKeys>(key0 + r, 2 * c + (lane >> 4))) =
+                  make_uint4(0, 0, 0, 0);
+          fence_proxy_async_shared();  // before the stage's next copy
+          __syncwarp();
+        }
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
+          uint32_t vf[4];
+          ldsm4_t(vf, vt + chunk_at<kKeys>(key0 + (lane & 7) + ((lane >> 3) & 1) * 8, 2 * c + (lane >> 4)));
+          mma16816<T>(o[2 * c], pa, vf[0], vf[1]);
+          mma16816<T>(o[2 * c + 1], pa, vf[2], vf[3]);
         }
       }
-    if (next < end) load_k(next);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[st]);
+    }
+  }
+  __syncthreads();  // every tile has been read: its memory takes the warps' outputs
 
-    // s[u][n][2 * r2 + j]: row g + 8 r2, key 16 u + 8 n + 2 t + j
-    const bool all = bits == (kStep == 32 ? 0xffffffffu : 0xffffu) && !p.causal;
-    float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int u = 0; u < kSub; ++u)
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kk = u * 16 + n * 8 + 2 * t + (i & 1);
-          float x = s[u][n][i] * p.sl2;
-          if (!all && (!((bits >> kk) & 1u) || (p.causal && step * kStep + kk > row_q[i >> 1])))
-            x = -INFINITY;
-          s[u][n][i] = x;
-          mx[i >> 1] = fmaxf(mx[i >> 1], x);
-        }
-    float corr[2], base[2];
+  // join the warps: o[n][2 r2 + j] is row g + 8 r2, column 8 n + 2 t + j
+  float* s_o = reinterpret_cast<float*>(sm.k);
+  if (warp < kWarps) {
 #pragma unroll
     for (int r2 = 0; r2 < 2; ++r2) {
-      mx[r2] = fmaxf(mx[r2], __shfl_xor_sync(0xffffffffu, mx[r2], 1));
-      mx[r2] = fmaxf(mx[r2], __shfl_xor_sync(0xffffffffu, mx[r2], 2));
-      const float mn = fmaxf(m[r2], mx[r2]);
-      base[r2] = mn == -INFINITY ? 0.f : mn;
-      corr[r2] = ex2(m[r2] - base[r2]);
-      m[r2] = mn;
-      l[r2] *= corr[r2];
-    }
-    if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
-#pragma unroll
-      for (int n = 0; n < kNT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] *= corr[i >> 1];
-    }
-#pragma unroll
-    for (int u = 0; u < kSub; ++u) {
-      uint32_t pa[4];  // P as the A fragment (rounded to 16 bits for the product, summed in f32)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float p0 = ex2(s[u][n][0] - base[0]), p1 = ex2(s[u][n][1] - base[0]);
-        const float p2 = ex2(s[u][n][2] - base[1]), p3 = ex2(s[u][n][3] - base[1]);
-        l[0] += p0 + p1;
-        l[1] += p2 + p3;
-        pa[2 * n] = pack<T>(p0, p1);
-        pa[2 * n + 1] = pack<T>(p2, p3);
-      }
-      // hidden keys' values may hold anything: zero them (0 * NaN is NaN)
-      if (!all) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!((bits >> (u * 16 + 2 * t + (i & 1) + 8 * (i >> 1))) & 1u))
-#pragma unroll
-            for (int c = 0; c < kVL; ++c) vr[u][i][c] = make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int c = 0; c < kVL; ++c) {
-        const uint32_t x0[4] = {vr[u][0][c].x, vr[u][0][c].y, vr[u][0][c].z, vr[u][0][c].w};
-        const uint32_t x1[4] = {vr[u][1][c].x, vr[u][1][c].y, vr[u][1][c].z, vr[u][1][c].w};
-        const uint32_t x2[4] = {vr[u][2][c].x, vr[u][2][c].y, vr[u][2][c].z, vr[u][2][c].w};
-        const uint32_t x3[4] = {vr[u][3][c].x, vr[u][3][c].y, vr[u][3][c].z, vr[u][3][c].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mma16816<T>(o[c * 8 + 2 * j], pa, __byte_perm(x0[j], x1[j], 0x5410),
-                      __byte_perm(x2[j], x3[j], 0x5410));
-          mma16816<T>(o[c * 8 + 2 * j + 1], pa, __byte_perm(x0[j], x1[j], 0x7632),
-                      __byte_perm(x2[j], x3[j], 0x7632));
+      l[r2] += __shfl_xor_sync(0xffffffffu, l[r2], 1);
+      l[r2] += __shfl_xor_sync(0xffffffffu, l[r2], 2);
+      const int r = g + 8 * r2;
+      if (r < p.rows) {
+        if (t == 0) {
+          sm.m[warp][r] = m[r2];
+          sm.l[warp][r] = l[r2];
         }
-      }
-    }
-    if (next < end) load_v(next);
-    step = next;
-  }
-
-  // join the warps: o[n][2 r2 + j] is row g + 8 r2, column (2 t + j) * kNT + n
 #pragma unroll
-  for (int r2 = 0; r2 < 2; ++r2) {
-    l[r2] += __shfl_xor_sync(0xffffffffu, l[r2], 1);
-    l[r2] += __shfl_xor_sync(0xffffffffu, l[r2], 2);
-    const int r = g + 8 * r2;
-    if (r < p.rows) {
-      if (t == 0) {
-        s_m[warp * 16 + r] = m[r2];
-        s_l[warp * 16 + r] = l[r2];
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float* dst = s_o + (warp * 16 + r) * kDP + (2 * t + j) * kNT;
-#pragma unroll
-        for (int n = 0; n < kNT; n += 4)
-          *reinterpret_cast<float4*>(dst + n) =
-              make_float4(o[n][2 * r2 + j], o[n + 1][2 * r2 + j], o[n + 2][2 * r2 + j],
-                          o[n + 3][2 * r2 + j]);
+        for (int n = 0; n < kDP / 8; ++n)
+          *reinterpret_cast<float2*>(s_o + (warp * 16 + r) * kDP + n * 8 + 2 * t) =
+              make_float2(o[n][2 * r2], o[n][2 * r2 + 1]);
       }
     }
   }
   __syncthreads();
   const int pairs = p.D / 2;
-  for (int i = threadIdx.x; i < p.rows * pairs; i += kWarps * 32) {
+  for (int i = threadIdx.x; i < p.rows * pairs; i += kThreads) {
     const int r = i / pairs, d = 2 * (i - r * pairs);
     float mm = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w * 16 + r]);
+    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm.m[w][r]);
     const float top = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f, a0 = 0.f, a1 = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2(s_m[w * 16 + r] - top);
-      ll = fmaf(s_l[w * 16 + r], f, ll);
+      const float f = ex2(sm.m[w][r] - top);
+      ll = fmaf(sm.l[w][r], f, ll);
       const float2 v = *reinterpret_cast<const float2*>(s_o + (w * 16 + r) * kDP + d);
       a0 = fmaf(v.x, f, a0);
       a1 = fmaf(v.y, f, a1);
@@ -408,17 +424,25 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
   }
 }
 
-constexpr int kWarps64 = 8, kWarps128 = 4;
-
-size_t few_smem(int dp, int warps, int words) {
-  return sizeof(float) * ((size_t)warps * 16 * dp + 2 * warps * 16) + 4ull * words;
-}
-
-template <typename K>
-cudaError_t opt_in(K kernel, size_t smem) {
-  return smem > 48 * 1024
-             ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)
-             : cudaSuccess;
+template <typename T, int kDP>
+cudaError_t run_few(const CrossAttnArgs& a, const FewParams& p, cudaStream_t st) {
+  CUtensorMap mk, mv;
+  if (!cross_attn_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kKeys) ||
+      !cross_attn_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kKeys))
+    return cudaErrorInvalidValue;
+  const int64_t ctas = (int64_t)a.B * a.Hk * p.splits;
+  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  const int tiles = (a.Sk + kKeys - 1) / kKeys;
+  const size_t words = a.key_pad ? 2 * (size_t)((tiles + p.splits - 1) / p.splits) : 0;
+  static std::atomic<uint64_t> done{0};
+  constexpr size_t base = sizeof(FewSmem<kDP>) + 1024;
+  cudaError_t e = cross_attn_opt_in((const void*)few_kernel<T, kDP>, base + 4 * kMaxWords, done);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(few_kernel<T, kDP>, dim3((unsigned)ctas), dim3(kThreads), base + 4 * words, st, mk,
+                 mv, p);
+  if (e != cudaSuccess) return e;
+  note_launch();
+  return cudaSuccess;
 }
 
 }  // namespace
@@ -427,51 +451,38 @@ bool cross_attn_is_few(const CrossAttnArgs& a) {
   return (int64_t)a.Sq * (a.H / a.Hk) <= kCrossFewRows;
 }
 
-// Key ranges per memory head: enough CTAs for two per SM, each with four steps
-// or more of keys per warp (a shorter range costs more in its join than it
-// saves), and no more mask words than a CTA's shared memory holds.
+// Key ranges per memory head: as many CTAs as fit the SMs at once (three each),
+// with four tiles or more in a range (a shorter one costs more in its join than
+// it saves), and no more mask words than a CTA's shared memory holds.
 int cross_attn_few_splits(const CrossAttnArgs& a) {
-  const int warps = a.D <= 64 ? kWarps64 : kWarps128, step = a.D <= 64 ? 32 : 16;
   const int64_t units = (int64_t)a.B * a.Hk;
-  const int64_t want = (2ll * num_sms() + units - 1) / units;
-  const int64_t fit = std::max<int64_t>(1, a.Sk / (4ll * warps * step));
-  const int64_t words = ((int64_t)a.Sk + kKeys - 1) / kKeys;
-  const int64_t need = (words + kMaxWords - 1) / kMaxWords;
-  return (int)std::max<int64_t>(need, std::min<int64_t>(want, fit));
+  const int64_t tiles = ((int64_t)a.Sk + kKeys - 1) / kKeys;
+  const int64_t want = std::min(3ll * num_sms() / units, (long long)(tiles / 4));
+  const int64_t need = (2 * tiles + kMaxWords - 1) / kMaxWords;
+  return (int)std::max<int64_t>({1, a.key_pad ? need : 1, want});
 }
 
 cudaError_t launch_cross_attn_few(const CrossAttnArgs& a, cudaStream_t st) {
   FewParams p{};
-  p.q = a.q; p.k = a.k; p.v = a.v; p.out = a.out; p.lse2 = a.lse2; p.key_pad = a.key_pad;
+  p.q = a.q; p.out = a.out; p.lse2 = a.lse2; p.key_pad = a.key_pad;
   p.qb = a.q_st[0]; p.qs = a.q_st[1]; p.qh = a.q_st[2];
-  p.kb = a.k_st[0]; p.ks = a.k_st[1]; p.kh = a.k_st[2];
-  p.vb = a.v_st[0]; p.vs = a.v_st[1]; p.vh = a.v_st[2];
   p.B = a.B; p.Sq = a.Sq; p.Sk = a.Sk; p.H = a.H; p.Hk = a.Hk; p.D = a.D;
   p.G = a.H / a.Hk;
   p.rows = p.G * a.Sq;
   p.splits = cross_attn_few_splits(a);
   p.causal = a.causal;
   p.sl2 = a.scale * kLog2e;
+  p.err = default_err_word();
   if (p.splits > 1) {
     if (!a.partials) return cudaErrorInvalidValue;
     p.part_o = a.partials;
     p.part_lse = a.partials + (int64_t)p.splits * a.B * a.Sq * a.H * a.D;
   }
-  const int64_t ctas = (int64_t)a.B * a.Hk * p.splits;
-  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-  const int words = a.key_pad ? ((a.Sk + kKeys - 1) / kKeys + p.splits - 1) / p.splits + 1 : 0;
   const bool wide = a.D > 64;
-  const int warps = wide ? kWarps128 : kWarps64;
-  const size_t smem = few_smem(wide ? 128 : 64, warps, words);
-  void (*k)(FewParams) = a.half ? (wide ? few_kernel<__half, 128, 1, kWarps128>
-                                        : few_kernel<__half, 64, 2, kWarps64>)
-                                : (wide ? few_kernel<__nv_bfloat16, 128, 1, kWarps128>
-                                        : few_kernel<__nv_bfloat16, 64, 2, kWarps64>);
-  cudaError_t e = opt_in(k, smem);
+  const cudaError_t e =
+      a.half ? (wide ? run_few<__half, 128>(a, p, st) : run_few<__half, 64>(a, p, st))
+             : (wide ? run_few<__nv_bfloat16, 128>(a, p, st) : run_few<__nv_bfloat16, 64>(a, p, st));
   if (e != cudaSuccess) return e;
-  e = launch_pdl(k, dim3((unsigned)ctas), dim3(warps * 32), smem, st, p);
-  if (e != cudaSuccess) return e;
-  note_launch();
   return p.splits > 1 ? launch_cross_attn_join(a, p.splits, st) : cudaGetLastError();
 }
 
