@@ -61,6 +61,10 @@ struct Type<__nv_bfloat16> {
   static constexpr uint32_t kIdesc = 1;  // tcgen05 kind::f16 operand format
   static constexpr float kShift = 0.f;
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+  static __device__ __forceinline__ uint64_t unpack(uint32_t v) {
+    const float2 f = unpack_bf16x2(v);
+    return f2_pack(f.x, f.y);
+  }
 };
 template <>
 struct Type<__half> {
@@ -72,6 +76,10 @@ struct Type<__half> {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  static __device__ __forceinline__ uint64_t unpack(uint32_t v) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    return f2_pack(f.x, f.y);
+  }
 };
 
 __host__ __device__ constexpr uint32_t idesc(uint32_t fmt, uint32_t M, uint32_t N, uint32_t b_mn) {
@@ -81,6 +89,11 @@ __host__ __device__ constexpr uint32_t idesc(uint32_t fmt, uint32_t M, uint32_t 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 
@@ -116,14 +129,11 @@ __device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a_tmem, uint32_t b
 // Zero the rows of a streamed tile whose bit in words is clear (thread `tid` of
 // `nthreads`), before a product reads them as B.
 template <int kN, int kDP>
-__device__ __forceinline__ void zero_hidden_rows(uint8_t* tile, const uint32_t (&words)[kN / 32],
-                                                 int tid, int nthreads) {
+__device__ __forceinline__ void zero_hidden_rows(uint8_t* tile, uint2 words, int tid, int nthreads) {
+  static_assert(kN == 64, "two words");
   for (int i = tid; i < kN * (kDP / 64); i += nthreads) {
     const int row = i % kN;
-    uint32_t word = words[0];  // words stay in registers: no index at run time
-#pragma unroll
-    for (int w = 1; w < kN / 32; ++w) word = row / 32 == w ? words[w] : word;
-    if (!((word >> (row % 32)) & 1u)) {
+    if (!(((row < 32 ? words.x : words.y) >> (row % 32)) & 1u)) {
       uint4* r = reinterpret_cast<uint4*>(tile + (i / kN) * kN * 128 + row * 128);
 #pragma unroll
       for (int c = 0; c < 8; ++c) r[c] = make_uint4(0, 0, 0, 0);
@@ -164,31 +174,31 @@ __device__ __forceinline__ void settle(uint64_t* bar, uint32_t issued) {
 }
 
 // ============================================================== forward
-// One item: 128 queries of a head, and a range of its key tiles. Warps: 0 TMA,
-// 1 MMA, 2..5 softmax (a row per thread). Two CTAs per SM (256 TMEM columns,
-// 97 KB of shared memory each) cover each other's waits.
-//   kDP =  64: tiles of 128 keys; S at 0 (128 columns), P at 128 (64), O at 192:
-//              the next S starts once this one has been read.
-//   kDP = 128: tiles of 64 keys; S double-buffered at 0 and 64 with P over its
-//              own scores, O at 128.
+// One item: 128 queries of a head, and a range of its key tiles (64 keys).
+// Warps: 0 TMA, 1 MMA, 2..5 softmax (a row per thread: 64 scores in registers).
+// Two CTAs per SM (256 TMEM columns, 97 KB of shared memory each) cover each
+// other's waits. TMEM: two score buffers at 0 and 64, P over its own scores, O
+// at 128. S of a tile is computed while the softmax works on the one before;
+// P V of a tile is issued behind S of the next.
+constexpr int kN = 64;
+constexpr uint32_t kTmemO = 128;
+constexpr int kFwdThreads = 192;
 template <int kDP>
 struct FwdGeo {
-  static constexpr int kN = kDP == 64 ? 128 : 64;
   static constexpr int kQBufs = kDP == 64 ? 2 : 1;
-  static constexpr int kStages = 2;
-  static constexpr uint32_t kO = kDP == 64 ? 192 : 128;
+  static constexpr int kStages = kDP == 64 ? 4 : 2;
 };
-constexpr int kFwdThreads = 192;
 
 template <int kDP>
 struct FwdSmem {
   using G = FwdGeo<kDP>;
   uint8_t q[G::kQBufs][kRows * kDP * 2];
-  uint8_t k[G::kStages][G::kN * kDP * 2];
-  uint8_t v[G::kStages][G::kN * kDP * 2];
-  uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], s_free, p_full, pv_done;
-  uint64_t drain;
+  uint8_t k[G::kStages][kN * kDP * 2];
+  uint8_t v[G::kStages][kN * kDP * 2];
+  uint64_t q_full[G::kQBufs], q_empty[G::kQBufs];
+  uint64_t k_full[G::kStages], k_empty[G::kStages], v_full[G::kStages], v_empty[G::kStages];
+  uint64_t s_full[2], p_full[2], pv_done[2], drain;  // [2]: by tile parity (a softmax warp
+                                                     // may be a tile ahead of another)
   uint32_t tmem_base, abort;
 };
 
@@ -197,7 +207,6 @@ struct FwdSmem {
 struct FwdItem {
   int qt, h, b, split, lo, hi;  // key tiles [lo, hi)
 };
-template <int kN>
 __device__ __forceinline__ FwdItem fwd_item(const Shape& s, int item, int n_qt) {
   FwdItem it;
   it.split = item % s.splits;
@@ -215,11 +224,11 @@ __device__ __forceinline__ FwdItem fwd_item(const Shape& s, int item, int n_qt) 
   return it;
 }
 
-// Visible-key words of the tile at key k0 (keys past Sk are clear).
-template <int kN>
-__device__ __forceinline__ void tile_words(const Shape& s, int b, int k0, uint32_t (&w)[kN / 32]) {
+// Visible-key words of the 64 keys from k0 (keys past Sk are clear).
+__device__ __forceinline__ uint2 tile_words(const Shape& s, int b, int k0) {
+  uint32_t w[2];
 #pragma unroll
-  for (int i = 0; i < kN / 32; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const int at = k0 / 32 + i;
     if (s.words) {
       w[i] = at < s.nwords ? __ldg(s.words + (int64_t)b * s.nwords + at) : 0u;
@@ -228,7 +237,9 @@ __device__ __forceinline__ void tile_words(const Shape& s, int b, int k0, uint32
       w[i] = left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
     }
   }
+  return make_uint2(w[0], w[1]);
 }
+__device__ __forceinline__ bool is_whole(uint2 w) { return (w.x & w.y) == 0xffffffffu; }
 
 template <typename T, int kDP>
 __global__ void __launch_bounds__(kFwdThreads, 2)
@@ -238,7 +249,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
                      T* __restrict__ out, float* __restrict__ lse2, float* __restrict__ part_o,
                      float* __restrict__ part_lse, int n_items, int n_qt) {
   using Geo = FwdGeo<kDP>;
-  constexpr int kN = Geo::kN;
+  constexpr uint32_t kStages = Geo::kStages, kQBufs = Geo::kQBufs;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   FwdSmem<kDP>& sm = *reinterpret_cast<FwdSmem<kDP>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -246,18 +257,22 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
   const Waiter wait{&sm.abort, sh.err};
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (uint32_t i = 0; i < kQBufs; ++i) {
       mbar_init(&sm.q_full[i], 1);
       mbar_init(&sm.q_empty[i], 1);
+    }
+    for (uint32_t i = 0; i < kStages; ++i) {
       mbar_init(&sm.k_full[i], 1);
       mbar_init(&sm.k_empty[i], 1);
       mbar_init(&sm.v_full[i], 1);
       mbar_init(&sm.v_empty[i], 1);
-      mbar_init(&sm.s_full[i], 1);
     }
-    mbar_init(&sm.s_free, 4);
-    mbar_init(&sm.p_full, 4);
-    mbar_init(&sm.pv_done, 1);
+    mbar_init(&sm.s_full[0], 1);
+    mbar_init(&sm.s_full[1], 1);
+    mbar_init(&sm.p_full[0], 4);
+    mbar_init(&sm.p_full[1], 4);
+    mbar_init(&sm.pv_done[0], 1);
+    mbar_init(&sm.pv_done[1], 1);
     mbar_init(&sm.drain, 1);
     sm.abort = 0;
     fence_mbar_init();
@@ -282,16 +297,16 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       uint32_t n = 0, t = 0;
       bool ok = true;
       for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-        const FwdItem it = fwd_item<kN>(sh, item, n_qt);
+        const FwdItem it = fwd_item(sh, item, n_qt);
         if (it.lo >= it.hi) continue;
-        const uint32_t qb = n % Geo::kQBufs;
-        if (!(ok = wait(&sm.q_empty[qb], ((n / Geo::kQBufs) & 1) ^ 1))) break;
+        const uint32_t qb = n % kQBufs;
+        if (!(ok = wait(&sm.q_empty[qb], ((n / kQBufs) & 1) ^ 1))) break;
         mbar_arrive_expect_tx(&sm.q_full[qb], kRows * kDP * 2);
         load_tile<kRows, kDP>(sm.q[qb], &tm_q, &sm.q_full[qb], it.qt * kRows, it.h, it.b);
         ++n;
         const int kh = it.h / sh.G;
         for (int j = it.lo; j < it.hi; ++j, ++t) {
-          const uint32_t st = t & 1, par = ((t >> 1) & 1) ^ 1;
+          const uint32_t st = t % kStages, par = ((t / kStages) & 1) ^ 1;
           if (!(ok = wait(&sm.k_empty[st], par))) break;
           mbar_arrive_expect_tx(&sm.k_full[st], kN * kDP * 2);
           load_tile<kN, kDP>(sm.k[st], &tm_k, &sm.k_full[st], j * kN, kh, it.b);
@@ -301,11 +316,10 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         }
       }
       if (!ok) {
-        for (uint32_t i = 0; i < Geo::kQBufs; ++i)
-          settle(&sm.q_full[i], (n + Geo::kQBufs - 1 - i) / Geo::kQBufs);
-        for (uint32_t i = 0; i < 2; ++i) {
-          settle(&sm.k_full[i], (t + 2 - i) / 2);
-          settle(&sm.v_full[i], (t + 1 - i) / 2);
+        for (uint32_t i = 0; i < kQBufs; ++i) settle(&sm.q_full[i], (n + kQBufs - 1 - i) / kQBufs);
+        for (uint32_t i = 0; i < kStages; ++i) {
+          settle(&sm.k_full[i], (t + kStages - i) / kStages);
+          settle(&sm.v_full[i], (t + kStages - 1 - i) / kStages);
         }
       }
     }
@@ -315,45 +329,43 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     if (elect_one_sync()) {
       constexpr uint32_t id_s = idesc(Type<T>::kIdesc, kRows, kN, 0);
       constexpr uint32_t id_o = idesc(Type<T>::kIdesc, kRows, kDP, 1);
-      const uint32_t t_o = tmem + Geo::kO;
       uint32_t n = 0, t = 0;  // t: tile whose S is issued next
       bool ok = true, issued = false;
       // P V of tile u (the u-th of this CTA)
       auto issue_pv = [&](uint32_t u, bool acc) -> bool {
-        if (!wait(&sm.v_full[u & 1], (u >> 1) & 1)) return false;
-        if (!wait(&sm.p_full, u & 1)) return false;
+        const uint32_t st = u % kStages;
+        if (!wait(&sm.v_full[st], (u / kStages) & 1)) return false;
+        if (!wait(&sm.p_full[u & 1], (u >> 1) & 1)) return false;
         tc_fence_after();
-        const uint32_t t_p = tmem + (kDP == 64 ? 128u : (u & 1) * 64u);
-        mma_cols<kN, kDP>(t_o, t_p, smem_u32(sm.v[u & 1]), id_o, acc);
-        umma_commit(&sm.v_empty[u & 1]);
-        umma_commit(&sm.pv_done);
+        mma_cols<kN, kDP>(tmem + kTmemO, tmem + (u & 1) * 64u, smem_u32(sm.v[st]), id_o, acc);
+        umma_commit(&sm.pv_done[u & 1]);
+        umma_commit(&sm.v_empty[st]);
         return true;
       };
       // P V of a tile is issued behind S of the next one, over item borders too
       // where the next item's Q has a buffer of its own
       bool behind = false, behind_acc = false;
       for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-        const FwdItem it = fwd_item<kN>(sh, item, n_qt);
+        const FwdItem it = fwd_item(sh, item, n_qt);
         if (it.lo >= it.hi) continue;
-        const uint32_t qb = n % Geo::kQBufs;
-        if (Geo::kQBufs == 1 && behind) {
+        const uint32_t qb = n % kQBufs;
+        if (kQBufs == 1 && behind) {
           if (!(ok = issue_pv(t - 1, behind_acc))) break;
           behind = false;
         }
-        if (!(ok = wait(&sm.q_full[qb], (n / Geo::kQBufs) & 1))) break;
+        if (!(ok = wait(&sm.q_full[qb], (n / kQBufs) & 1))) break;
         ++n;
         const uint32_t q_addr = smem_u32(sm.q[qb]);
         for (int j = it.lo; j < it.hi; ++j, ++t) {
-          if (!(ok = wait(&sm.k_full[t & 1], (t >> 1) & 1))) break;
-          // the single S buffer has been read (kDP = 64); with two, S of tile
-          // t - 2 became P, whose product was issued before this one
-          if (kDP == 64 && !(ok = wait(&sm.s_free, (t & 1) ^ 1))) break;
+          const uint32_t st = t % kStages;
+          if (!(ok = wait(&sm.k_full[st], (t / kStages) & 1))) break;
           tc_fence_after();
-          mma_rows<kRows, kN, kDP>(tmem + (kDP == 64 ? 0u : (t & 1) * 64u), q_addr,
-                                   smem_u32(sm.k[t & 1]), id_s);
+          // this buffer's scores of tile t - 2 became P, whose product was
+          // issued before: in order
+          mma_rows<kRows, kN, kDP>(tmem + (t & 1) * 64u, q_addr, smem_u32(sm.k[st]), id_s);
           issued = true;
-          umma_commit(&sm.k_empty[t & 1]);
           umma_commit(&sm.s_full[t & 1]);
+          umma_commit(&sm.k_empty[st]);
           if (j == it.hi - 1) umma_commit(&sm.q_empty[qb]);
           if (behind && !(ok = issue_pv(t - 1, behind_acc))) break;
           behind = true;
@@ -371,148 +383,119 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     // ------------------------------------------------------------ softmax
     const int r = (warp & 3) * 32 + lane;  // query row within the tile
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_o = tmem + Geo::kO + lanes;
+    const uint32_t t_o = tmem + kTmemO + lanes;
     const float sl2 = sh.scale * kLog2e;
     const uint64_t sl2x2 = f2_splat(sl2);
     uint32_t t = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-      const FwdItem it = fwd_item<kN>(sh, item, n_qt);
+      const FwdItem it = fwd_item(sh, item, n_qt);
       const int qi = it.qt * kRows + r;
-      float m_ref = -INFINITY, l = 0.f;  // reference maximum (scaled, log2 units), row sum
+      // tiles before `plain` hold no hidden score
+      int plain = sh.Sk / kN;
+      if (sh.causal) plain = min(plain, (it.qt * kRows + 1) / kN);
+      if (sh.words) plain = 0;
+      // Reference maximum (scaled, log2 units). l sums P as computed, for the
+      // lse; lr sums P as rounded for the product, which O is divided by: a
+      // row's O is then a mean of its values with weights that add up to 1.
+      float m_ref = -INFINITY, l = 0.f, lr = 0.f;
+      uint2 words = sh.words && it.lo < it.hi ? tile_words(sh, it.b, it.lo * kN) : make_uint2(0, 0);
       for (int j = it.lo; j < it.hi; ++j, ++t) {
-        const int k0 = j * kN;
-        uint32_t words[kN / 32];
-        tile_words<kN>(sh, it.b, k0, words);
-        bool mixed = false;  // the tile holds hidden keys (not counting those past Sk)
-        if (sh.words) {
-#pragma unroll
-          for (int i = 0; i < kN / 32; ++i) {
-            const int left = sh.Sk - k0 - 32 * i;
-            const uint32_t whole = left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
-            mixed |= words[i] != whole;
-          }
-        }
-        const uint32_t t_s = tmem + lanes + (kDP == 64 ? 0u : (t & 1) * 64u);
-        const uint32_t t_p = kDP == 64 ? tmem + lanes + 128u : t_s;
-        const bool diag = sh.causal && k0 + kN - 1 > it.qt * kRows;
+        const uint32_t t_s = tmem + lanes + (t & 1) * 64u;
         ok = wait(&sm.s_full[t & 1], (t >> 1) & 1);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
-        // scores of 32 columns, hidden ones -inf
-        auto scores = [&](int c, const uint32_t (&raw)[32], float (&v)[32]) {
+        uint32_t v[64];  // the row's scores
+        tmem_ld_64cols(t_s, v);
+        tmem_ld_wait();
+        if (j >= plain) {  // hidden scores become -inf
+          const uint2 w = sh.words ? words : tile_words(sh, it.b, j * kN);
+          if (sh.words && j + 1 < it.hi) words = tile_words(sh, it.b, (j + 1) * kN);
+          const int lim = sh.causal ? qi - j * kN : kN;  // last visible column
+          if (!is_whole(w) || __any_sync(0xffffffffu, lim < kN - 1)) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
-          if (words[c] != 0xffffffffu) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = (words[c] >> i) & 1u ? v[i] : -INFINITY;
-          }
-          if (diag) {
-            const int lim = qi - (k0 + c * 32);  // last visible column
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = i <= lim ? v[i] : -INFINITY;
-          }
-        };
-        // pass 1: row maximum of the raw scores (the scale is positive)
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c2 = 0; c2 < kN / 64; ++c2) {
-          uint32_t raw[2][32];
-          tmem_ld_32cols(t_s + c2 * 64, raw[0]);
-          tmem_ld_32cols(t_s + c2 * 64 + 32, raw[1]);
-          tmem_ld_wait();
-#pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2) {
-            float v[32];
-            scores(c2 * 2 + h2, raw[h2], v);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
+            for (int i = 0; i < 64; ++i)
+              v[i] = (((i < 32 ? w.x : w.y) >> (i % 32)) & 1u) && i <= lim ? v[i] : 0xff800000u;
+            if (sh.words && !is_whole(w)) {
+              const uint32_t st = t % kStages;
+              ok = wait(&sm.v_full[st], (t / kStages) & 1);
+              if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+              zero_hidden_rows<kN, kDP>(sm.v[st], w, threadIdx.x - 64, 128);
+            }
           }
         }
-        const float mraw = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 64; i += 2)
+          m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        const float mraw = max3(m4[0], m4[1], fmaxf(m4[2], m4[3]));
         const float mx = mraw == -INFINITY ? -INFINITY : mraw * sl2;
         // the reference moves only when the maximum grew by more than the
         // threshold, so O is seldom rescaled
         const bool move = mx > m_ref + kRescaleThreshold;
-        const float m_new = move ? mx : m_ref;
-        const float corr = (move && m_ref != -INFINITY) ? ex2(m_ref - m_new) : 1.f;
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        m_ref = m_new;
-        // P V of the tile before reads P (kDP = 64) and writes O
-        if (j > it.lo) {
-          ok = wait(&sm.pv_done, (t - 1) & 1);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          tc_fence_after();
-        }
-        // pass 2: P = 2^(c s - m) as 16-bit pairs, row sum of the f32 values
-        const uint64_t neg_m = f2_splat(-m_use);
-        uint64_t la = f2_splat(0.f), lb = f2_splat(0.f);
+        if (__any_sync(0xffffffffu, move)) {
+          const float c = (move && m_ref != -INFINITY) ? ex2(m_ref - mx) : 1.f;
+          if (move) m_ref = mx;
+          l *= c;
+          lr *= c;
+          if (j > it.lo) {
+            // P V of the tile before adds to O no more. (Not waited for at every
+            // tile: of this barrier's phases all but that one are complete,
+            // since S of this tile is.)
+            ok = wait(&sm.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll 1
+            for (int k = 0; k < kDP / 16; ++k) {
+              uint32_t o[16];
+              tmem_ld_16cols(t_o + k * 16, o);
+              tmem_ld_wait();
 #pragma unroll
-        for (int c2 = 0; c2 < kN / 64; ++c2) {
-          uint32_t raw[2][32];
-          tmem_ld_32cols(t_s + c2 * 64, raw[0]);
-          tmem_ld_32cols(t_s + c2 * 64 + 32, raw[1]);
-          tmem_ld_wait();
-          if (kDP == 64 && c2 == kN / 64 - 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.s_free);
-          }
-#pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2) {
-            const int c = c2 * 2 + h2;
-            float v[32];
-            scores(c, raw[h2], v);
-            uint32_t pw[16];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float a0, a1;
-              f2_unpack(f2_fma(f2_pack(v[i], v[i + 1]), sl2x2, neg_m), a0, a1);
-              const float p0 = ex2(a0), p1 = ex2(a1);
-              if (i & 2)
-                lb = f2_add(lb, f2_pack(p0, p1));
-              else
-                la = f2_add(la, f2_pack(p0, p1));
-              pw[i / 2] = Type<T>::pack(p0, p1);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
+              tmem_st_16cols(t_o + k * 16, o);
             }
-            tmem_st_16cols(t_p + c * 16, pw);
           }
         }
-        float la0, la1, lb0, lb1;
-        f2_unpack(la, la0, la1);
-        f2_unpack(lb, lb0, lb1);
-        l = l * corr + ((la0 + la1) + (lb0 + lb1));
-        if (j > it.lo && __any_sync(0xffffffffu, corr != 1.f)) {
+        // P = 2^(c s - m) as 16-bit pairs
+        const uint64_t neg_m = f2_splat(m_ref == -INFINITY ? 0.f : -m_ref);
+        uint64_t a[2] = {f2_splat(0.f), f2_splat(0.f)}, b[2] = {f2_splat(0.f), f2_splat(0.f)};
 #pragma unroll
-          for (int c = 0; c < kDP / 16; ++c) {
-            uint32_t o[16];
-            tmem_ld_16cols(t_o + c * 16, o);
-            tmem_ld_wait();
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pw[8];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-            tmem_st_16cols(t_o + c * 16, o);
+          for (int i = 0; i < 8; ++i) {
+            float a0, a1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c * 16 + 2 * i]),
+                                     __uint_as_float(v[c * 16 + 2 * i + 1])), sl2x2, neg_m), a0, a1);
+            const float p0 = ex2(a0), p1 = ex2(a1);
+            pw[i] = Type<T>::pack(p0, p1);
+            a[i & 1] = f2_add(a[i & 1], f2_pack(p0, p1));
+            b[i & 1] = f2_add(b[i & 1], Type<T>::unpack(pw[i]));
           }
+          tmem_st_8cols(t_s + c * 8, pw);
         }
-        if (mixed) {
-          ok = wait(&sm.v_full[t & 1], (t >> 1) & 1);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          zero_hidden_rows<kN, kDP>(sm.v[t & 1], words, threadIdx.x - 64, 128);
-        }
+        float x0, x1;
+        f2_unpack(f2_add(a[0], a[1]), x0, x1);
+        l += x0 + x1;
+        f2_unpack(f2_add(b[0], b[1]), x0, x1);
+        lr += x0 + x1;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full);
+        if (lane == 0) mbar_arrive(&sm.p_full[t & 1]);
       }
       if (!ok) break;
       // ---- output: O / l and lse
       const bool any = it.lo < it.hi;
       if (any) {
-        ok = wait(&sm.pv_done, (t - 1) & 1);
+        ok = wait(&sm.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
       }
-      const bool none = l == 0.f;  // (a NaN sum is not equal and passes through)
-      const float inv_l = none ? 0.f : 1.f / l;
+      // no visible key: zeros (a NaN sum passes through). Rounded, P is not 0 where
+      // l is not: the row's maximum is at least 2^0 of its reference.
+      const bool none = l == 0.f;
+      const float inv_l = none ? 0.f : 1.f / lr;
       const int64_t rows_all = (int64_t)sh.B * sh.Sq * sh.H;
       const int64_t orow = ((int64_t)it.b * sh.Sq + qi) * sh.H + it.h;
       const int64_t lrow = ((int64_t)it.b * sh.H + it.h) * sh.Sq + qi;
@@ -906,8 +889,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int j = it.lo + (int)((u0 ^ (uint32_t)group) & 1u); j < it.hi; j += 2) {
         const uint32_t w = u0 + (uint32_t)(j - it.lo), stage = w % kStages;
         const int col0 = kKeys ? (it.first + j % it.n) * kBN : j * kBN;
-        uint32_t words[2] = {0xffffffffu, 0xffffffffu};
-        if (!kKeys) tile_words<kBN>(sh, it.b, col0, words);
+        uint2 words = make_uint2(0xffffffffu, 0xffffffffu);
+        if (!kKeys) words = tile_words(sh, it.b, col0);
         const bool diag = sh.causal && (kKeys ? col0 < it.row0 + kRows - 1
                                               : col0 + kBN - 1 > it.row0);
         // the statistics came with the tile (already complete: S was computed)
@@ -942,7 +925,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             if (kShift != 0.f) d = f2_mul(d, f2_splat(unshift));
             f2_unpack(f2_mul(f2_pack(p0, p1), d), d0, d1);
             if (decltype(masked)::value) {
-              bool v0 = row_ok && ((words[c] >> i) & 1u), v1 = row_ok && ((words[c] >> (i + 1)) & 1u);
+              const uint32_t wc = c == 0 ? words.x : words.y;
+              bool v0 = row_ok && ((wc >> i) & 1u), v1 = row_ok && ((wc >> (i + 1)) & 1u);
               if (diag) {
                 v0 = v0 && (kKeys ? i >= lim : i <= lim);
                 v1 = v1 && (kKeys ? i + 1 >= lim : i + 1 <= lim);
@@ -958,14 +942,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           if (kKeys) tmem_st_16cols(t_s + c * 16, pk);
           tmem_st_16cols(t_s + (kKeys ? 64u : 0u) + c * 16, dk);
         };
-        if (diag || !rows_ok || (words[0] & words[1]) != 0xffffffffu) {
+        if (diag || !rows_ok || !is_whole(words)) {
           columns(0, std::true_type{});
           columns(1, std::true_type{});
         } else {
           columns(0, std::false_type{});
           columns(1, std::false_type{});
         }
-        if (!kKeys && sh.words && (words[0] & words[1]) != 0xffffffffu)
+        if (!kKeys && sh.words && !is_whole(words))
           zero_hidden_rows<kBN, kDP>(sm.b1[stage], words, (warp & 3) * 32 + lane, 128);
         tmem_st_wait();
         tc_fence_before();
@@ -1171,8 +1155,7 @@ int pieces(int64_t items, int64_t places, int64_t tiles) {
 int64_t row_tiles(int n) { return ((int64_t)n + kRows - 1) / kRows; }
 
 int fwd_splits(const CrossAttnArgs& a) {
-  const int kn = a.D <= 64 ? 128 : 64;
-  return pieces(row_tiles(a.Sq) * a.H * a.B, 2ll * num_sms(), ((int64_t)a.Sk + kn - 1) / kn);
+  return pieces(row_tiles(a.Sq) * a.H * a.B, 2ll * num_sms(), ((int64_t)a.Sk + kN - 1) / kN);
 }
 int dq_splits(const CrossAttnArgs& a) {
   return pieces(row_tiles(a.Sq) * a.H * a.B, num_sms(), ((int64_t)a.Sk + kBN - 1) / kBN);
@@ -1187,11 +1170,10 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   const int splits = fwd_splits(a);
   const int64_t rows = (int64_t)a.B * a.Sq * a.H;
   if (splits > 1 && !a.partials) return cudaErrorInvalidValue;
-  constexpr int kn = FwdGeo<kDP>::kN;
   CUtensorMap mq, mk, mv;
   if (!cross_attn_map(&mq, a.q, a.half, a.D, a.Sq, a.H, a.B, a.q_st, kRows) ||
-      !cross_attn_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kn) ||
-      !cross_attn_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kn))
+      !cross_attn_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kN) ||
+      !cross_attn_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kN))
     return cudaErrorInvalidValue;
   static std::atomic<uint64_t> done{0};
   const int smem = (int)sizeof(FwdSmem<kDP>) + 1024;
