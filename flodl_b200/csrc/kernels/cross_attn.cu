@@ -107,23 +107,59 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
     tma_load_4d(dst + c * kN * 128, map, bar, c * 64, row, head, batch);
 }
 
-// D[128, n] (+)= A[128, kDP] B[n, kDP]^T, both tiles K-major in shared memory.
+// The MMA thread's instructions. Descriptors are a constant upper half and a
+// lower half (address / 16) that advances by constants.
+constexpr uint32_t desc_hi(uint32_t sbo) {
+  return ((sbo >> 4) & 0x3FFFu) | (1u << 14) | (2u << 29);  // version, 128-byte swizzle
+}
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) {
+  return (addr >> 4) | ((lbo >> 4) << 16);
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id,
+                                        uint32_t acc) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b64 da, db;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "mov.b64 da, {%1, %5};\n"
+      "mov.b64 db, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(id), "r"(acc), "n"(desc_hi(1024))
+      : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t id,
+                                        uint32_t acc) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b64 db;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "mov.b64 db, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(id), "r"(acc), "n"(desc_hi(1024))
+      : "memory");
+}
+// D[128, n] = A[128, kDP] B[n, kDP]^T, both tiles K-major in shared memory.
 template <int kNA, int kNB, int kDP>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t id) {
+  const uint32_t al = desc_lo(a, 16), bl = desc_lo(b, 16);
 #pragma unroll
   for (int kk = 0; kk < kDP / 16; ++kk)
-    umma_bf16(d, make_sdesc_sw128(a + (kk / 4) * (kNA * 128) + (kk % 4) * 32, 16, 1024),
-              make_sdesc_sw128(b + (kk / 4) * (kNB * 128) + (kk % 4) * 32, 16, 1024), id, kk > 0);
+    umma_ss(d, al + ((kk / 4) * (kNA * 128) + (kk % 4) * 32) / 16,
+            bl + ((kk / 4) * (kNB * 128) + (kk % 4) * 32) / 16, id, kk > 0);
 }
 // D[128, kDP] (+)= A[128, kK] B[kK, kDP], A 16-bit pairs in TMEM, B a streamed
 // tile read along its rows (MN-major).
 template <int kK, int kDP>
 __device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t id,
                                          bool acc) {
+  const uint32_t bl = desc_lo(b, kK * 128);
 #pragma unroll
   for (int kk = 0; kk < kK / 16; ++kk)
-    umma_bf16_tmem_a(d, a_tmem + kk * 8, make_sdesc_sw128(b + kk * 2048, kK * 128, 1024), id,
-                     (acc || kk > 0) ? 1u : 0u);
+    umma_ts(d, a_tmem + kk * 8, bl + kk * 2048 / 16, id, (acc || kk > 0) ? 1u : 0u);
 }
 
 // Zero the rows of a streamed tile whose bit in words is clear (thread `tid` of
@@ -161,6 +197,18 @@ struct Waiter {
   uint32_t* err;
   __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
     return mbar_wait_bounded(bar, parity, abort, err, kWaitNs);
+  }
+};
+
+// Position and parity in a ring of barriers.
+template <uint32_t kSize>
+struct Ring {
+  uint32_t at = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == kSize) {
+      at = 0;
+      phase ^= 1;
+    }
   }
 };
 
@@ -329,17 +377,21 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     if (elect_one_sync()) {
       constexpr uint32_t id_s = idesc(Type<T>::kIdesc, kRows, kN, 0);
       constexpr uint32_t id_o = idesc(Type<T>::kIdesc, kRows, kDP, 1);
-      uint32_t n = 0, t = 0;  // t: tile whose S is issued next
+      const uint32_t q0 = smem_u32(sm.q[0]), k0 = smem_u32(sm.k[0]), v0 = smem_u32(sm.v[0]);
+      Ring<kStages> ks, vs;  // stages of K (tile t) and V (the tile behind)
+      Ring<kQBufs> qs;
+      uint32_t t = 0;  // tile whose S is issued next
       bool ok = true, issued = false;
-      // P V of tile u (the u-th of this CTA)
-      auto issue_pv = [&](uint32_t u, bool acc) -> bool {
-        const uint32_t st = u % kStages;
-        if (!wait(&sm.v_full[st], (u / kStages) & 1)) return false;
+      // P V of tile t - 1
+      auto issue_pv = [&](bool acc) -> bool {
+        const uint32_t u = t - 1;
+        if (!wait(&sm.v_full[vs.at], vs.phase)) return false;
         if (!wait(&sm.p_full[u & 1], (u >> 1) & 1)) return false;
         tc_fence_after();
-        mma_cols<kN, kDP>(tmem + kTmemO, tmem + (u & 1) * 64u, smem_u32(sm.v[st]), id_o, acc);
+        mma_cols<kN, kDP>(tmem + kTmemO, tmem + (u & 1) * 64u, v0 + vs.at * (kN * kDP * 2), id_o, acc);
         umma_commit(&sm.pv_done[u & 1]);
-        umma_commit(&sm.v_empty[st]);
+        umma_commit(&sm.v_empty[vs.at]);
+        vs.next();
         return true;
       };
       // P V of a tile is issued behind S of the next one, over item borders too
@@ -348,31 +400,31 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
         const FwdItem it = fwd_item(sh, item, n_qt);
         if (it.lo >= it.hi) continue;
-        const uint32_t qb = n % kQBufs;
         if (kQBufs == 1 && behind) {
-          if (!(ok = issue_pv(t - 1, behind_acc))) break;
+          if (!(ok = issue_pv(behind_acc))) break;
           behind = false;
         }
-        if (!(ok = wait(&sm.q_full[qb], (n / kQBufs) & 1))) break;
-        ++n;
-        const uint32_t q_addr = smem_u32(sm.q[qb]);
-        for (int j = it.lo; j < it.hi; ++j, ++t) {
-          const uint32_t st = t % kStages;
-          if (!(ok = wait(&sm.k_full[st], (t / kStages) & 1))) break;
+        if (!(ok = wait(&sm.q_full[qs.at], qs.phase))) break;
+        const uint32_t q_addr = q0 + qs.at * (kRows * kDP * 2);
+        for (int j = it.lo; j < it.hi; ++j) {
+          if (!(ok = wait(&sm.k_full[ks.at], ks.phase))) break;
           tc_fence_after();
           // this buffer's scores of tile t - 2 became P, whose product was
           // issued before: in order
-          mma_rows<kRows, kN, kDP>(tmem + (t & 1) * 64u, q_addr, smem_u32(sm.k[st]), id_s);
+          mma_rows<kRows, kN, kDP>(tmem + (t & 1) * 64u, q_addr, k0 + ks.at * (kN * kDP * 2), id_s);
           issued = true;
           umma_commit(&sm.s_full[t & 1]);
-          umma_commit(&sm.k_empty[st]);
-          if (j == it.hi - 1) umma_commit(&sm.q_empty[qb]);
-          if (behind && !(ok = issue_pv(t - 1, behind_acc))) break;
+          umma_commit(&sm.k_empty[ks.at]);
+          ks.next();
+          if (j == it.hi - 1) umma_commit(&sm.q_empty[qs.at]);
+          if (behind && !(ok = issue_pv(behind_acc))) break;
+          ++t;
           behind = true;
           behind_acc = j > it.lo;
         }
+        qs.next();
       }
-      if (ok && behind) ok = issue_pv(t - 1, behind_acc);
+      if (ok && behind) ok = issue_pv(behind_acc);
       if (!ok && issued) {
         umma_commit(&sm.drain);
         settle(&sm.drain, 1);
@@ -651,28 +703,37 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // (A1 = K, A2 = V), the stream is Q, dO of every query head that reads this
 // memory head, acc1 = dS^T Q, acc2 = P^T dO.
 // Warps: 0 TMA, 1 MMA, 2..5 and 6..9 two compute groups that take the streamed
-// tiles of 64 in turn: one group's exponentials run beside the tensor cores'
-// work for the other. TMEM: [S, dP] of two tiles at 0 and 128, acc1 at 256,
-// acc2 behind it; dS lies over S (kKeys: P over S, dS over dP).
+// tiles of 64 in turn. TMEM: [S, dP] of kBufs tiles, 128 columns each, then acc1
+// and acc2; dS lies over S (kKeys: P over S, dS over dP). The products with a
+// tile's dS are issued kBufs - 1 tiles behind its scores: with three buffers
+// (all but the keys' kernel at head size 128, whose accumulators leave room for
+// two) the tensor cores' round trip for a tile - about 1400 cycles from dS to
+// the buffer's next scores - passes while the groups are on two others.
 constexpr int kBN = 64;
 constexpr int kBwdThreads = 320;
 
-template <int kDP>
+// Shared memory: kABufs stationary pairs (two: the next item's loads early) and
+// kStages streamed pairs.
+template <int kDP, bool kKeys, int kABufs>
 struct BwdGeo {
-  static constexpr int kStages = kDP == 64 ? 4 : 3;
+  static constexpr int kBufs = kKeys && kDP == 128 ? 2 : 3;
+  static constexpr int kStages = kDP == 64 ? 6 : (kABufs == 2 ? 3 : 5);
   static constexpr int kABytes = kRows * kDP * 2;
   static constexpr int kBBytes = kBN * kDP * 2;
+  static constexpr uint32_t kAcc = 128 * kBufs;
+  static_assert(kAcc + (kKeys ? 2 : 1) * kDP <= 512, "TMEM columns");
 };
-template <int kDP>
+template <int kDP, bool kKeys, int kABufs>
 struct BwdSmem {
-  using G = BwdGeo<kDP>;
-  uint8_t a1[2][G::kABytes], a2[2][G::kABytes];
+  using G = BwdGeo<kDP, kKeys, kABufs>;
+  uint8_t a1[kABufs][G::kABytes], a2[kABufs][G::kABytes];
   uint8_t b1[G::kStages][G::kBBytes], b2[G::kStages][G::kBBytes];
-  float2 stat[G::kStages][kBN];  // kKeys: the streamed queries' statistics
-  uint64_t a_full[2], a_empty[2], b_full[G::kStages], b_empty[G::kStages];
-  uint64_t s_full[2], ds_full[2], acc_full, acc_free, drain;
+  float2 stat[kKeys ? G::kStages : 1][kBN];  // kKeys: the streamed queries' statistics
+  uint64_t a_full[kABufs], a_empty[kABufs], b_full[G::kStages], b_empty[G::kStages];
+  uint64_t s_full[G::kBufs], ds_full[G::kBufs], acc_full, acc_free, drain;
   uint32_t tmem_base, abort;
 };
+
 struct BwdItem {
   int row0, head, b, split, lo, hi;  // stream tiles [lo, hi); kKeys: tile index = group * n + tile
   int first, n;                      // kKeys: first query tile, query tiles per head
@@ -715,29 +776,32 @@ struct BwdOut {
   float* part;         // [splits][1 or 2][rows][D] when splits > 1
 };
 
-template <typename T, int kDP, bool kKeys>
+template <typename T, int kDP, bool kKeys, int kABufs>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     cross_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1,
                      const __grid_constant__ CUtensorMap tm_a2,
                      const __grid_constant__ CUtensorMap tm_b1,
                      const __grid_constant__ CUtensorMap tm_b2, const __grid_constant__ Shape sh,
                      const float2* __restrict__ stats, const __grid_constant__ BwdOut<T> outs, int n_items, int n_rt) {
-  using Geo = BwdGeo<kDP>;
-  constexpr int kStages = Geo::kStages;
+  using Geo = BwdGeo<kDP, kKeys, kABufs>;
+  using Smem = BwdSmem<kDP, kKeys, kABufs>;
+  constexpr uint32_t kStages = Geo::kStages, kBufs = Geo::kBufs;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  BwdSmem<kDP>& sm = *reinterpret_cast<BwdSmem<kDP>*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                      ~uintptr_t(1023));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const Waiter wait{&sm.abort, sh.err};
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kABufs; ++i) {
       mbar_init(&sm.a_full[i], 1);
       mbar_init(&sm.a_empty[i], 1);
+    }
+    for (uint32_t i = 0; i < kBufs; ++i) {
       mbar_init(&sm.s_full[i], 1);
       mbar_init(&sm.ds_full[i], 4);
     }
-    for (int i = 0; i < kStages; ++i) {
+    for (uint32_t i = 0; i < kStages; ++i) {
       mbar_init(&sm.b_full[i], 1);
       mbar_init(&sm.b_empty[i], 1);
     }
@@ -755,7 +819,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
-  const uint32_t t_acc1 = tmem + 256, t_acc2 = tmem + 256 + kDP;
+  const uint32_t t_acc1 = tmem + Geo::kAcc, t_acc2 = t_acc1 + kDP;
   pdl_wait();
   pdl_trigger();
 
@@ -771,10 +835,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
         const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
         if (it.lo >= it.hi) continue;
-        if (!(ok = wait(&sm.a_empty[n & 1], ((n >> 1) & 1) ^ 1))) break;
-        mbar_arrive_expect_tx(&sm.a_full[n & 1], 2 * Geo::kABytes);
-        load_tile<kRows, kDP>(sm.a1[n & 1], &tm_a1, &sm.a_full[n & 1], it.row0, it.head, it.b);
-        load_tile<kRows, kDP>(sm.a2[n & 1], &tm_a2, &sm.a_full[n & 1], it.row0, it.head, it.b);
+        const uint32_t ab = n % kABufs;
+        if (!(ok = wait(&sm.a_empty[ab], ((n / kABufs) & 1) ^ 1))) break;
+        mbar_arrive_expect_tx(&sm.a_full[ab], 2 * Geo::kABytes);
+        load_tile<kRows, kDP>(sm.a1[ab], &tm_a1, &sm.a_full[ab], it.row0, it.head, it.b);
+        load_tile<kRows, kDP>(sm.a2[ab], &tm_a2, &sm.a_full[ab], it.row0, it.head, it.b);
         ++n;
         for (int j = it.lo; j < it.hi; ++j, ++u) {
           const uint32_t st = u % kStages;
@@ -791,7 +856,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
       if (!ok) {
-        for (uint32_t i = 0; i < 2; ++i) settle(&sm.a_full[i], (n + 1 - i) / 2);
+        for (uint32_t i = 0; i < kABufs; ++i) settle(&sm.a_full[i], (n + kABufs - 1 - i) / kABufs);
         for (uint32_t i = 0; i < kStages; ++i)
           settle(&sm.b_full[i], (u + kStages - 1 - i) / kStages);
       }
@@ -802,51 +867,66 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     if (elect_one_sync()) {
       constexpr uint32_t id_s = idesc(Type<T>::kIdesc, kRows, kBN, 0);
       constexpr uint32_t id_acc = idesc(Type<T>::kIdesc, kRows, kDP, 1);
-      uint32_t n = 0, u = 0, m = 0;  // items started, tiles, items whose products began
+      const uint32_t a10 = smem_u32(sm.a1[0]), a20 = smem_u32(sm.a2[0]);
+      const uint32_t b10 = smem_u32(sm.b1[0]), b20 = smem_u32(sm.b2[0]);
+      Ring<kStages> ss, as;  // stages of the tile whose scores come next, and of the products
+      Ring<kBufs> sb, ab;    // their TMEM buffers
+      Ring<kABufs> is;       // stationary pairs
+      uint32_t m = 0;        // items whose products began
       bool ok = true, issued = false;
-      bool behind = false, behind_first = false, behind_last = false;
-      auto issue_acc = [&](uint32_t w, bool first, bool last) -> bool {
+      // tiles whose products are still to come, the oldest's flags in bit 0
+      uint32_t pending = 0, firsts = 0, lasts = 0;
+      auto issue_acc = [&]() -> bool {
+        const bool first = firsts & 1u, last = lasts & 1u;
+        firsts >>= 1;
+        lasts >>= 1;
+        --pending;
         if (first) {  // the item before has been read out
           if (!wait(&sm.acc_free, (m & 1) ^ 1)) return false;
           ++m;
         }
-        if (!wait(&sm.ds_full[w & 1], (w >> 1) & 1)) return false;
+        if (!wait(&sm.ds_full[ab.at], ab.phase)) return false;
         tc_fence_after();
-        const uint32_t t_s = tmem + (w & 1) * 128u, st = w % kStages;
+        const uint32_t t_s = tmem + ab.at * 128u;
+        const uint32_t b1 = b10 + as.at * Geo::kBBytes, b2 = b20 + as.at * Geo::kBBytes;
         if (kKeys) {
-          mma_cols<kBN, kDP>(t_acc2, t_s, smem_u32(sm.b2[st]), id_acc, !first);
-          mma_cols<kBN, kDP>(t_acc1, t_s + 64, smem_u32(sm.b1[st]), id_acc, !first);
+          mma_cols<kBN, kDP>(t_acc2, t_s, b2, id_acc, !first);
+          mma_cols<kBN, kDP>(t_acc1, t_s + 64, b1, id_acc, !first);
         } else {
-          mma_cols<kBN, kDP>(t_acc1, t_s, smem_u32(sm.b1[st]), id_acc, !first);
+          mma_cols<kBN, kDP>(t_acc1, t_s, b1, id_acc, !first);
         }
-        umma_commit(&sm.b_empty[st]);
+        umma_commit(&sm.b_empty[as.at]);
         if (last) umma_commit(&sm.acc_full);
+        ab.next();
+        as.next();
         return true;
       };
       for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
         const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
         if (it.lo >= it.hi) continue;
-        if (!(ok = wait(&sm.a_full[n & 1], (n >> 1) & 1))) break;
-        const uint32_t a1 = smem_u32(sm.a1[n & 1]), a2 = smem_u32(sm.a2[n & 1]);
-        for (int j = it.lo; j < it.hi; ++j, ++u) {
-          const uint32_t st = u % kStages;
-          if (!(ok = wait(&sm.b_full[st], (u / kStages) & 1))) break;
+        if (kABufs == 1)  // the wait below is long: what is there to do first
+          while (ok && pending) ok = issue_acc();
+        if (!ok || !(ok = wait(&sm.a_full[is.at], is.phase))) break;
+        const uint32_t a1 = a10 + is.at * Geo::kABytes, a2 = a20 + is.at * Geo::kABytes;
+        for (int j = it.lo; j < it.hi; ++j) {
+          if (!(ok = wait(&sm.b_full[ss.at], ss.phase))) break;
           tc_fence_after();
-          // this buffer's last product (tile u - 2) was issued before: in order
-          const uint32_t t_s = tmem + (u & 1) * 128u;
-          mma_rows<kRows, kBN, kDP>(t_s, a1, smem_u32(sm.b1[st]), id_s);
-          mma_rows<kRows, kBN, kDP>(t_s + 64, a2, smem_u32(sm.b2[st]), id_s);
+          // this buffer's last product (kBufs tiles ago) was issued before: in order
+          const uint32_t t_s = tmem + sb.at * 128u;
+          mma_rows<kRows, kBN, kDP>(t_s, a1, b10 + ss.at * Geo::kBBytes, id_s);
+          mma_rows<kRows, kBN, kDP>(t_s + 64, a2, b20 + ss.at * Geo::kBBytes, id_s);
           issued = true;
-          umma_commit(&sm.s_full[u & 1]);
-          if (j == it.hi - 1) umma_commit(&sm.a_empty[n & 1]);
-          if (behind && !(ok = issue_acc(u - 1, behind_first, behind_last))) break;
-          behind = true;
-          behind_first = j == it.lo;
-          behind_last = j == it.hi - 1;
+          umma_commit(&sm.s_full[sb.at]);
+          if (j == it.hi - 1) umma_commit(&sm.a_empty[is.at]);
+          ss.next();
+          sb.next();
+          firsts |= (j == it.lo ? 1u : 0u) << pending;
+          lasts |= (j == it.hi - 1 ? 1u : 0u) << pending;
+          if (++pending == kBufs && !(ok = issue_acc())) break;
         }
-        ++n;
+        is.next();
       }
-      if (ok && behind) ok = issue_acc(u - 1, behind_first, behind_last);
+      while (ok && pending) ok = issue_acc();
       if (!ok && issued) {
         umma_commit(&sm.drain);
         settle(&sm.drain, 1);
@@ -858,7 +938,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int group = (warp - 2) >> 2;
     const int r = (warp & 3) * 32 + lane;  // row within the tile
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lanes + (uint32_t)group * 128u;
     const uint64_t sl2x2 = f2_splat(sh.scale * kLog2e);
     constexpr float kShift = kKeys ? Type<T>::kShift : 0.f;
     const float unshift = exp2f(-kShift);
@@ -887,7 +966,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       // tiles of this group: u counts the CTA's tiles
       const uint32_t u0 = u;
       for (int j = it.lo + (int)((u0 ^ (uint32_t)group) & 1u); j < it.hi; j += 2) {
-        const uint32_t w = u0 + (uint32_t)(j - it.lo), stage = w % kStages;
+        const uint32_t w = u0 + (uint32_t)(j - it.lo), stage = w % kStages, buf = w % kBufs;
+        const uint32_t t_s = tmem + lanes + buf * 128u;
         const int col0 = kKeys ? (it.first + j % it.n) * kBN : j * kBN;
         uint2 words = make_uint2(0xffffffffu, 0xffffffffu);
         if (!kKeys) words = tile_words(sh, it.b, col0);
@@ -895,7 +975,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                                               : col0 + kBN - 1 > it.row0);
         // the statistics came with the tile (already complete: S was computed)
         ok = !kKeys || wait(&sm.b_full[stage], (w / kStages) & 1);
-        ok = ok && wait(&sm.s_full[group], (w >> 1) & 1);
+        ok = ok && wait(&sm.s_full[buf], (w / kBufs) & 1);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
         // 32 columns: P and dS as 16-bit pairs. Hidden pairs are replaced by
@@ -954,7 +1034,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.ds_full[group]);
+        if (lane == 0) mbar_arrive(&sm.ds_full[buf]);
       }
       if (!ok) break;
       u = u0 + (uint32_t)max(0, it.hi - it.lo);
@@ -1191,7 +1271,7 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   return splits > 1 ? launch_cross_attn_join(a, splits, st) : cudaGetLastError();
 }
 
-template <typename T, int kDP, bool kKeys>
+template <typename T, int kDP, bool kKeys, int kABufs>
 cudaError_t run_bwd_half(const CrossAttnArgs& a, cudaStream_t st) {
   const int splits = kKeys ? dkv_splits(a) : dq_splits(a);
   if (splits > 1 && !a.partials) return cudaErrorInvalidValue;
@@ -1203,9 +1283,9 @@ cudaError_t run_bwd_half(const CrossAttnArgs& a, cudaStream_t st) {
       !cross_attn_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kKeys ? rb : cb))
     return cudaErrorInvalidValue;
   static std::atomic<uint64_t> done{0};
-  constexpr int smem = (int)sizeof(BwdSmem<kDP>) + 1024;
+  constexpr int smem = (int)sizeof(BwdSmem<kDP, kKeys, kABufs>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory");
-  auto kernel = cross_bwd_kernel<T, kDP, kKeys>;
+  auto kernel = cross_bwd_kernel<T, kDP, kKeys, kABufs>;
   cudaError_t e = cross_attn_opt_in((const void*)kernel, smem, done);
   if (e != cudaSuccess) return e;
   const int S = kKeys ? a.Sk : a.Sq, heads = kKeys ? a.Hk : a.H;
@@ -1250,11 +1330,19 @@ cudaError_t run_stats(const CrossAttnArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
+constexpr int kLongItem = 1024;  // keys
 template <typename T, int kDP>
 cudaError_t run_bwd(const CrossAttnArgs& a, cudaStream_t st) {
   cudaError_t e = run_stats<T>(a, st);
-  if (e == cudaSuccess) e = run_bwd_half<T, kDP, false>(a, st);
-  if (e == cudaSuccess) e = run_bwd_half<T, kDP, true>(a, st);
+  if (e != cudaSuccess) return e;
+  // At head size 128 the queries' kernel has room for two stationary pairs and
+  // three stages or for one and five: the second where items are long.
+  if constexpr (kDP == 128) {
+    e = a.Sk >= kLongItem ? run_bwd_half<T, kDP, false, 1>(a, st) : run_bwd_half<T, kDP, false, 2>(a, st);
+  } else {
+    e = run_bwd_half<T, kDP, false, 2>(a, st);
+  }
+  if (e == cudaSuccess) e = run_bwd_half<T, kDP, true, 2>(a, st);
   return e;
 }
 
