@@ -186,7 +186,33 @@ struct Shape {
   const int* vis_end;     // [B]
   int nwords;
   uint32_t* err;
+  // item -> (row tile, batch, head, piece): divisors of an item's index
+  FastDiv by_splits, by_bh, by_heads, by_group;
 };
+
+// An item's coordinates: the piece fastest, then heads, batches, row tiles.
+struct ItemAt {
+  int rt, b, head, split;
+};
+__device__ __forceinline__ ItemAt item_at(const Shape& s, int item) {
+  ItemAt a;
+  const uint32_t i = s.by_splits.div(item);
+  a.split = item - i * s.by_splits.d;
+  a.rt = s.by_bh.div(i);
+  const uint32_t bh = i - a.rt * s.by_bh.d;
+  a.b = s.by_heads.div(bh);
+  a.head = bh - a.b * s.by_heads.d;
+  return a;
+}
+// Streamed tiles [lo, hi) of piece `split` of nt.
+__device__ __forceinline__ void piece_of(const Shape& s, int split, int nt, int& lo, int& hi) {
+  lo = 0;
+  hi = nt;
+  if (s.splits > 1) {  // (64-bit divisions: not for every item)
+    lo = (int)((int64_t)nt * split / s.splits);
+    hi = (int)((int64_t)nt * (split + 1) / s.splits);
+  }
+}
 
 __device__ __forceinline__ int visible_end(const Shape& s, int b) {
   return s.vis_end ? __ldg(s.vis_end + b) : s.Sk;
@@ -257,18 +283,14 @@ struct FwdItem {
 };
 __device__ __forceinline__ FwdItem fwd_item(const Shape& s, int item, int n_qt) {
   FwdItem it;
-  it.split = item % s.splits;
-  item /= s.splits;
-  const int n_bh = s.H * s.B;
-  it.qt = n_qt - 1 - item / n_bh;
-  const int bh = item % n_bh;
-  it.h = bh % s.H;
-  it.b = bh / s.H;
+  const ItemAt at = item_at(s, item);
+  it.split = at.split;
+  it.qt = n_qt - 1 - at.rt;
+  it.h = at.head;
+  it.b = at.b;
   int end = visible_end(s, it.b);
   if (s.causal) end = min(end, (it.qt + 1) * kRows);
-  const int nt = (end + kN - 1) / kN;
-  it.lo = (int)((int64_t)nt * it.split / s.splits);
-  it.hi = (int)((int64_t)nt * (it.split + 1) / s.splits);
+  piece_of(s, it.split, (end + kN - 1) / kN, it.lo, it.hi);
   return it;
 }
 
@@ -352,7 +374,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         mbar_arrive_expect_tx(&sm.q_full[qb], kRows * kDP * 2);
         load_tile<kRows, kDP>(sm.q[qb], &tm_q, &sm.q_full[qb], it.qt * kRows, it.h, it.b);
         ++n;
-        const int kh = it.h / sh.G;
+        const int kh = sh.by_group.div(it.h);
         for (int j = it.lo; j < it.hi; ++j, ++t) {
           const uint32_t st = t % kStages, par = ((t / kStages) & 1) ^ 1;
           if (!(ok = wait(&sm.k_empty[st], par))) break;
@@ -702,15 +724,17 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // A2 = dO), the stream is K, V, acc1 = dS K. kKeys true: rows are 128 keys
 // (A1 = K, A2 = V), the stream is Q, dO of every query head that reads this
 // memory head, acc1 = dS^T Q, acc2 = P^T dO.
-// Warps: 0 TMA, 1 MMA, 2..5 and 6..9 two compute groups that take the streamed
-// tiles of 64 in turn. TMEM: [S, dP] of kBufs tiles, 128 columns each, then acc1
-// and acc2; dS lies over S (kKeys: P over S, dS over dP). The products with a
-// tile's dS are issued kBufs - 1 tiles behind its scores: with three buffers
-// (all but the keys' kernel at head size 128, whose accumulators leave room for
-// two) the tensor cores' round trip for a tile - about 1400 cycles from dS to
-// the buffer's next scores - passes while the groups are on two others.
+// Warps: 0 TMA, 1 the scores' MMA, 2..5 and 6..9 two compute groups that take
+// the streamed tiles of 64 in turn, 10 the products' MMA. TMEM: [S, dP] of kBufs
+// tiles, 128 columns each, then acc1 and acc2; dS lies over S (kKeys: P over S,
+// dS over dP). With three buffers (all but the keys' kernel at head size 128,
+// whose accumulators leave room for two) the tensor cores' round trip for a
+// tile passes while the groups are on two others, and two warps issue the MMAs,
+// because one thread's waits, issues and commits for a tile took about 1000
+// cycles. With two buffers a tile's scores follow the products before them in
+// the tensor pipe's order, from one thread (two threads: 592 instead of 528 us
+// on 16 x 2048 queries, 8192 keys, batch 2).
 constexpr int kBN = 64;
-constexpr int kBwdThreads = 320;
 
 // Shared memory: kABufs stationary pairs (two: the next item's loads early) and
 // kStages streamed pairs.
@@ -721,6 +745,8 @@ struct BwdGeo {
   static constexpr int kABytes = kRows * kDP * 2;
   static constexpr int kBBytes = kBN * kDP * 2;
   static constexpr uint32_t kAcc = 128 * kBufs;
+  static constexpr bool kSplitMma = kBufs == 3;
+  static constexpr int kThreads = kSplitMma ? 352 : 320;
   static_assert(kAcc + (kKeys ? 2 : 1) * kDP <= 512, "TMEM columns");
 };
 template <int kDP, bool kKeys, int kABufs>
@@ -730,7 +756,7 @@ struct BwdSmem {
   uint8_t b1[G::kStages][G::kBBytes], b2[G::kStages][G::kBBytes];
   float2 stat[kKeys ? G::kStages : 1][kBN];  // kKeys: the streamed queries' statistics
   uint64_t a_full[kABufs], a_empty[kABufs], b_full[G::kStages], b_empty[G::kStages];
-  uint64_t s_full[G::kBufs], ds_full[G::kBufs], acc_full, acc_free, drain;
+  uint64_t s_full[G::kBufs], ds_full[G::kBufs], buf_free[G::kBufs], acc_full, acc_free, drain[2];
   uint32_t tmem_base, abort;
 };
 
@@ -741,17 +767,12 @@ struct BwdItem {
 template <bool kKeys>
 __device__ __forceinline__ BwdItem bwd_item(const Shape& s, int item, int n_rt) {
   BwdItem it;
-  it.split = item % s.splits;
-  item /= s.splits;
-  const int heads = kKeys ? s.Hk : s.H;
-  const int n_bh = heads * s.B;
-  int rt = item / n_bh;
+  const ItemAt at = item_at(s, item);
+  it.split = at.split;
   // heaviest first under a causal mask: the last queries, the first keys
-  if (!kKeys) rt = n_rt - 1 - rt;
-  const int bh = item % n_bh;
-  it.head = bh % heads;
-  it.b = bh / heads;
-  it.row0 = rt * kRows;
+  it.row0 = (kKeys ? at.rt : n_rt - 1 - at.rt) * kRows;
+  it.head = at.head;
+  it.b = at.b;
   const int end = visible_end(s, it.b);
   int nt;
   it.first = 0;
@@ -764,8 +785,7 @@ __device__ __forceinline__ BwdItem bwd_item(const Shape& s, int item, int n_rt) 
   } else {
     nt = ((s.causal ? min(end, it.row0 + kRows) : end) + kBN - 1) / kBN;
   }
-  it.lo = (int)((int64_t)nt * it.split / s.splits);
-  it.hi = (int)((int64_t)nt * (it.split + 1) / s.splits);
+  piece_of(s, it.split, nt, it.lo, it.hi);
   return it;
 }
 
@@ -777,7 +797,7 @@ struct BwdOut {
 };
 
 template <typename T, int kDP, bool kKeys, int kABufs>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
     cross_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1,
                      const __grid_constant__ CUtensorMap tm_a2,
                      const __grid_constant__ CUtensorMap tm_b1,
@@ -800,6 +820,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     for (uint32_t i = 0; i < kBufs; ++i) {
       mbar_init(&sm.s_full[i], 1);
       mbar_init(&sm.ds_full[i], 4);
+      mbar_init(&sm.buf_free[i], 1);
     }
     for (uint32_t i = 0; i < kStages; ++i) {
       mbar_init(&sm.b_full[i], 1);
@@ -807,7 +828,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     mbar_init(&sm.acc_full, 1);
     mbar_init(&sm.acc_free, 8);
-    mbar_init(&sm.drain, 1);
+    mbar_init(&sm.drain[0], 1);
+    mbar_init(&sm.drain[1], 1);
     sm.abort = 0;
     fence_mbar_init();
   }
@@ -841,11 +863,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         load_tile<kRows, kDP>(sm.a1[ab], &tm_a1, &sm.a_full[ab], it.row0, it.head, it.b);
         load_tile<kRows, kDP>(sm.a2[ab], &tm_a2, &sm.a_full[ab], it.row0, it.head, it.b);
         ++n;
+        // keys: tile j is query tile `first + j % n` of head j / n of the group
+        int row = kKeys ? (it.first + it.lo % it.n) * kBN : it.lo * kBN;
+        int head = kKeys ? it.head * sh.G + it.lo / it.n : (int)sh.by_group.div(it.head);
         for (int j = it.lo; j < it.hi; ++j, ++u) {
           const uint32_t st = u % kStages;
           if (!(ok = wait(&sm.b_empty[st], ((u / kStages) & 1) ^ 1))) break;
-          const int row = kKeys ? (it.first + j % it.n) * kBN : j * kBN;
-          const int head = kKeys ? it.head * sh.G + j / it.n : it.head / sh.G;
           mbar_arrive_expect_tx(&sm.b_full[st],
                                 2 * Geo::kBBytes + (kKeys ? (uint32_t)sizeof(sm.stat[st]) : 0u));
           if (kKeys)
@@ -853,6 +876,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                       sizeof(sm.stat[st]), &sm.b_full[st]);
           load_tile<kBN, kDP>(sm.b1[st], &tm_b1, &sm.b_full[st], row, head, it.b);
           load_tile<kBN, kDP>(sm.b2[st], &tm_b2, &sm.b_full[st], row, head, it.b);
+          row += kBN;
+          if (kKeys && row >= (it.first + it.n) * kBN) {
+            row = it.first * kBN;
+            ++head;
+          }
         }
       }
       if (!ok) {
@@ -862,8 +890,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
+  } else if (warp == 1 && !Geo::kSplitMma) {
+    // ------------------------------------------------------------ both MMAs
     if (elect_one_sync()) {
       constexpr uint32_t id_s = idesc(Type<T>::kIdesc, kRows, kBN, 0);
       constexpr uint32_t id_acc = idesc(Type<T>::kIdesc, kRows, kDP, 1);
@@ -904,9 +932,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
         const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
         if (it.lo >= it.hi) continue;
-        if (kABufs == 1)  // the wait below is long: what is there to do first
-          while (ok && pending) ok = issue_acc();
-        if (!ok || !(ok = wait(&sm.a_full[is.at], is.phase))) break;
+        if (!(ok = wait(&sm.a_full[is.at], is.phase))) break;
         const uint32_t a1 = a10 + is.at * Geo::kABytes, a2 = a20 + is.at * Geo::kABytes;
         for (int j = it.lo; j < it.hi; ++j) {
           if (!(ok = wait(&sm.b_full[ss.at], ss.phase))) break;
@@ -928,8 +954,86 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       while (ok && pending) ok = issue_acc();
       if (!ok && issued) {
-        umma_commit(&sm.drain);
-        settle(&sm.drain, 1);
+        umma_commit(&sm.drain[0]);
+        settle(&sm.drain[0], 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ scores' MMA
+    if (elect_one_sync()) {
+      constexpr uint32_t id_s = idesc(Type<T>::kIdesc, kRows, kBN, 0);
+      const uint32_t a10 = smem_u32(sm.a1[0]), a20 = smem_u32(sm.a2[0]);
+      const uint32_t b10 = smem_u32(sm.b1[0]), b20 = smem_u32(sm.b2[0]);
+      Ring<kStages> ss;
+      Ring<kBufs> sb;
+      Ring<kABufs> is;
+      bool ok = true, issued = false;
+      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+        const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
+        if (it.lo >= it.hi) continue;
+        if (!(ok = wait(&sm.a_full[is.at], is.phase))) break;
+        const uint32_t a1 = a10 + is.at * Geo::kABytes, a2 = a20 + is.at * Geo::kABytes;
+        for (int j = it.lo; j < it.hi; ++j) {
+          if (!(ok = wait(&sm.b_full[ss.at], ss.phase))) break;
+          // the products with this buffer's last dS are complete
+          if (!(ok = wait(&sm.buf_free[sb.at], sb.phase ^ 1))) break;
+          tc_fence_after();
+          const uint32_t t_s = tmem + sb.at * 128u;
+          mma_rows<kRows, kBN, kDP>(t_s, a1, b10 + ss.at * Geo::kBBytes, id_s);
+          mma_rows<kRows, kBN, kDP>(t_s + 64, a2, b20 + ss.at * Geo::kBBytes, id_s);
+          issued = true;
+          umma_commit(&sm.s_full[sb.at]);
+          if (j == it.hi - 1) umma_commit(&sm.a_empty[is.at]);
+          ss.next();
+          sb.next();
+        }
+        is.next();
+      }
+      if (!ok && issued) {
+        umma_commit(&sm.drain[0]);
+        settle(&sm.drain[0], 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 10) {
+    // ------------------------------------------------------------ products' MMA
+    if (elect_one_sync()) {
+      constexpr uint32_t id_acc = idesc(Type<T>::kIdesc, kRows, kDP, 1);
+      const uint32_t b10 = smem_u32(sm.b1[0]), b20 = smem_u32(sm.b2[0]);
+      Ring<kStages> ss;
+      Ring<kBufs> sb;
+      uint32_t n = 0;
+      bool ok = true, issued = false;
+      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+        const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
+        if (it.lo >= it.hi) continue;
+        // the item before has been read out
+        if (!(ok = wait(&sm.acc_free, (n & 1) ^ 1))) break;
+        ++n;
+        for (int j = it.lo; j < it.hi; ++j) {
+          if (!(ok = wait(&sm.b_full[ss.at], ss.phase))) break;
+          if (!(ok = wait(&sm.ds_full[sb.at], sb.phase))) break;
+          tc_fence_after();
+          const uint32_t t_s = tmem + sb.at * 128u;
+          const uint32_t b1 = b10 + ss.at * Geo::kBBytes, b2 = b20 + ss.at * Geo::kBBytes;
+          if (kKeys) {
+            mma_cols<kBN, kDP>(t_acc2, t_s, b2, id_acc, j > it.lo);
+            mma_cols<kBN, kDP>(t_acc1, t_s + 64, b1, id_acc, j > it.lo);
+          } else {
+            mma_cols<kBN, kDP>(t_acc1, t_s, b1, id_acc, j > it.lo);
+          }
+          issued = true;
+          umma_commit(&sm.buf_free[sb.at]);
+          umma_commit(&sm.b_empty[ss.at]);
+          if (j == it.hi - 1) umma_commit(&sm.acc_full);
+          ss.next();
+          sb.next();
+        }
+      }
+      if (!ok && issued) {
+        umma_commit(&sm.drain[1]);
+        settle(&sm.drain[1], 1);
       }
     }
     __syncwarp();
@@ -941,7 +1045,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint64_t sl2x2 = f2_splat(sh.scale * kLog2e);
     constexpr float kShift = kKeys ? Type<T>::kShift : 0.f;
     const float unshift = exp2f(-kShift);
-    uint32_t u = 0, n = 0;
+    Ring<kStages> ss;
+    Ring<kBufs> sb;
+    uint32_t turn = 0, n = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
       const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
@@ -963,72 +1069,87 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           row_ok = (__ldg(sh.words + (int64_t)it.b * sh.nwords + row / 32) >> (row & 31)) & 1u;
       }
       const bool rows_ok = __all_sync(0xffffffffu, row_ok);
-      // tiles of this group: u counts the CTA's tiles
-      const uint32_t u0 = u;
-      for (int j = it.lo + (int)((u0 ^ (uint32_t)group) & 1u); j < it.hi; j += 2) {
-        const uint32_t w = u0 + (uint32_t)(j - it.lo), stage = w % kStages, buf = w % kBufs;
+      // the CTA's tiles alternate between the groups: mine is every second one
+      int col0 = kKeys && any ? (it.first + it.lo % it.n) * kBN : it.lo * kBN;
+      for (int j = it.lo; j < it.hi; ++j) {
+        const bool mine = turn == (uint32_t)group;
+        const uint32_t stage = ss.at, sphase = ss.phase, buf = sb.at, bphase = sb.phase;
+        const int col = col0;
+        turn ^= 1;
+        ss.next();
+        sb.next();
+        col0 += kBN;
+        if (kKeys && col0 >= (it.first + it.n) * kBN) col0 = it.first * kBN;
+        if (!mine) continue;
         const uint32_t t_s = tmem + lanes + buf * 128u;
-        const int col0 = kKeys ? (it.first + j % it.n) * kBN : j * kBN;
-        uint2 words = make_uint2(0xffffffffu, 0xffffffffu);
-        if (!kKeys) words = tile_words(sh, it.b, col0);
-        const bool diag = sh.causal && (kKeys ? col0 < it.row0 + kRows - 1
-                                              : col0 + kBN - 1 > it.row0);
         // the statistics came with the tile (already complete: S was computed)
-        ok = !kKeys || wait(&sm.b_full[stage], (w / kStages) & 1);
-        ok = ok && wait(&sm.s_full[buf], (w / kBufs) & 1);
+        ok = !kKeys || wait(&sm.b_full[stage], sphase);
+        ok = ok && wait(&sm.s_full[buf], bphase);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
-        // 32 columns: P and dS as 16-bit pairs. Hidden pairs are replaced by
-        // zero, whatever the products gave.
-        auto columns = [&](int c, auto masked) {
-          uint32_t rs[32], rd[32];
-          tmem_ld_32cols(t_s + c * 32, rs);
-          tmem_ld_32cols(t_s + 64 + c * 32, rd);
-          tmem_ld_wait();
-          uint32_t pk[16], dk[16];
-          const int lim = row - (col0 + c * 32);  // causal: key <= query
+        uint2 words = make_uint2(0xffffffffu, 0xffffffffu);
+        if (!kKeys && (sh.words || col + kBN > sh.Sk)) words = tile_words(sh, it.b, col);
+        const bool diag = sh.causal && (kKeys ? col < it.row0 + kRows - 1
+                                              : col + kBN - 1 > it.row0);
+        // P and dS as 16-bit pairs, 16 columns at a time with the next 16 on
+        // their way from TMEM. Hidden pairs are replaced by zero, whatever the
+        // products gave.
+        auto columns = [&](auto masked) {
+          uint32_t rs[2][16], rd[2][16];
+          tmem_ld_16cols(t_s, rs[0]);
+          tmem_ld_16cols(t_s + 64, rd[0]);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            uint64_t nl = row_lse, nd = row_delta;
-            if (kKeys) {
-              const float4 v = *reinterpret_cast<const float4*>(&sm.stat[stage][c * 32 + i]);
-              nl = f2_pack(v.x, v.z);
-              nd = f2_pack(v.y, v.w);
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_wait();
+            if (c < 3) {
+              tmem_ld_16cols(t_s + (c + 1) * 16, rs[(c + 1) & 1]);
+              tmem_ld_16cols(t_s + 64 + (c + 1) * 16, rd[(c + 1) & 1]);
             }
-            uint64_t e = f2_fma(f2_pack(__uint_as_float(rs[i]), __uint_as_float(rs[i + 1])), sl2x2, nl);
-            if (kShift != 0.f) e = f2_add(e, f2_splat(kShift));
-            float p0, p1, d0, d1;
-            f2_unpack(e, p0, p1);
-            p0 = ex2(p0);
-            p1 = ex2(p1);
-            uint64_t d = f2_add(f2_pack(__uint_as_float(rd[i]), __uint_as_float(rd[i + 1])), nd);
-            if (kShift != 0.f) d = f2_mul(d, f2_splat(unshift));
-            f2_unpack(f2_mul(f2_pack(p0, p1), d), d0, d1);
-            if (decltype(masked)::value) {
-              const uint32_t wc = c == 0 ? words.x : words.y;
-              bool v0 = row_ok && ((wc >> i) & 1u), v1 = row_ok && ((wc >> (i + 1)) & 1u);
-              if (diag) {
-                v0 = v0 && (kKeys ? i >= lim : i <= lim);
-                v1 = v1 && (kKeys ? i + 1 >= lim : i + 1 <= lim);
+            const uint32_t (&s16)[16] = rs[c & 1];
+            const uint32_t (&d16)[16] = rd[c & 1];
+            uint32_t pk[8], dk[8];
+            const uint32_t wc = (c < 2 ? words.x : words.y) >> (c % 2 * 16);
+            const int lim = row - (col + c * 16);  // causal: key <= query
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              uint64_t nl = row_lse, nd = row_delta;
+              if (kKeys) {
+                const float4 v = *reinterpret_cast<const float4*>(&sm.stat[stage][c * 16 + i]);
+                nl = f2_pack(v.x, v.z);
+                nd = f2_pack(v.y, v.w);
               }
-              p0 = v0 ? p0 : 0.f;
-              p1 = v1 ? p1 : 0.f;
-              d0 = v0 ? d0 : 0.f;
-              d1 = v1 ? d1 : 0.f;
+              uint64_t e =
+                  f2_fma(f2_pack(__uint_as_float(s16[i]), __uint_as_float(s16[i + 1])), sl2x2, nl);
+              if (kShift != 0.f) e = f2_add(e, f2_splat(kShift));
+              float p0, p1, d0, d1;
+              f2_unpack(e, p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+              uint64_t d = f2_add(f2_pack(__uint_as_float(d16[i]), __uint_as_float(d16[i + 1])), nd);
+              if (kShift != 0.f) d = f2_mul(d, f2_splat(unshift));
+              f2_unpack(f2_mul(f2_pack(p0, p1), d), d0, d1);
+              if (decltype(masked)::value) {
+                bool v0 = row_ok && ((wc >> i) & 1u), v1 = row_ok && ((wc >> (i + 1)) & 1u);
+                if (diag) {
+                  v0 = v0 && (kKeys ? i >= lim : i <= lim);
+                  v1 = v1 && (kKeys ? i + 1 >= lim : i + 1 <= lim);
+                }
+                p0 = v0 ? p0 : 0.f;
+                p1 = v1 ? p1 : 0.f;
+                d0 = v0 ? d0 : 0.f;
+                d1 = v1 ? d1 : 0.f;
+              }
+              if (kKeys) pk[i / 2] = Type<T>::pack(p0, p1);
+              dk[i / 2] = Type<T>::pack(d0, d1);
             }
-            if (kKeys) pk[i / 2] = Type<T>::pack(p0, p1);
-            dk[i / 2] = Type<T>::pack(d0, d1);
+            if (kKeys) tmem_st_8cols(t_s + c * 8, pk);
+            tmem_st_8cols(t_s + (kKeys ? 64u : 0u) + c * 8, dk);
           }
-          if (kKeys) tmem_st_16cols(t_s + c * 16, pk);
-          tmem_st_16cols(t_s + (kKeys ? 64u : 0u) + c * 16, dk);
         };
-        if (diag || !rows_ok || !is_whole(words)) {
-          columns(0, std::true_type{});
-          columns(1, std::true_type{});
-        } else {
-          columns(0, std::false_type{});
-          columns(1, std::false_type{});
-        }
+        if (diag || !rows_ok || !is_whole(words))
+          columns(std::true_type{});
+        else
+          columns(std::false_type{});
         if (!kKeys && sh.words && !is_whole(words))
           zero_hidden_rows<kBN, kDP>(sm.b1[stage], words, (warp & 3) * 32 + lane, 128);
         tmem_st_wait();
@@ -1037,7 +1158,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (lane == 0) mbar_arrive(&sm.ds_full[buf]);
       }
       if (!ok) break;
-      u = u0 + (uint32_t)max(0, it.hi - it.lo);
       // ---- read the accumulators out
       if (any) {
         ok = wait(&sm.acc_full, n & 1);
@@ -1207,7 +1327,8 @@ cudaError_t cross_attn_opt_in(const void* kernel, size_t smem, std::atomic<uint6
 
 namespace {
 
-Shape shape_of(const CrossAttnArgs& a, int splits) {
+// `heads` of the rows that an item's index runs over.
+Shape shape_of(const CrossAttnArgs& a, int splits, int heads) {
   Shape s{};
   s.B = a.B; s.Sq = a.Sq; s.Sk = a.Sk; s.H = a.H; s.Hk = a.Hk; s.G = a.H / a.Hk; s.D = a.D;
   s.causal = a.causal;
@@ -1217,12 +1338,17 @@ Shape shape_of(const CrossAttnArgs& a, int splits) {
   s.vis_end = a.key_pad ? a.vis_end : nullptr;
   s.nwords = (a.Sk + 31) / 32;
   s.err = default_err_word();
+  s.by_splits = FastDiv((uint32_t)splits);
+  s.by_bh = FastDiv((uint32_t)(heads * a.B));
+  s.by_heads = FastDiv((uint32_t)heads);
+  s.by_group = FastDiv((uint32_t)s.G);
   return s;
 }
 
 bool bad_shape(const CrossAttnArgs& a) {
   return a.B <= 0 || a.Sq <= 0 || a.Sk <= 0 || a.H <= 0 || a.Hk <= 0 || a.H % a.Hk || a.D <= 0 ||
          a.D > 128 || a.D % 8 || (a.causal && a.Sq != a.Sk) || !(a.scale > 0.f) ||
+         (int64_t)a.H * a.B > 0x3fffffff ||
          (a.key_pad && !cross_attn_is_few(a) && (!a.words || !a.vis_end));
 }
 
@@ -1264,7 +1390,7 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   const int64_t items = (int64_t)n_qt * a.H * a.B * splits;
   if (items > 0x7fffffff - 4096) return cudaErrorInvalidValue;
   const int grid = (int)std::min<int64_t>(items, 2ll * num_sms());
-  e = launch_pdl(kernel, dim3(grid), dim3(kFwdThreads), smem, st, mq, mk, mv, shape_of(a, splits),
+  e = launch_pdl(kernel, dim3(grid), dim3(kFwdThreads), smem, st, mq, mk, mv, shape_of(a, splits, a.H),
                  (T*)a.out, a.lse2, a.partials, a.partials + splits * rows * a.D, (int)items, n_qt);
   if (e != cudaSuccess) return e;
   note_launch();
@@ -1300,8 +1426,8 @@ cudaError_t run_bwd_half(const CrossAttnArgs& a, cudaStream_t st) {
   o.s2 = kKeys ? s3(a.dv_st) : o.s1;
   o.part = a.partials;
   const int grid = (int)std::min<int64_t>(items, num_sms());
-  e = launch_pdl(kernel, dim3(grid), dim3(kBwdThreads), smem, st, kKeys ? mk : mq, kKeys ? mv : mo,
-                 kKeys ? mq : mk, kKeys ? mo : mv, shape_of(a, splits), (const float2*)a.stats, o, (int)items, n_rt);
+  e = launch_pdl(kernel, dim3(grid), dim3(BwdGeo<kDP, kKeys, kABufs>::kThreads), smem, st, kKeys ? mk : mq, kKeys ? mv : mo,
+                 kKeys ? mq : mk, kKeys ? mo : mv, shape_of(a, splits, heads), (const float2*)a.stats, o, (int)items, n_rt);
   if (e != cudaSuccess) return e;
   note_launch();
   if (splits > 1) {
