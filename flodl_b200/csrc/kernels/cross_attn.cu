@@ -178,6 +178,62 @@ __device__ __forceinline__ void zero_hidden_rows(uint8_t* tile, uint2 words, int
   fence_proxy_async_shared();
 }
 
+// Sixteen columns of a row that lies in TMEM from t on, times f (`use` false:
+// zeros; `there`, the same for the warp, says whether TMEM holds them).
+__device__ __forceinline__ void row16(uint32_t t, bool there, bool use, float f, float (&v)[16]) {
+  uint32_t o[16];
+  if (there) {
+    tmem_ld_16cols(t, o);
+    tmem_ld_wait();
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = there && use ? __uint_as_float(o[i]) * f : 0.f;
+}
+// An item's output tile leaves through the shared memory of its stationary
+// operand, which no product reads any more, by TMA. (Stored from registers, a
+// row per lane, an instruction touches 32 lines with 16 bytes each: the 128 rows
+// of dK and dV then took 3000 cycles.) `block`: the warp's 32 rows x 64 columns
+// in 128-byte swizzle.
+template <typename T>
+__device__ __forceinline__ void stage_rows(uint32_t t, int lane, bool use, float f, uint8_t* block) {
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    float v[16];
+    row16(t + c * 16, true, use, f, v);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *reinterpret_cast<uint4*>(block + lane * 128 + (((2 * c + h) ^ (lane & 7)) << 4)) = make_uint4(
+          Type<T>::pack(v[8 * h], v[8 * h + 1]), Type<T>::pack(v[8 * h + 2], v[8 * h + 3]),
+          Type<T>::pack(v[8 * h + 4], v[8 * h + 5]), Type<T>::pack(v[8 * h + 6], v[8 * h + 7]));
+  }
+}
+// The plain form: a row's columns below D as 16-bit values to out, or as f32 to
+// part (pieces of a split axis; rows without a visible tile).
+template <typename T>
+__device__ __forceinline__ void store_row(uint32_t t, int D, bool there, bool use, bool row, float f,
+                                          T* out, float* part) {
+#pragma unroll 1
+  for (int c = 0; c < D; c += 16) {
+    float v[16];
+    row16(t + c, there, use, f, v);
+    if (!row) continue;
+    if (part == nullptr) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (c + 8 * h < D)
+          *reinterpret_cast<uint4*>(out + c + 8 * h) = make_uint4(
+              Type<T>::pack(v[8 * h], v[8 * h + 1]), Type<T>::pack(v[8 * h + 2], v[8 * h + 3]),
+              Type<T>::pack(v[8 * h + 4], v[8 * h + 5]), Type<T>::pack(v[8 * h + 6], v[8 * h + 7]));
+    } else {
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        if (c + 4 * h < D)
+          *reinterpret_cast<float4*>(part + c + 4 * h) =
+              make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+    }
+  }
+}
+
 struct Shape {
   int B, Sq, Sk, H, Hk, G, D, causal;
   int splits;
@@ -315,7 +371,8 @@ template <typename T, int kDP>
 __global__ void __launch_bounds__(kFwdThreads, 2)
     cross_fwd_kernel(const __grid_constant__ CUtensorMap tm_q,
                      const __grid_constant__ CUtensorMap tm_k,
-                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Shape sh,
+                     const __grid_constant__ CUtensorMap tm_v,
+                     const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ Shape sh,
                      T* __restrict__ out, float* __restrict__ lse2, float* __restrict__ part_o,
                      float* __restrict__ part_lse, int n_items, int n_qt) {
   using Geo = FwdGeo<kDP>;
@@ -329,7 +386,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < kQBufs; ++i) {
       mbar_init(&sm.q_full[i], 1);
-      mbar_init(&sm.q_empty[i], 1);
+      mbar_init(&sm.q_empty[i], 4);
     }
     for (uint32_t i = 0; i < kStages; ++i) {
       mbar_init(&sm.k_full[i], 1);
@@ -438,7 +495,6 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
           umma_commit(&sm.s_full[t & 1]);
           umma_commit(&sm.k_empty[ks.at]);
           ks.next();
-          if (j == it.hi - 1) umma_commit(&sm.q_empty[qs.at]);
           if (behind && !(ok = issue_pv(behind_acc))) break;
           ++t;
           behind = true;
@@ -461,7 +517,18 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     const float sl2 = sh.scale * kLog2e;
     const uint64_t sl2x2 = f2_splat(sl2);
     uint32_t t = 0;
+    Ring<kQBufs> qs;
     bool ok = true;
+    // The Q buffer whose output store may still be read: given back once the
+    // next item is under way, or at once where there is no other buffer.
+    uint64_t* owed = nullptr;
+    auto give_back = [&]() {
+      if (owed != nullptr && lane == 0) {
+        bulk_wait_group_read<0>();
+        mbar_arrive(owed);
+      }
+      owed = nullptr;
+    };
     for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
       const FwdItem it = fwd_item(sh, item, n_qt);
       const int qi = it.qt * kRows + r;
@@ -557,6 +624,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.p_full[t & 1]);
+        give_back();
       }
       if (!ok) break;
       // ---- output: O / l and lse
@@ -573,35 +641,26 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       const int64_t rows_all = (int64_t)sh.B * sh.Sq * sh.H;
       const int64_t orow = ((int64_t)it.b * sh.Sq + qi) * sh.H + it.h;
       const int64_t lrow = ((int64_t)it.b * sh.H + it.h) * sh.Sq + qi;
-#pragma unroll
-      for (int c = 0; c < kDP / 32; ++c) {
-        uint32_t o[32];
-        if (any) {
-          tmem_ld_32cols(t_o + c * 32, o);
-          tmem_ld_wait();
+      if (any && sh.splits == 1) {
+        uint8_t* block = sm.q[qs.at] + (warp & 3) * 4096;
+#pragma unroll 1
+        for (int c = 0; c < kDP / 64; ++c)
+          stage_rows<T>(t_o + c * 64, lane, !none, inv_l, block + c * kRows * 128);
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          for (int c = 0; c * 64 < sh.D; ++c)
+            tma_store_4d(&tm_o, block + c * kRows * 128, c * 64, qi - lane, it.h, it.b);
+          bulk_commit_group();
         }
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          o[i] = any && !none ? __float_as_uint(__uint_as_float(o[i]) * inv_l) : 0u;
-        if (qi < sh.Sq) {
-          if (sh.splits == 1) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (c * 32 + q * 8 < sh.D)
-                *reinterpret_cast<uint4*>(out + orow * sh.D + c * 32 + q * 8) = make_uint4(
-                    Type<T>::pack(__uint_as_float(o[8 * q]), __uint_as_float(o[8 * q + 1])),
-                    Type<T>::pack(__uint_as_float(o[8 * q + 2]), __uint_as_float(o[8 * q + 3])),
-                    Type<T>::pack(__uint_as_float(o[8 * q + 4]), __uint_as_float(o[8 * q + 5])),
-                    Type<T>::pack(__uint_as_float(o[8 * q + 6]), __uint_as_float(o[8 * q + 7])));
-          } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              if (c * 32 + q * 4 < sh.D)
-                *reinterpret_cast<uint4*>(part_o + (it.split * rows_all + orow) * sh.D + c * 32 +
-                                          q * 4) =
-                    make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
-          }
-        }
+      } else {
+        store_row<T>(t_o, sh.D, any, !none, qi < sh.Sq, inv_l, out + orow * sh.D,
+                     sh.splits > 1 ? part_o + (it.split * rows_all + orow) * sh.D : nullptr);
+      }
+      if (any) {
+        owed = &sm.q_empty[qs.at];
+        if (kQBufs == 1) give_back();
+        qs.next();
       }
       if (qi < sh.Sq) {
         if (sh.splits > 1)
@@ -611,6 +670,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       }
       tc_fence_before();
     }
+    if (lane == 0) bulk_wait_group<0>();
   }
   tc_fence_before();
   __syncthreads();
@@ -801,7 +861,9 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
     cross_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1,
                      const __grid_constant__ CUtensorMap tm_a2,
                      const __grid_constant__ CUtensorMap tm_b1,
-                     const __grid_constant__ CUtensorMap tm_b2, const __grid_constant__ Shape sh,
+                     const __grid_constant__ CUtensorMap tm_b2,
+                     const __grid_constant__ CUtensorMap tm_o1,
+                     const __grid_constant__ CUtensorMap tm_o2, const __grid_constant__ Shape sh,
                      const float2* __restrict__ stats, const __grid_constant__ BwdOut<T> outs, int n_items, int n_rt) {
   using Geo = BwdGeo<kDP, kKeys, kABufs>;
   using Smem = BwdSmem<kDP, kKeys, kABufs>;
@@ -815,7 +877,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kABufs; ++i) {
       mbar_init(&sm.a_full[i], 1);
-      mbar_init(&sm.a_empty[i], 1);
+      mbar_init(&sm.a_empty[i], 8);
     }
     for (uint32_t i = 0; i < kBufs; ++i) {
       mbar_init(&sm.s_full[i], 1);
@@ -864,8 +926,9 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
         load_tile<kRows, kDP>(sm.a2[ab], &tm_a2, &sm.a_full[ab], it.row0, it.head, it.b);
         ++n;
         // keys: tile j is query tile `first + j % n` of head j / n of the group
-        int row = kKeys ? (it.first + it.lo % it.n) * kBN : it.lo * kBN;
-        int head = kKeys ? it.head * sh.G + it.lo / it.n : (int)sh.by_group.div(it.head);
+        int row = (kKeys ? it.first + (it.lo > 0 ? it.lo % it.n : 0) : it.lo) * kBN;
+        int head = kKeys ? it.head * sh.G + (it.lo > 0 ? it.lo / it.n : 0)
+                         : (int)sh.by_group.div(it.head);
         for (int j = it.lo; j < it.hi; ++j, ++u) {
           const uint32_t st = u % kStages;
           if (!(ok = wait(&sm.b_empty[st], ((u / kStages) & 1) ^ 1))) break;
@@ -943,7 +1006,6 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
           mma_rows<kRows, kBN, kDP>(t_s + 64, a2, b20 + ss.at * Geo::kBBytes, id_s);
           issued = true;
           umma_commit(&sm.s_full[sb.at]);
-          if (j == it.hi - 1) umma_commit(&sm.a_empty[is.at]);
           ss.next();
           sb.next();
           firsts |= (j == it.lo ? 1u : 0u) << pending;
@@ -984,7 +1046,6 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
           mma_rows<kRows, kBN, kDP>(t_s + 64, a2, b20 + ss.at * Geo::kBBytes, id_s);
           issued = true;
           umma_commit(&sm.s_full[sb.at]);
-          if (j == it.hi - 1) umma_commit(&sm.a_empty[is.at]);
           ss.next();
           sb.next();
         }
@@ -1047,8 +1108,18 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
     const float unshift = exp2f(-kShift);
     Ring<kStages> ss;
     Ring<kBufs> sb;
+    Ring<kABufs> is;
     uint32_t turn = 0, n = 0;
     bool ok = true;
+    // The stationary buffer whose output store may still be read (see forward)
+    uint64_t* owed = nullptr;
+    auto give_back = [&]() {
+      if (owed != nullptr && lane == 0) {
+        bulk_wait_group_read<0>();
+        mbar_arrive(owed);
+      }
+      owed = nullptr;
+    };
     for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
       const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
       const int row = it.row0 + r;
@@ -1070,7 +1141,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       }
       const bool rows_ok = __all_sync(0xffffffffu, row_ok);
       // the CTA's tiles alternate between the groups: mine is every second one
-      int col0 = kKeys && any ? (it.first + it.lo % it.n) * kBN : it.lo * kBN;
+      int col0 = (kKeys ? it.first + (it.lo > 0 ? it.lo % it.n : 0) : it.lo) * kBN;
       for (int j = it.lo; j < it.hi; ++j) {
         const bool mine = turn == (uint32_t)group;
         const uint32_t stage = ss.at, sphase = ss.phase, buf = sb.at, bphase = sb.phase;
@@ -1156,6 +1227,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.ds_full[buf]);
+        give_back();
       }
       if (!ok) break;
       // ---- read the accumulators out
@@ -1165,49 +1237,40 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
         tc_fence_after();
         ++n;
       }
-      const int rows_n = kKeys ? sh.Sk : sh.Sq, heads = kKeys ? sh.Hk : sh.H;
-      const int64_t flat = ((int64_t)it.b * rows_n + row) * heads + it.head;
-      const int64_t rows_all = (int64_t)sh.B * rows_n * heads;
-      // queries: each group takes half of dQ's columns; keys: group 0 takes dV,
-      // group 1 dK
-      constexpr int kCols = kKeys ? kDP : kDP / 2;
+      give_back();
+      // keys: group 0 takes dV, group 1 dK; queries: 64 of dQ's columns each (one
+      // group at head size 64)
       const bool second = kKeys && group == 0;
-      const uint32_t t_a = (second ? t_acc2 : t_acc1) + lanes + (kKeys ? 0 : group * kCols);
+      const uint32_t t_a = (second ? t_acc2 : t_acc1) + lanes;
       const float f = second ? unshift : sh.scale;
-      T* dst = second ? outs.o2 : outs.o1;
-      const Stride3& st3 = second ? outs.s2 : outs.s1;
-      dst += it.b * st3.b + (int64_t)row * st3.s + it.head * st3.h;
-      float* part = outs.part + ((int64_t)it.split * (kKeys ? 2 : 1) + (second ? 1 : 0)) * rows_all * sh.D +
-                    flat * sh.D;
-#pragma unroll
-      for (int c = 0; c < kCols / 32; ++c) {
-        uint32_t o[32];
-        if (any) {
-          tmem_ld_32cols(t_a + c * 32, o);
-          tmem_ld_wait();
+      if (any && sh.splits == 1) {
+        uint8_t* block = (second ? sm.a2[is.at] : sm.a1[is.at]) + (warp & 3) * 4096;
+#pragma unroll 1
+        for (int c = kKeys ? 0 : group; c < kDP / 64; c += kKeys ? 1 : 2)
+          stage_rows<T>(t_a + c * 64, lane, true, f, block + c * kRows * 128);
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          for (int c = kKeys ? 0 : group; c * 64 < sh.D; c += kKeys ? 1 : 2)
+            tma_store_4d(second ? &tm_o2 : &tm_o1, block + c * kRows * 128, c * 64, row - lane, it.head,
+                         it.b);
+          bulk_commit_group();
         }
-        const int col0 = (kKeys ? 0 : group * kCols) + c * 32;
-        float v[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = any ? __uint_as_float(o[i]) * f : 0.f;
-        if (row < rows_n) {
-          if (sh.splits == 1) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (col0 + q * 8 < sh.D)
-                *reinterpret_cast<uint4*>(dst + col0 + q * 8) =
-                    make_uint4(Type<T>::pack(v[8 * q], v[8 * q + 1]),
-                               Type<T>::pack(v[8 * q + 2], v[8 * q + 3]),
-                               Type<T>::pack(v[8 * q + 4], v[8 * q + 5]),
-                               Type<T>::pack(v[8 * q + 6], v[8 * q + 7]));
-          } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              if (col0 + q * 4 < sh.D)
-                *reinterpret_cast<float4*>(part + col0 + q * 4) =
-                    make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-          }
-        }
+      } else if (kKeys || group == 0) {
+        const int rows_n = kKeys ? sh.Sk : sh.Sq, heads = kKeys ? sh.Hk : sh.H;
+        const int64_t flat = ((int64_t)it.b * rows_n + row) * heads + it.head;
+        const int64_t rows_all = (int64_t)sh.B * rows_n * heads;
+        const Stride3 st3 = second ? outs.s2 : outs.s1;
+        T* dst = (second ? outs.o2 : outs.o1) + it.b * st3.b + (int64_t)row * st3.s + it.head * st3.h;
+        float* part = sh.splits == 1 ? nullptr
+                                     : outs.part + ((int64_t)it.split * (kKeys ? 2 : 1) + (second ? 1 : 0)) *
+                                                       rows_all * sh.D + flat * sh.D;
+        store_row<T>(t_a, sh.D, any, true, row < rows_n, f, dst, part);
+      }
+      if (any) {
+        owed = &sm.a_empty[is.at];
+        if (kABufs == 1) give_back();
+        is.next();
       }
       if (any) {
         tc_fence_before();
@@ -1215,6 +1278,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
         if (lane == 0) mbar_arrive(&sm.acc_free);
       }
     }
+    if (lane == 0) bulk_wait_group<0>();
   }
   tc_fence_before();
   __syncthreads();
@@ -1376,8 +1440,10 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   const int splits = fwd_splits(a);
   const int64_t rows = (int64_t)a.B * a.Sq * a.H;
   if (splits > 1 && !a.partials) return cudaErrorInvalidValue;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
+  const int64_t o_st[3] = {(int64_t)a.Sq * a.H * a.D, (int64_t)a.H * a.D, a.D};
   if (!cross_attn_map(&mq, a.q, a.half, a.D, a.Sq, a.H, a.B, a.q_st, kRows) ||
+      !cross_attn_map(&mo, a.out, a.half, a.D, a.Sq, a.H, a.B, o_st, 32) ||
       !cross_attn_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kN) ||
       !cross_attn_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kN))
     return cudaErrorInvalidValue;
@@ -1390,7 +1456,7 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   const int64_t items = (int64_t)n_qt * a.H * a.B * splits;
   if (items > 0x7fffffff - 4096) return cudaErrorInvalidValue;
   const int grid = (int)std::min<int64_t>(items, 2ll * num_sms());
-  e = launch_pdl(kernel, dim3(grid), dim3(kFwdThreads), smem, st, mq, mk, mv, shape_of(a, splits, a.H),
+  e = launch_pdl(kernel, dim3(grid), dim3(kFwdThreads), smem, st, mq, mk, mv, mo, shape_of(a, splits, a.H),
                  (T*)a.out, a.lse2, a.partials, a.partials + splits * rows * a.D, (int)items, n_qt);
   if (e != cudaSuccess) return e;
   note_launch();
@@ -1407,6 +1473,11 @@ cudaError_t run_bwd_half(const CrossAttnArgs& a, cudaStream_t st) {
       !cross_attn_map(&mo, a.dout, a.half, a.D, a.Sq, a.H, a.B, a.do_st, kKeys ? cb : rb) ||
       !cross_attn_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kKeys ? rb : cb) ||
       !cross_attn_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kKeys ? rb : cb))
+    return cudaErrorInvalidValue;
+  CUtensorMap m1, m2;
+  if (!(kKeys ? cross_attn_map(&m1, a.dk, a.half, a.D, a.Sk, a.Hk, a.B, a.dk_st, 32) &&
+                    cross_attn_map(&m2, a.dv, a.half, a.D, a.Sk, a.Hk, a.B, a.dv_st, 32)
+              : cross_attn_map(&m1, a.dq, a.half, a.D, a.Sq, a.H, a.B, a.dq_st, 32)))
     return cudaErrorInvalidValue;
   static std::atomic<uint64_t> done{0};
   constexpr int smem = (int)sizeof(BwdSmem<kDP, kKeys, kABufs>) + 1024;
@@ -1427,7 +1498,7 @@ cudaError_t run_bwd_half(const CrossAttnArgs& a, cudaStream_t st) {
   o.part = a.partials;
   const int grid = (int)std::min<int64_t>(items, num_sms());
   e = launch_pdl(kernel, dim3(grid), dim3(BwdGeo<kDP, kKeys, kABufs>::kThreads), smem, st, kKeys ? mk : mq, kKeys ? mv : mo,
-                 kKeys ? mq : mk, kKeys ? mo : mv, shape_of(a, splits, heads), (const float2*)a.stats, o, (int)items, n_rt);
+                 kKeys ? mq : mk, kKeys ? mo : mv, m1, kKeys ? m2 : m1, shape_of(a, splits, heads), (const float2*)a.stats, o, (int)items, n_rt);
   if (e != cudaSuccess) return e;
   note_launch();
   if (splits > 1) {
