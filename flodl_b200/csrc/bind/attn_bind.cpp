@@ -150,16 +150,19 @@ Tensor cross_attn_mask(const Tensor& key_pad) {
   return bits;
 }
 
-// -> (output [B, Sq, H, D], lse2 [B, H, Sq] f32 or undefined, mask bits or undefined)
-std::tuple<Tensor, Tensor, Tensor> cross_attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
-                                                  const optional<Tensor>& key_pad, bool causal,
-                                                  double scale, bool want_lse) {
+// -> (output [B, Sq, H, D]; for a backward pass the remainders of its rounding
+// and lse2 [B, H, Sq] f32; mask bits), undefined where not there
+std::tuple<Tensor, Tensor, Tensor, Tensor> cross_attn_fwd(
+    const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& key_pad, bool causal,
+    double scale, bool want_lse) {
   auto a = cross_args(q, k, v, key_pad, c10::nullopt, causal, scale);
   c10::cuda::CUDAGuard guard(q.device());
   Tensor out = at::empty({a.B, a.Sq, a.H, a.D}, q.options());
   a.out = out.data_ptr();
-  Tensor lse, bits;
+  Tensor res, lse, bits;
   if (want_lse) {
+    res = at::empty({a.B, a.Sq, a.H, a.D}, q.options());
+    a.out_res = res.data_ptr();
     lse = at::empty({a.B, a.H, a.Sq}, q.options().dtype(at::kFloat));
     a.lse2 = lse.data_ptr<float>();
   }
@@ -174,12 +177,13 @@ std::tuple<Tensor, Tensor, Tensor> cross_attn_fwd(const Tensor& q, const Tensor&
     a.partials = part.data_ptr<float>();
   }
   FL_CUDA_OK(flodl::launch_cross_attn_fwd(a, cur_stream()));
-  return {out, lse, bits};
+  return {out, res, lse, bits};
 }
 
 // Gradients into dq, dk, dv (any strides of 16 bytes).
 void cross_attn_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v,
-                    const Tensor& out, const Tensor& lse2, const optional<Tensor>& key_pad,
+                    const Tensor& out, const Tensor& res, const Tensor& lse2,
+                    const optional<Tensor>& key_pad,
                     const optional<Tensor>& mask_bits, bool causal, double scale, Tensor& dq,
                     Tensor& dk, Tensor& dv) {
   auto a = cross_args(q, k, v, key_pad, mask_bits, causal, scale);
@@ -187,14 +191,16 @@ void cross_attn_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const 
   cross_strides(dq, "dq", a.B, a.Sq, a.H, a.D, q, a.dq_st);
   cross_strides(dk, "dk", a.B, a.Sk, a.Hk, a.D, q, a.dk_st);
   cross_strides(dv, "dv", a.B, a.Sk, a.Hk, a.D, q, a.dv_st);
-  FL_CHECK(out.sizes() == q.sizes() && out.is_contiguous() && out.scalar_type() == q.scalar_type() &&
-               out.device() == q.device(), "cross_attn: out must be the forward's");
+  for (const Tensor* t : {&out, &res})
+    FL_CHECK(t->sizes() == q.sizes() && t->is_contiguous() && t->scalar_type() == q.scalar_type() &&
+                 t->device() == q.device(), "cross_attn: out and its remainders must be the forward's");
   FL_CHECK(lse2.scalar_type() == at::kFloat && lse2.is_contiguous() &&
                lse2.numel() == (int64_t)a.B * a.H * a.Sq && lse2.device() == q.device(),
            "cross_attn: lse2 must be the forward's");
   c10::cuda::CUDAGuard guard(q.device());
   a.dout = dout.data_ptr();
   a.out = out.data_ptr();
+  a.out_res = res.data_ptr();
   a.lse2 = lse2.data_ptr<float>();
   a.dq = dq.data_ptr();
   a.dk = dk.data_ptr();
@@ -227,8 +233,8 @@ struct CrossAttn : public torch::autograd::Function<CrossAttn> {
                         const Tensor& v0, const optional<Tensor>& key_pad, bool causal,
                         double scale) {
     const Tensor q = tma_ready(q0), k = tma_ready(k0), v = tma_ready(v0);
-    auto [out, lse, bits] = cross_attn_fwd(q, k, v, key_pad, causal, scale, true);
-    ctx->save_for_backward({q, k, v, out, lse, key_pad ? *key_pad : Tensor(), bits});
+    auto [out, res, lse, bits] = cross_attn_fwd(q, k, v, key_pad, causal, scale, true);
+    ctx->save_for_backward({q, k, v, out, res, lse, key_pad ? *key_pad : Tensor(), bits});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     return out;
@@ -246,7 +252,7 @@ struct CrossAttn : public torch::autograd::Function<CrossAttn> {
       dq = at::empty(q.sizes(), q.options());
       dk = at::empty(k.sizes(), k.options());
       dv = at::empty(v.sizes(), v.options());
-      cross_attn_bwd(dout, q, k, v, s[3], s[4], if_defined(s[5]), if_defined(s[6]),
+      cross_attn_bwd(dout, q, k, v, s[3], s[4], s[5], if_defined(s[6]), if_defined(s[7]),
                      ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), dq, dk,
                      dv);
     }
@@ -300,12 +306,13 @@ void register_attention(py::module& m) {
   m.def("cross_attn_fwd",
         [](const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& key_pad,
            bool causal, double scale, bool want_lse) {
-          auto [out, lse, bits] = cross_attn_fwd(q, k, v, key_pad, causal, scale, want_lse);
-          return std::make_tuple(out, if_defined(lse), if_defined(bits));
+          auto [out, res, lse, bits] = cross_attn_fwd(q, k, v, key_pad, causal, scale, want_lse);
+          return std::make_tuple(out, if_defined(res), if_defined(lse), if_defined(bits));
         },
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("key_pad"), py::arg("causal"),
         py::arg("scale"), py::arg("want_lse"));
   m.def("cross_attn_bwd", &cross_attn_bwd, py::arg("dout"), py::arg("q"), py::arg("k"),
-        py::arg("v"), py::arg("out"), py::arg("lse2"), py::arg("key_pad"), py::arg("mask_bits"),
+        py::arg("v"), py::arg("out"), py::arg("res"), py::arg("lse2"), py::arg("key_pad"),
+        py::arg("mask_bits"),
         py::arg("causal"), py::arg("scale"), py::arg("dq"), py::arg("dk"), py::arg("dv"));
 }

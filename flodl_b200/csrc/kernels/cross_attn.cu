@@ -194,7 +194,22 @@ __device__ __forceinline__ void row16(uint32_t t, bool there, bool use, float f,
 // row per lane, an instruction touches 32 lines with 16 bytes each: the 128 rows
 // of dK and dV then took 3000 cycles.) `block`: the warp's 32 rows x 64 columns
 // in 128-byte swizzle.
-template <typename T>
+// Eight values in 16 bits; kRes: instead what that rounding leaves off.
+template <typename T, bool kRes>
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = Type<T>::pack(v[2 * i], v[2 * i + 1]);
+    if (kRes) {
+      float a, b;
+      f2_unpack(Type<T>::unpack(w[i]), a, b);
+      w[i] = Type<T>::pack(v[2 * i] - a, v[2 * i + 1] - b);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T, bool kRes>
 __device__ __forceinline__ void stage_rows(uint32_t t, int lane, bool use, float f, uint8_t* block) {
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
@@ -202,16 +217,16 @@ __device__ __forceinline__ void stage_rows(uint32_t t, int lane, bool use, float
     row16(t + c * 16, true, use, f, v);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      *reinterpret_cast<uint4*>(block + lane * 128 + (((2 * c + h) ^ (lane & 7)) << 4)) = make_uint4(
-          Type<T>::pack(v[8 * h], v[8 * h + 1]), Type<T>::pack(v[8 * h + 2], v[8 * h + 3]),
-          Type<T>::pack(v[8 * h + 4], v[8 * h + 5]), Type<T>::pack(v[8 * h + 6], v[8 * h + 7]));
+      *reinterpret_cast<uint4*>(block + lane * 128 + (((2 * c + h) ^ (lane & 7)) << 4)) =
+          pack8<T, kRes>(v + 8 * h);
   }
 }
-// The plain form: a row's columns below D as 16-bit values to out, or as f32 to
-// part (pieces of a split axis; rows without a visible tile).
+// The plain form: a row's columns below D as 16-bit values to out (and their
+// remainders to res), or as f32 to part (pieces of a split axis; rows without a
+// visible tile).
 template <typename T>
 __device__ __forceinline__ void store_row(uint32_t t, int D, bool there, bool use, bool row, float f,
-                                          T* out, float* part) {
+                                          T* out, T* res, float* part) {
 #pragma unroll 1
   for (int c = 0; c < D; c += 16) {
     float v[16];
@@ -220,10 +235,10 @@ __device__ __forceinline__ void store_row(uint32_t t, int D, bool there, bool us
     if (part == nullptr) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if (c + 8 * h < D)
-          *reinterpret_cast<uint4*>(out + c + 8 * h) = make_uint4(
-              Type<T>::pack(v[8 * h], v[8 * h + 1]), Type<T>::pack(v[8 * h + 2], v[8 * h + 3]),
-              Type<T>::pack(v[8 * h + 4], v[8 * h + 5]), Type<T>::pack(v[8 * h + 6], v[8 * h + 7]));
+        if (c + 8 * h < D) {
+          *reinterpret_cast<uint4*>(out + c + 8 * h) = pack8<T, false>(v + 8 * h);
+          if (res != nullptr) *reinterpret_cast<uint4*>(res + c + 8 * h) = pack8<T, true>(v + 8 * h);
+        }
     } else {
 #pragma unroll
       for (int h = 0; h < 4; ++h)
@@ -372,8 +387,9 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     cross_fwd_kernel(const __grid_constant__ CUtensorMap tm_q,
                      const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v,
-                     const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ Shape sh,
-                     T* __restrict__ out, float* __restrict__ lse2, float* __restrict__ part_o,
+                     const __grid_constant__ CUtensorMap tm_o,
+                     const __grid_constant__ CUtensorMap tm_r, const __grid_constant__ Shape sh,
+                     T* __restrict__ out, T* __restrict__ out_res, float* __restrict__ lse2, float* __restrict__ part_o,
                      float* __restrict__ part_lse, int n_items, int n_qt) {
   using Geo = FwdGeo<kDP>;
   constexpr uint32_t kStages = Geo::kStages, kQBufs = Geo::kQBufs;
@@ -643,9 +659,23 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       const int64_t lrow = ((int64_t)it.b * sh.H + it.h) * sh.Sq + qi;
       if (any && sh.splits == 1) {
         uint8_t* block = sm.q[qs.at] + (warp & 3) * 4096;
+        if (out_res != nullptr) {  // the remainders first: the same memory
+#pragma unroll 1
+          for (int c = 0; c < kDP / 64; ++c)
+            stage_rows<T, true>(t_o + c * 64, lane, !none, inv_l, block + c * kRows * 128);
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            for (int c = 0; c * 64 < sh.D; ++c)
+              tma_store_4d(&tm_r, block + c * kRows * 128, c * 64, qi - lane, it.h, it.b);
+            bulk_commit_group();
+            bulk_wait_group_read<0>();
+          }
+          __syncwarp();
+        }
 #pragma unroll 1
         for (int c = 0; c < kDP / 64; ++c)
-          stage_rows<T>(t_o + c * 64, lane, !none, inv_l, block + c * kRows * 128);
+          stage_rows<T, false>(t_o + c * 64, lane, !none, inv_l, block + c * kRows * 128);
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) {
@@ -655,6 +685,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         }
       } else {
         store_row<T>(t_o, sh.D, any, !none, qi < sh.Sq, inv_l, out + orow * sh.D,
+                     out_res != nullptr ? out_res + orow * sh.D : nullptr,
                      sh.splits > 1 ? part_o + (it.split * rows_all + orow) * sh.D : nullptr);
       }
       if (any) {
@@ -742,6 +773,7 @@ struct Stride3 {
 __host__ __device__ constexpr int stat_pitch(int Sq) { return (Sq + 63) / 64 * 64; }
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) cross_stats_kernel(const T* __restrict__ out,
+                                                          const T* __restrict__ out_res,
                                                           const T* __restrict__ dout, Stride3 ds,
                                                           const float* __restrict__ lse2,
                                                           float2* __restrict__ stats, int B, int Sq,
@@ -759,10 +791,15 @@ __global__ void __launch_bounds__(256) cross_stats_kernel(const T* __restrict__ 
     const int64_t b = bi / pitch;
     const int i = (int)(bi - b * pitch);
     float s = 0.f;
-    if (row < rows && i < Sq && part * 8 < D)
-      s = dot8<T>(
-          __ldg(reinterpret_cast<const uint4*>(out + ((b * Sq + i) * H + h) * D + part * 8)),
-          __ldg(reinterpret_cast<const uint4*>(dout + b * ds.b + i * ds.s + h * ds.h + part * 8)));
+    if (row < rows && i < Sq && part * 8 < D) {
+      const int64_t at = ((b * Sq + i) * H + h) * D + part * 8;
+      const uint4 g =
+          __ldg(reinterpret_cast<const uint4*>(dout + b * ds.b + i * ds.s + h * ds.h + part * 8));
+      s = dot8<T>(__ldg(reinterpret_cast<const uint4*>(out + at)), g);
+      // with what O's rounding left off: in a row that one key dominates, dP and
+      // delta nearly cancel, and the rounding of O would be the largest error
+      if (out_res != nullptr) s += dot8<T>(__ldg(reinterpret_cast<const uint4*>(out_res + at)), g);
+    }
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (row < rows && part == 0)
@@ -1247,7 +1284,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
         uint8_t* block = (second ? sm.a2[is.at] : sm.a1[is.at]) + (warp & 3) * 4096;
 #pragma unroll 1
         for (int c = kKeys ? 0 : group; c < kDP / 64; c += kKeys ? 1 : 2)
-          stage_rows<T>(t_a + c * 64, lane, true, f, block + c * kRows * 128);
+          stage_rows<T, false>(t_a + c * 64, lane, true, f, block + c * kRows * 128);
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) {
@@ -1265,7 +1302,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
         float* part = sh.splits == 1 ? nullptr
                                      : outs.part + ((int64_t)it.split * (kKeys ? 2 : 1) + (second ? 1 : 0)) *
                                                        rows_all * sh.D + flat * sh.D;
-        store_row<T>(t_a, sh.D, any, true, row < rows_n, f, dst, part);
+        store_row<T>(t_a, sh.D, any, true, row < rows_n, f, dst, (T*)nullptr, part);
       }
       if (any) {
         owed = &sm.a_empty[is.at];
@@ -1440,10 +1477,11 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   const int splits = fwd_splits(a);
   const int64_t rows = (int64_t)a.B * a.Sq * a.H;
   if (splits > 1 && !a.partials) return cudaErrorInvalidValue;
-  CUtensorMap mq, mk, mv, mo;
+  CUtensorMap mq, mk, mv, mo, mr;
   const int64_t o_st[3] = {(int64_t)a.Sq * a.H * a.D, (int64_t)a.H * a.D, a.D};
   if (!cross_attn_map(&mq, a.q, a.half, a.D, a.Sq, a.H, a.B, a.q_st, kRows) ||
       !cross_attn_map(&mo, a.out, a.half, a.D, a.Sq, a.H, a.B, o_st, 32) ||
+      (a.out_res && !cross_attn_map(&mr, a.out_res, a.half, a.D, a.Sq, a.H, a.B, o_st, 32)) ||
       !cross_attn_map(&mk, a.k, a.half, a.D, a.Sk, a.Hk, a.B, a.k_st, kN) ||
       !cross_attn_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kN))
     return cudaErrorInvalidValue;
@@ -1456,8 +1494,8 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   const int64_t items = (int64_t)n_qt * a.H * a.B * splits;
   if (items > 0x7fffffff - 4096) return cudaErrorInvalidValue;
   const int grid = (int)std::min<int64_t>(items, 2ll * num_sms());
-  e = launch_pdl(kernel, dim3(grid), dim3(kFwdThreads), smem, st, mq, mk, mv, mo, shape_of(a, splits, a.H),
-                 (T*)a.out, a.lse2, a.partials, a.partials + splits * rows * a.D, (int)items, n_qt);
+  e = launch_pdl(kernel, dim3(grid), dim3(kFwdThreads), smem, st, mq, mk, mv, mo,
+                 a.out_res ? mr : mo, shape_of(a, splits, a.H), (T*)a.out, (T*)a.out_res, a.lse2, a.partials, a.partials + splits * rows * a.D, (int)items, n_qt);
   if (e != cudaSuccess) return e;
   note_launch();
   return splits > 1 ? launch_cross_attn_join(a, splits, st) : cudaGetLastError();
@@ -1520,7 +1558,8 @@ cudaError_t run_stats(const CrossAttnArgs& a, cudaStream_t st) {
   const dim3 grid((unsigned)std::min<int64_t>((rows + per - 1) / per, num_sms() * 16ll));
   const Stride3 ds{a.do_st[0], a.do_st[1], a.do_st[2]};
   auto k = a.D <= 64 ? cross_stats_kernel<T, 8> : cross_stats_kernel<T, 16>;
-  cudaError_t e = launch_pdl(k, grid, dim3(256), 0, st, (const T*)a.out, (const T*)a.dout, ds,
+  cudaError_t e = launch_pdl(k, grid, dim3(256), 0, st, (const T*)a.out,
+                             (const T*)a.out_res, (const T*)a.dout, ds,
                              (const float*)a.lse2, (float2*)a.stats, a.B, a.Sq, a.H, a.D);
   if (e != cudaSuccess) return e;
   note_launch();

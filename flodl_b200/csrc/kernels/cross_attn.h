@@ -19,6 +19,8 @@ struct CrossAttnArgs {
   const void *q = nullptr, *k = nullptr, *v = nullptr;
   int64_t q_st[3] = {}, k_st[3] = {}, v_st[3] = {};
   void* out = nullptr;                 // [B, Sq, H, D] contiguous (backward: the forward's output)
+  void* out_res = nullptr;             // like out: what its rounding left off, rounded (nullable;
+                                       // the backward's row sums dO * O need it)
   float* lse2 = nullptr;               // [B, H, Sq] base-2 log-sum-exp, +inf for a row without a key
   const uint8_t* key_pad = nullptr;    // [B, Sk] contiguous, nonzero = hidden (nullable)
   // from cross_attn_pack_mask, only with key_pad and outside the few-row form

@@ -40,7 +40,7 @@ constexpr uint64_t kWaitNs = 2000000000ull;
 
 struct FewParams {
   const void* q;
-  void* out;
+  void *out, *out_res;
   float *lse2, *part_o, *part_lse;
   const uint8_t* key_pad;
   int64_t qb, qs, qh;
@@ -101,6 +101,20 @@ template <>
 __device__ __forceinline__ uint32_t pack<__half>(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// What the rounding of a pair to 16 bits leaves off, rounded.
+template <typename T>
+__device__ __forceinline__ uint32_t remainder2(uint32_t packed, float a, float b);
+template <>
+__device__ __forceinline__ uint32_t remainder2<__nv_bfloat16>(uint32_t packed, float a, float b) {
+  const float2 f = unpack_bf16x2(packed);
+  return pack<__nv_bfloat16>(a - f.x, b - f.y);
+}
+template <>
+__device__ __forceinline__ uint32_t remainder2<__half>(uint32_t packed, float a, float b) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&packed));
+  return pack<__half>(a - f.x, b - f.y);
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -367,7 +381,11 @@ __global__ void __launch_bounds__(kThreads, 3)
     const int64_t orow = ((int64_t)b * p.Sq + iq) * p.H + h;
     const int64_t lrow = ((int64_t)b * p.H + h) * p.Sq + iq;
     if (p.splits == 1) {
-      *reinterpret_cast<uint32_t*>((T*)p.out + orow * p.D + d) = pack<T>(a0 * inv, a1 * inv);
+      const uint32_t w = pack<T>(a0 * inv, a1 * inv);
+      *reinterpret_cast<uint32_t*>((T*)p.out + orow * p.D + d) = w;
+      if (p.out_res)
+        *reinterpret_cast<uint32_t*>((T*)p.out_res + orow * p.D + d) =
+            remainder2<T>(w, a0 * inv, a1 * inv);
       if (d == 0 && p.lse2) p.lse2[lrow] = none ? INFINITY : top + log2f(ll);
     } else {
       const int64_t rows_all = (int64_t)p.B * p.Sq * p.H;
@@ -383,7 +401,8 @@ __global__ void __launch_bounds__(kThreads, 3)
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part_o,
                                                    const float* __restrict__ part_lse,
-                                                   T* __restrict__ out, float* __restrict__ lse2,
+                                                   T* __restrict__ out, T* __restrict__ out_res,
+                                                   float* __restrict__ lse2,
                                                    int splits, int B, int Sq, int H, int D) {
   pdl_wait();
   pdl_trigger();
@@ -417,9 +436,13 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
     }
     const bool none = w == 0.f;
     const float inv = none ? 0.f : 1.f / w;
-    if (mine)
-      *reinterpret_cast<uint2*>(out + row * D + lane * 4) =
-          make_uint2(pack<T>(a.x * inv, a.y * inv), pack<T>(a.z * inv, a.w * inv));
+    if (mine) {
+      const uint2 w = make_uint2(pack<T>(a.x * inv, a.y * inv), pack<T>(a.z * inv, a.w * inv));
+      *reinterpret_cast<uint2*>(out + row * D + lane * 4) = w;
+      if (out_res)
+        *reinterpret_cast<uint2*>(out_res + row * D + lane * 4) =
+            make_uint2(remainder2<T>(w.x, a.x * inv, a.y * inv), remainder2<T>(w.y, a.z * inv, a.w * inv));
+    }
     if (lane == 0 && lse2) lse2[lrow] = none ? INFINITY : base + log2f(w);
   }
 }
@@ -464,7 +487,7 @@ int cross_attn_few_splits(const CrossAttnArgs& a) {
 
 cudaError_t launch_cross_attn_few(const CrossAttnArgs& a, cudaStream_t st) {
   FewParams p{};
-  p.q = a.q; p.out = a.out; p.lse2 = a.lse2; p.key_pad = a.key_pad;
+  p.q = a.q; p.out = a.out; p.out_res = a.out_res; p.lse2 = a.lse2; p.key_pad = a.key_pad;
   p.qb = a.q_st[0]; p.qs = a.q_st[1]; p.qh = a.q_st[2];
   p.B = a.B; p.Sq = a.Sq; p.Sk = a.Sk; p.H = a.H; p.Hk = a.Hk; p.D = a.D;
   p.G = a.H / a.Hk;
@@ -493,9 +516,9 @@ cudaError_t launch_cross_attn_join(const CrossAttnArgs& a, int splits, cudaStrea
   const int grid = (int)std::min<int64_t>((rows + 7) / 8, (int64_t)num_sms() * 8);
   cudaError_t e =
       a.half ? launch_pdl(join_kernel<__half>, dim3(grid), dim3(256), 0, st, po, pl, (__half*)a.out,
-                          a.lse2, splits, a.B, a.Sq, a.H, a.D)
+                          (__half*)a.out_res, a.lse2, splits, a.B, a.Sq, a.H, a.D)
              : launch_pdl(join_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, st, po, pl,
-                          (__nv_bfloat16*)a.out, a.lse2, splits, a.B, a.Sq, a.H, a.D);
+                          (__nv_bfloat16*)a.out, (__nv_bfloat16*)a.out_res, a.lse2, splits, a.B, a.Sq, a.H, a.D);
   if (e != cudaSuccess) return e;
   note_launch();
   return cudaGetLastError();

@@ -9,7 +9,8 @@ c 2 D u sum|q||k| + 2 u |c s| and its exponential by that and 2^-22, so a
 probability by a relative e, the largest of these over the row plus the row
 sum's e + 2 Sk u and the stored lse's rounding u |lse|. For the kernels
 probabilities and dS are rounded to the tensors' type (t each), and
-delta = sum dO * O uses the rounded O. The bounds below add these parts; the
+delta = sum dO * O uses O to t^2 (its rounding's remainder is kept, rounded)
+with the error of its probabilities. The bounds below add these parts; the
 composed form (f32 throughout, one rounding at the end) lies within them too.
 f16 has no normal numbers below 2^-14: a rounding there is off by up to 2^-25
 whatever the value (P is kept relative to a row's maximum or, for dV, at 2^7
@@ -66,7 +67,8 @@ def reference(q, k, v, pad, causal, scale, dout=None):
     dO = dout.double().transpose(1, 2)
     dP = dO @ V.transpose(-1, -2)
     delta = (dO * O).sum(-1, keepdim=True)
-    b_dP = 2 * D * U * (dO.abs() @ V.abs().transpose(-1, -2)) + (dO.abs() * bO).sum(-1, keepdim=True) \
+    err_O = bO - (t - 2 * t * t) * O.abs()  # of O before its rounding, and of the remainder's
+    b_dP = 2 * D * U * (dO.abs() @ V.abs().transpose(-1, -2)) + (dO.abs() * err_O).sum(-1, keepdim=True) \
         + 2 * D * U * (dO * O).abs().sum(-1, keepdim=True)
     dS = P * (dP - delta)
     b_dS = (P * b_dP + (t + e) * dS.abs() + sub) * vis
