@@ -597,18 +597,34 @@ class MultiheadAttention(NamedInputModule):
 
     Self-attention packs Q/K/V into one projection GEMM and runs the sm_100a
     flash kernel on the packed buffer. Cross-attention (``using`` a tagged
-    memory) projects K/V from the memory tensor.
+    memory) projects K/V from the memory tensor - of any length - and runs
+    :func:`flodl_b200.ops.cross_attention` on the packed projection; a query
+    whose memory is hidden entirely gets zeros.
+
+    ``qk_norm`` norms the queries and keys of each head (RMSNorm with weights
+    ``q_norm.weight`` / ``k_norm.weight`` over the head size); ``rotary`` (a
+    :class:`RotaryEmbedding` of at most the head size) turns them by their
+    positions, in self-attention only. Together they run as one pass over the
+    packed projection (:func:`flodl_b200.ops.attention_qk_norm`).
     """
 
     NAME = "multihead_attention"
 
-    def __init__(self, embed_dim: int, num_heads: int, causal: bool = False, device=None):
+    def __init__(self, embed_dim: int, num_heads: int, causal: bool = False, device=None,
+                 qk_norm: bool = False, rotary: Optional["RotaryEmbedding"] = None):
         super().__init__()
         assert embed_dim % num_heads == 0
         self.embed_dim, self.num_heads, self.causal = embed_dim, num_heads, causal
         dev = _dev(device)
         self.qkv = Linear(embed_dim, 3 * embed_dim, device=dev)
         self.out_proj = Linear(embed_dim, embed_dim, device=dev)
+        head = embed_dim // num_heads
+        self.q_norm = RMSNorm(head, device=dev) if qk_norm else None
+        self.k_norm = RMSNorm(head, device=dev) if qk_norm else None
+        if rotary is not None and 2 * rotary.cos.shape[1] > head:
+            raise ValueError(f"rotary turns {2 * rotary.cos.shape[1]} values, more than the head "
+                             f"size {head}")
+        self.rotary = rotary
 
     def forward_named(self, x, refs):
         memory = None
@@ -616,28 +632,60 @@ class MultiheadAttention(NamedInputModule):
             memory = next(iter(refs.values()))
         return self.attend(x, memory)
 
-    def forward(self, x, refs=None, key_padding_mask=None):
+    def forward(self, x, refs=None, key_padding_mask=None, positions=None):
+        """``positions`` (int64 ``[B, S]``) are the rotary positions of a batch
+        whose sequences do not start at 0 (left padding)."""
         if isinstance(refs, torch.Tensor):
-            return self.attend(x, refs, key_padding_mask)
-        return self.attend(x, next(iter(refs.values())) if refs else None, key_padding_mask)
+            return self.attend(x, refs, key_padding_mask, positions)
+        return self.attend(x, next(iter(refs.values())) if refs else None, key_padding_mask, positions)
 
-    def attend(self, x, memory=None, key_padding_mask=None):
+    def _cross(self, x, q, kv, key_padding_mask, causal=False):
         B, S, Cd = x.shape
         H = self.num_heads
-        D = Cd // H
-        if memory is None:
-            qkv = self.qkv(x.reshape(B * S, Cd))
-            o = ops.attention_packed(qkv, B, S, H, self.causal, key_padding_mask)
+        q = q.view(B, S, H, Cd // H)
+        kv = kv.view(B, kv.shape[1], 2, H, Cd // H)
+        if self.q_norm is not None:
+            k = ops.rms_norm(kv[:, :, 0], self.k_norm.weight, self.k_norm.eps)
+            q = ops.rms_norm(q, self.q_norm.weight, self.q_norm.eps)
+            return ops.cross_attention(q, k, kv[:, :, 1], key_padding_mask, causal).view(B * S, Cd)
+        return ops.cross_attention_packed(q, kv, key_padding_mask, causal).view(B * S, Cd)
+
+    def attend(self, x, memory=None, key_padding_mask=None, positions=None):
+        B, S, Cd = x.shape
+        H = self.num_heads
+        if positions is not None and (memory is not None or self.rotary is None):
+            raise ValueError("positions need self-attention with a rotary embedding")
+        if memory is not None:
+            q, kv = ops.cross_projection(x, memory, self.qkv.weight, self.qkv.bias)
+            o = self._cross(x, q, kv, key_padding_mask, self.causal and S == memory.shape[1])
         else:
-            Wq, Wk, Wv = self.qkv.weight.chunk(3, 0)
-            bq, bk, bv = (self.qkv.bias.chunk(3, 0) if self.qkv.bias is not None else (None,) * 3)
-            q = ops.linear(x, Wq, bq).view(B, S, H, D).transpose(1, 2)
-            Sm = memory.shape[1]
-            k = ops.linear(memory, Wk, bk).view(B, Sm, H, D).transpose(1, 2)
-            v = ops.linear(memory, Wv, bv).view(B, Sm, H, D).transpose(1, 2)
-            mask = None if key_padding_mask is None else ~key_padding_mask[:, None, None, :]
-            o = ops.scaled_dot_product_attention(q, k, v, mask, self.causal and S == Sm)
-            o = o.transpose(1, 2).reshape(B * S, Cd)
+            qkv = self.qkv(x.reshape(B * S, Cd))
+            if self.q_norm is not None:
+                cos, sin = (self.rotary.cos, self.rotary.sin) if self.rotary is not None else (None, None)
+                o = ops.attention_qk_norm(qkv, B, S, H, self.q_norm.weight, self.k_norm.weight, cos, sin,
+                                          self.causal, key_padding_mask, positions, self.q_norm.eps)
+            elif self.rotary is not None:
+                q, k, v = qkv.view(B, S, 3, H, Cd // H).unbind(2)
+                q, k = (self.rotary.rotate(t.transpose(1, 2), positions).transpose(1, 2) for t in (q, k))
+                o = ops.cross_attention(q, k, v, key_padding_mask, self.causal).view(B * S, Cd)
+            else:
+                o = ops.attention_packed(qkv, B, S, H, self.causal, key_padding_mask)
+        return self.out_proj(o).reshape(B, S, Cd).to(x.dtype)
+
+    @torch.no_grad()
+    def project_memory(self, memory):
+        """Keys and values ``[B, Sm, 2C]`` of a memory, for :meth:`attend_memory`
+        at every step of serving (no gradients)."""
+        n = self.embed_dim
+        return ops.project_rows(memory, self.qkv.weight, self.qkv.bias, n, 3 * n)
+
+    @torch.no_grad()
+    def attend_memory(self, x, memory_kv, key_padding_mask=None):
+        """Cross-attention of ``x [B, S, C]`` (a new token, or a few) over
+        :meth:`project_memory`'s result."""
+        B, S, Cd = x.shape
+        q = ops.project_rows(x, self.qkv.weight, self.qkv.bias, 0, self.embed_dim)
+        o = self._cross(x, q, memory_kv, key_padding_mask)
         return self.out_proj(o).reshape(B, S, Cd).to(x.dtype)
 
 
@@ -661,3 +709,15 @@ class RotaryEmbedding(Module):
         x1, x2 = x[..., 0::2], x[..., 1::2]
         out = torch.stack((x1 * cos - x2 * sin, x1 * sin + x2 * cos), dim=-1)
         return out.flatten(-2)
+
+    def rotate(self, x, positions=None):
+        """The first ``dim`` values of each head of ``x [B, H, S, D]``, turned by
+        positions 0.. or ``positions [B, S]``; the others as they are."""
+        R = 2 * self.cos.shape[1]
+        if positions is None:
+            y = self.forward(x[..., :R])
+        else:
+            cos, sin = (t[positions][:, None].to(x.dtype) for t in (self.cos, self.sin))
+            x1, x2 = x[..., 0:R:2], x[..., 1:R:2]
+            y = torch.stack((x1 * cos - x2 * sin, x1 * sin + x2 * cos), dim=-1).flatten(-2)
+        return torch.cat((y, x[..., R:]), -1) if R < x.shape[-1] else y

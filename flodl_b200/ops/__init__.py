@@ -1,7 +1,7 @@
 """Fused op layer: autograd Functions over the sm_100a kernel library."""
-from .attention import (attention_packed, cross_attention,  # noqa: F401
-                        scaled_dot_product_attention)
-from .linear import linear  # noqa: F401
+from .attention import (attention_packed, attention_qk_norm, cross_attention,  # noqa: F401
+                        cross_attention_packed, scaled_dot_product_attention)
+from .linear import cross_projection, linear, project_rows  # noqa: F401
 from .loss import cross_entropy  # noqa: F401
 from .misc import (batch_norm2d, conv1d, conv2d, conv_transpose1d, conv_transpose2d,  # noqa: F401
                    dropout, embedding, gelu, max_pool1d, max_pool2d)

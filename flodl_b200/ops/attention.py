@@ -15,8 +15,10 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from ._common import C, use_kernels
+from .norm import qk_norm_rope
 
 
 def attn_fwd_packed(qkv: torch.Tensor, B: int, S: int, H: int, causal: bool,
@@ -195,3 +197,127 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite (got {scale})")
     return _cross_composed(q, k, v, key_padding, causal, scale)
+
+
+def _fresh(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and 16-byte aligned."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class _CrossPackedFn(torch.autograd.Function):
+    """cross_attention on a packed key/value projection: the gradient comes as
+    one packed tensor, without copies of its halves."""
+
+    @staticmethod
+    def forward(ctx, q, kv, key_padding, causal, scale):
+        q, kv = _fresh(q), _fresh(kv)
+        out, res, lse, bits = C().cross_attn_fwd(q, kv[:, :, 0], kv[:, :, 1], key_padding, causal, scale,
+                                                 True)
+        ctx.save_for_backward(q, kv, out, res, lse, key_padding, bits)
+        ctx.consts = (causal, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, kv, out, res, lse, key_padding, bits = ctx.saved_tensors
+        dq, dkv = torch.empty_like(q), torch.empty_like(kv)
+        C().cross_attn_bwd(_fresh(dout.to(q.dtype)), q, kv[:, :, 0], kv[:, :, 1], out, res, lse,
+                           key_padding, bits, *ctx.consts, dq, dkv[:, :, 0], dkv[:, :, 1])
+        return dq, dkv, None, None, None
+
+
+def _kernels_take(t: torch.Tensor) -> bool:
+    D = t.shape[-1]
+    return (use_kernels(t) and t.dtype in (torch.bfloat16, torch.float16) and D % 8 == 0 and D <= 128
+            and t.numel() > 0)
+
+
+def cross_attention_packed(q: torch.Tensor, kv: torch.Tensor,
+                           key_padding: Optional[torch.Tensor] = None, causal: bool = False,
+                           scale: Optional[float] = None) -> torch.Tensor:
+    """:func:`cross_attention` with the memory's keys and values in one packed
+    projection ``kv [B, Sk, 2, Hk, D]``; its gradient is packed likewise."""
+    if kv.dim() != 5 or kv.shape[2] != 2:
+        raise ValueError(f"packed keys and values are [B, Sk, 2, Hk, D] (got {tuple(kv.shape)})")
+    if (torch.is_grad_enabled() and (q.requires_grad or kv.requires_grad) and q.dim() == 4
+            and _kernels_take(q) and kv.numel() > 0 and kv.dtype == q.dtype and kv.device == q.device
+            and kv.shape[0] == q.shape[0] and kv.shape[4] == q.shape[3]
+            and q.shape[2] % kv.shape[3] == 0 and not (causal and q.shape[1] != kv.shape[1])):
+        pad = key_padding
+        ok = pad is None or (pad.dtype == torch.bool and pad.shape == kv.shape[:2]
+                             and pad.device == q.device)
+        c = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
+        if ok and c > 0.0 and math.isfinite(c):
+            return _CrossPackedFn.apply(q, kv, pad.contiguous() if pad is not None else None,
+                                        bool(causal), c)
+    return cross_attention(q, kv[:, :, 0], kv[:, :, 1], key_padding, causal, scale)
+
+
+class _QkNormAttnFn(torch.autograd.Function):
+    """Norm and rotation of a packed projection's queries and keys, then
+    attention with its values in place; the packed gradient is written once."""
+
+    @staticmethod
+    def forward(ctx, qkv, q_weight, k_weight, cos, sin, positions, eps, causal, key_padding, scale):
+        qkv = _fresh(qkv)
+        q, k, v = qkv.unbind(2)
+        det = (lambda w: w.detach() if w is not None else None)
+        yq, yk = C().qk_norm_rope(q, k, det(q_weight), det(k_weight), cos, sin, positions, 0, eps)
+        out, res, lse, bits = C().cross_attn_fwd(yq, yk, v, key_padding, causal, scale, True)
+        ctx.save_for_backward(qkv, yq, yk, q_weight, k_weight, cos, sin, positions, out, res, lse,
+                              key_padding, bits)
+        ctx.consts = (eps, causal, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        (qkv, yq, yk, q_weight, k_weight, cos, sin, positions, out, res, lse, key_padding,
+         bits) = ctx.saved_tensors
+        eps, causal, scale = ctx.consts
+        dqkv = torch.empty_like(qkv)
+        q, k, v = qkv.unbind(2)
+        dq, dk, dv = dqkv.unbind(2)
+        dyq, dyk = torch.empty_like(yq), torch.empty_like(yk)
+        C().cross_attn_bwd(_fresh(dout.to(qkv.dtype)), yq, yk, v, out, res, lse, key_padding, bits,
+                           causal, scale, dyq, dyk, dv)
+        dwq, dwk = C().qk_norm_rope_backward(dyq, dyk, q, k, q_weight, k_weight, cos, sin, positions,
+                                             0, eps, dq, dk)
+        return dqkv, dwq, dwk, None, None, None, None, None, None, None
+
+
+def attention_qk_norm(qkv: torch.Tensor, B: int, S: int, H: int, q_weight: Optional[torch.Tensor] = None,
+                      k_weight: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+                      sin: Optional[torch.Tensor] = None, causal: bool = False,
+                      key_padding: Optional[torch.Tensor] = None,
+                      positions: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """Self-attention over packed ``qkv [B*S, 3C]`` whose queries and keys are
+    normed per head and rotated first (:func:`qk_norm_rope`, then
+    :func:`cross_attention` over the same positions); returns ``[B*S, C]``."""
+    if qkv.dim() != 2 or qkv.shape[0] != B * S or qkv.shape[1] % (3 * H):
+        raise ValueError(f"qkv must be [{B * S}, 3 * {H} * D] (got {tuple(qkv.shape)})")
+    if use_kernels(qkv) and qkv.dtype not in (torch.bfloat16, torch.float16):
+        qkv = qkv.to(torch.bfloat16)
+    D = qkv.shape[1] // (3 * H)
+    packed = qkv.view(B, S, 3, H, D) if qkv.is_contiguous() else qkv.reshape(B, S, 3, H, D)
+    needs = any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight))
+    if torch.is_grad_enabled() and needs and _kernels_take(packed):
+        # the checks of both operators, on views (nothing is launched for them)
+        from .norm import check_qk_norm_rope
+        check_qk_norm_rope(packed[:, :, 0], packed[:, :, 1], q_weight, k_weight, cos, sin, positions, 0)
+        if key_padding is not None and (key_padding.dtype != torch.bool
+                                        or key_padding.shape != (B, S)
+                                        or key_padding.device != qkv.device):
+            raise ValueError(f"key_padding must be bool [{B}, {S}] on {qkv.device}")
+        if cos is not None and cos.shape[1] == 0:
+            cos = sin = positions = None
+        c = (lambda t: t.contiguous() if t is not None else None)
+        out = _QkNormAttnFn.apply(packed, c(q_weight), c(k_weight), c(cos), c(sin), c(positions),
+                                  float(eps), bool(causal), c(key_padding), 1.0 / math.sqrt(D))
+    else:
+        q, k, v = packed.unbind(2)
+        q, k = qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=positions, eps=eps)
+        out = cross_attention(q, k, v, key_padding, causal)
+    return out.reshape(B * S, H * D)

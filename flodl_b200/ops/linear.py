@@ -237,3 +237,95 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         y = F.relu(y) if act == "relu" else y
         return y if residual is None else residual + y
     return _LinearFn.apply(x, weight, bias, act, residual)
+
+
+def _rows_gemm(x2, w16, bias, bias16):
+    """``x2 @ w16^T + bias`` in bf16 for a row range of a weight's shadow; a few
+    output tiles go to the library GEMM, as in :func:`linear`."""
+    T, K = x2.shape
+    N = w16.shape[0]
+    if _few_tiles(T, N):
+        return F.linear(x2, w16, bias16)
+    out = torch.empty((T, N), device=x2.device, dtype=torch.bfloat16)
+    C().gemm(x2, w16, out, T, N, K, False, False, bias=bias)
+    return out
+
+
+def _rows_dgrad(dy2, w16, x):
+    T, N = dy2.shape
+    K = w16.shape[1]
+    if _few_tiles(T, K):
+        return torch.mm(dy2, w16).reshape(x[0]).to(x[1])
+    dx = torch.empty((T, K), device=dy2.device,
+                     dtype=torch.float32 if x[1] == torch.float32 else torch.bfloat16)
+    C().gemm(dy2, w16, dx, T, K, N, False, True)
+    return dx.reshape(x[0])
+
+
+class _CrossProjFn(torch.autograd.Function):
+    """Query projection of ``x`` and key/value projection of ``memory`` by row
+    ranges of one packed weight; the weight's gradients accumulate into their
+    ranges of ``.grad`` and its listeners are notified once."""
+
+    @staticmethod
+    def forward(ctx, x, memory, weight, bias):
+        n = weight.shape[0] // 3
+        x2, m2, w16 = as_bf16_2d(x), as_bf16_2d(memory), bf16_shadow(weight)
+        b = bias.detach() if bias is not None else None
+        b16 = bf16_shadow(bias) if bias is not None else None
+        part = (lambda t, lo, hi: t[lo:hi] if t is not None else None)
+        q = _rows_gemm(x2, w16[:n], part(b, 0, n), part(b16, 0, n))
+        kv = _rows_gemm(m2, w16[n:], part(b, n, None), part(b16, n, None))
+        ctx.save_for_backward(x2, m2, weight, bias)
+        ctx.like = (x.shape, x.dtype), (memory.shape, memory.dtype)
+        return q.reshape(*x.shape[:-1], n), kv.reshape(*memory.shape[:-1], 2 * n)
+
+    @staticmethod
+    def backward(ctx, dq, dkv):
+        x2, m2, weight, bias = ctx.saved_tensors
+        n, K = weight.shape[0] // 3, weight.shape[1]
+        dq2, dkv2, w16 = as_bf16_2d(dq), as_bf16_2d(dkv), bf16_shadow(weight)
+        dx = _rows_dgrad(dq2, w16[:n], ctx.like[0]) if ctx.needs_input_grad[0] else None
+        dm = _rows_dgrad(dkv2, w16[n:], ctx.like[1]) if ctx.needs_input_grad[1] else None
+        for dy2, in2, lo, hi in ((dq2, x2, 0, n), (dkv2, m2, n, 3 * n)):
+            if wants_grad(weight):
+                C().gemm(dy2, in2, grad_buffer(weight)[lo:hi], hi - lo, K, in2.shape[0], True, True,
+                         flags=C().EPI_ACCUMULATE, k_splits=splitk_for(hi - lo, K, in2.shape[0]))
+            if wants_grad(bias):
+                C().colsum(dy2, grad_buffer(bias)[lo:hi])
+        for t in (weight, bias):
+            if wants_grad(t):
+                grad_ready(t)
+        return dx, dm, None, None
+
+
+def cross_projection(x: torch.Tensor, memory: torch.Tensor, weight: torch.Tensor,
+                     bias: Optional[torch.Tensor] = None):
+    """``(queries of x, keys and values of memory)`` by a packed ``[3N, K]``
+    weight's rows: ``x [..., K] -> [..., N]``, ``memory [..., K] -> [..., 2N]``."""
+    n = weight.shape[0] // 3
+    if use_kernels(x) and n % 8 == 0 and weight.shape[1] % 8 == 0 and weight.is_leaf:
+        return _CrossProjFn.apply(x, memory, weight, bias)
+    if use_kernels(x):
+        x, memory, weight = x.bfloat16(), memory.bfloat16(), weight.bfloat16()
+        bias = bias.bfloat16() if bias is not None else None
+    part = (lambda lo, hi: bias[lo:hi] if bias is not None else None)
+    return (F.linear(x, weight[:n], part(0, n)), F.linear(memory, weight[n:], part(n, None)))
+
+
+@torch.no_grad()
+def project_rows(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], lo: int,
+                 hi: int) -> torch.Tensor:
+    """``x @ weight[lo:hi]^T + bias[lo:hi]`` without gradients: one part of a
+    packed projection, from the weight's cached bf16 shadow on CUDA."""
+    part = (lambda t: t[lo:hi] if t is not None else None)
+    if not use_kernels(x):
+        return F.linear(x, weight[lo:hi], part(bias))
+    b16 = bf16_shadow(bias) if bias is not None else None
+    w16 = bf16_shadow(weight)[lo:hi]
+    x2 = as_bf16_2d(x)
+    if (hi - lo) % 8 or weight.shape[1] % 8 or lo * weight.shape[1] % 8:
+        y = F.linear(x2, w16, part(b16))
+    else:
+        y = _rows_gemm(x2, w16, part(bias.detach() if bias is not None else None), part(b16))
+    return y.reshape(*x.shape[:-1], hi - lo)

@@ -154,7 +154,8 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     return _GroupNormFn.apply(x, int(groups), weight, bias, float(eps))
 
 
-def _check_qk(q, k, q_weight, k_weight, cos, sin, positions, offset):
+def check_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, offset):
+    """Raises ValueError for arguments that :func:`qk_norm_rope` does not take."""
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError(f"qk_norm_rope takes [B, S, heads, D] queries and keys (got {tuple(q.shape)}"
                          f" and {tuple(k.shape)})")
@@ -172,6 +173,9 @@ def _check_qk(q, k, q_weight, k_weight, cos, sin, positions, offset):
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
     if cos is None:
+        if use_kernels(q) and any(t is not None and t.dtype != torch.float32
+                                  for t in (q_weight, k_weight)):
+            raise ValueError("on CUDA the weights must be f32")
         if positions is not None:
             raise ValueError("positions need the cos and sin tables")
         return
@@ -180,6 +184,9 @@ def _check_qk(q, k, q_weight, k_weight, cos, sin, positions, offset):
                          f"{tuple(cos.shape)} and {tuple(sin.shape)})")
     if cos.device != q.device or sin.device != q.device:
         raise ValueError("the tables must be on the inputs' device")
+    if use_kernels(q) and any(t is not None and t.dtype != torch.float32
+                              for t in (q_weight, k_weight, cos, sin)):
+        raise ValueError("on CUDA the weights and tables must be f32")
     if positions is not None:
         if offset != 0:
             raise ValueError("give positions or an offset, not both")
@@ -230,7 +237,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
         y = C().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, offset, eps)
         if y is not None:
             return y
-    _check_qk(q, k, q_weight, k_weight, cos, sin, positions, offset)
+    check_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, offset)
     if cos is not None and cos.shape[1] == 0:
         cos = sin = positions = None
     c = s = None
