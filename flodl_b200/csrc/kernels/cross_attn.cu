@@ -211,7 +211,7 @@ __device__ __forceinline__ uint4 pack8(const float* v) {
 }
 template <typename T, bool kRes>
 __device__ __forceinline__ void stage_rows(uint32_t t, int lane, bool use, float f, uint8_t* block) {
-#pragma unroll 1
+#pragma unroll 2
   for (int c = 0; c < 4; ++c) {
     float v[16];
     row16(t + c * 16, true, use, f, v);
@@ -255,7 +255,7 @@ struct Shape {
   float scale;
   const uint32_t* words;  // [B, nwords] or null
   const int* vis_end;     // [B]
-  int nwords;
+  int nwords, n_items;
   uint32_t* err;
   // item -> (row tile, batch, head, piece): divisors of an item's index
   FastDiv by_splits, by_bh, by_heads, by_group;
@@ -324,15 +324,18 @@ __device__ __forceinline__ void settle(uint64_t* bar, uint32_t issued) {
 // Two CTAs per SM (256 TMEM columns, 97 KB of shared memory each) cover each
 // other's waits. TMEM: two score buffers at 0 and 64, P over its own scores, O
 // at 128. S of a tile is computed while the softmax works on the one before;
-// P V of a tile is issued behind S of the next.
+// P V of a tile is issued behind S of the next. (Three CTAs with one score buffer
+// each, at head size 64, have 96 registers a thread and spill: 87 instead of 62
+// us on 8 x 16 heads, 1024 x 1024.)
 constexpr int kN = 64;
-constexpr uint32_t kTmemO = 128;
 constexpr int kFwdThreads = 192;
 template <int kDP>
 struct FwdGeo {
   static constexpr int kQBufs = kDP == 64 ? 2 : 1;
   static constexpr int kStages = kDP == 64 ? 4 : 2;
 };
+constexpr int kFwdCtas = 2;       // per SM
+constexpr uint32_t kTmemO = 128;
 
 template <int kDP>
 struct FwdSmem {
@@ -353,7 +356,8 @@ struct FwdItem {
   int qt, h, b, split, lo, hi;  // key tiles [lo, hi)
 };
 __device__ __forceinline__ FwdItem fwd_item(const Shape& s, int item, int n_qt) {
-  FwdItem it;
+  FwdItem it{};
+  if (item >= s.n_items) return it;  // asked for ahead of time
   const ItemAt at = item_at(s, item);
   it.split = at.split;
   it.qt = n_qt - 1 - at.rt;
@@ -382,8 +386,8 @@ __device__ __forceinline__ uint2 tile_words(const Shape& s, int b, int k0) {
 }
 __device__ __forceinline__ bool is_whole(uint2 w) { return (w.x & w.y) == 0xffffffffu; }
 
-template <typename T, int kDP>
-__global__ void __launch_bounds__(kFwdThreads, 2)
+template <typename T, int kDP, bool kTrain>
+__global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
     cross_fwd_kernel(const __grid_constant__ CUtensorMap tm_q,
                      const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v,
@@ -410,12 +414,11 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       mbar_init(&sm.v_full[i], 1);
       mbar_init(&sm.v_empty[i], 1);
     }
-    mbar_init(&sm.s_full[0], 1);
-    mbar_init(&sm.s_full[1], 1);
-    mbar_init(&sm.p_full[0], 4);
-    mbar_init(&sm.p_full[1], 4);
-    mbar_init(&sm.pv_done[0], 1);
-    mbar_init(&sm.pv_done[1], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[i], 4);
+      mbar_init(&sm.pv_done[i], 1);
+    }
     mbar_init(&sm.drain, 1);
     sm.abort = 0;
     fence_mbar_init();
@@ -475,26 +478,30 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       const uint32_t q0 = smem_u32(sm.q[0]), k0 = smem_u32(sm.k[0]), v0 = smem_u32(sm.v[0]);
       Ring<kStages> ks, vs;  // stages of K (tile t) and V (the tile behind)
       Ring<kQBufs> qs;
-      uint32_t t = 0;  // tile whose S is issued next
+      Ring<2> ss, ps;   // score buffers of tile t and of the tile behind
       bool ok = true, issued = false;
-      // P V of tile t - 1
+      // P V of the tile behind
       auto issue_pv = [&](bool acc) -> bool {
-        const uint32_t u = t - 1;
         if (!wait(&sm.v_full[vs.at], vs.phase)) return false;
-        if (!wait(&sm.p_full[u & 1], (u >> 1) & 1)) return false;
+        if (!wait(&sm.p_full[ps.at], ps.phase)) return false;
         tc_fence_after();
-        mma_cols<kN, kDP>(tmem + kTmemO, tmem + (u & 1) * 64u, v0 + vs.at * (kN * kDP * 2), id_o, acc);
-        umma_commit(&sm.pv_done[u & 1]);
+        mma_cols<kN, kDP>(tmem + kTmemO, tmem + ps.at * 64u, v0 + vs.at * (kN * kDP * 2), id_o, acc);
+        umma_commit(&sm.pv_done[ps.at]);
         umma_commit(&sm.v_empty[vs.at]);
         vs.next();
+        ps.next();
         return true;
       };
       // P V of a tile is issued behind S of the next one, over item borders too
       // where the next item's Q has a buffer of its own
       bool behind = false, behind_acc = false;
+      FwdItem after = fwd_item(sh, blockIdx.x, n_qt);
       for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-        const FwdItem it = fwd_item(sh, item, n_qt);
-        if (it.lo >= it.hi) continue;
+        const FwdItem it = after;
+        if (it.lo >= it.hi) {
+          after = fwd_item(sh, item + gridDim.x, n_qt);
+          continue;
+        }
         if (kQBufs == 1 && behind) {
           if (!(ok = issue_pv(behind_acc))) break;
           behind = false;
@@ -504,15 +511,15 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         for (int j = it.lo; j < it.hi; ++j) {
           if (!(ok = wait(&sm.k_full[ks.at], ks.phase))) break;
           tc_fence_after();
-          // this buffer's scores of tile t - 2 became P, whose product was
-          // issued before: in order
-          mma_rows<kRows, kN, kDP>(tmem + (t & 1) * 64u, q_addr, k0 + ks.at * (kN * kDP * 2), id_s);
+          // the products with this buffer's last P were issued before: in order
+          mma_rows<kRows, kN, kDP>(tmem + ss.at * 64u, q_addr, k0 + ks.at * (kN * kDP * 2), id_s);
           issued = true;
-          umma_commit(&sm.s_full[t & 1]);
+          umma_commit(&sm.s_full[ss.at]);
           umma_commit(&sm.k_empty[ks.at]);
           ks.next();
+          ss.next();
+          if (j == it.hi - 1) after = fwd_item(sh, item + gridDim.x, n_qt);  // while products run
           if (behind && !(ok = issue_pv(behind_acc))) break;
-          ++t;
           behind = true;
           behind_acc = j > it.lo;
         }
@@ -532,7 +539,8 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     const uint32_t t_o = tmem + kTmemO + lanes;
     const float sl2 = sh.scale * kLog2e;
     const uint64_t sl2x2 = f2_splat(sl2);
-    uint32_t t = 0;
+    Ring<2> ss, last;  // score buffers of this tile and of the one before
+    Ring<kStages> vs;
     Ring<kQBufs> qs;
     bool ok = true;
     // The Q buffer whose output store may still be read: given back once the
@@ -545,21 +553,23 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       }
       owed = nullptr;
     };
+    FwdItem after = fwd_item(sh, blockIdx.x, n_qt);
     for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-      const FwdItem it = fwd_item(sh, item, n_qt);
+      const FwdItem it = after;
       const int qi = it.qt * kRows + r;
       // tiles before `plain` hold no hidden score
       int plain = sh.Sk / kN;
       if (sh.causal) plain = min(plain, (it.qt * kRows + 1) / kN);
       if (sh.words) plain = 0;
-      // Reference maximum (scaled, log2 units). l sums P as computed, for the
-      // lse; lr sums P as rounded for the product, which O is divided by: a
-      // row's O is then a mean of its values with weights that add up to 1.
+      // Reference maximum (scaled, log2 units), and the sum of P. For a backward
+      // pass lr sums P as rounded for the product as well, and O is divided by
+      // it: a mean of the values with weights that add up to 1, or else a row
+      // that one key dominates has that weight's rounding in its dO * O.
       float m_ref = -INFINITY, l = 0.f, lr = 0.f;
       uint2 words = sh.words && it.lo < it.hi ? tile_words(sh, it.b, it.lo * kN) : make_uint2(0, 0);
-      for (int j = it.lo; j < it.hi; ++j, ++t) {
-        const uint32_t t_s = tmem + lanes + (t & 1) * 64u;
-        ok = wait(&sm.s_full[t & 1], (t >> 1) & 1);
+      for (int j = it.lo; j < it.hi; ++j) {
+        const uint32_t t_s = tmem + lanes + ss.at * 64u;
+        ok = wait(&sm.s_full[ss.at], ss.phase);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
         uint32_t v[64];  // the row's scores
@@ -574,10 +584,9 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
             for (int i = 0; i < 64; ++i)
               v[i] = (((i < 32 ? w.x : w.y) >> (i % 32)) & 1u) && i <= lim ? v[i] : 0xff800000u;
             if (sh.words && !is_whole(w)) {
-              const uint32_t st = t % kStages;
-              ok = wait(&sm.v_full[st], (t / kStages) & 1);
+              ok = wait(&sm.v_full[vs.at], vs.phase);
               if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-              zero_hidden_rows<kN, kDP>(sm.v[st], w, threadIdx.x - 64, 128);
+              zero_hidden_rows<kN, kDP>(sm.v[vs.at], w, threadIdx.x - 64, 128);
             }
           }
         }
@@ -594,12 +603,12 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
           const float c = (move && m_ref != -INFINITY) ? ex2(m_ref - mx) : 1.f;
           if (move) m_ref = mx;
           l *= c;
-          lr *= c;
+          if (kTrain) lr *= c;
           if (j > it.lo) {
             // P V of the tile before adds to O no more. (Not waited for at every
             // tile: of this barrier's phases all but that one are complete,
             // since S of this tile is.)
-            ok = wait(&sm.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
+            ok = wait(&sm.pv_done[last.at], last.phase);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc_fence_after();
 #pragma unroll 1
@@ -627,39 +636,45 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
             const float p0 = ex2(a0), p1 = ex2(a1);
             pw[i] = Type<T>::pack(p0, p1);
             a[i & 1] = f2_add(a[i & 1], f2_pack(p0, p1));
-            b[i & 1] = f2_add(b[i & 1], Type<T>::unpack(pw[i]));
+            if (kTrain) b[i & 1] = f2_add(b[i & 1], Type<T>::unpack(pw[i]));
           }
           tmem_st_8cols(t_s + c * 8, pw);
         }
         float x0, x1;
         f2_unpack(f2_add(a[0], a[1]), x0, x1);
         l += x0 + x1;
-        f2_unpack(f2_add(b[0], b[1]), x0, x1);
-        lr += x0 + x1;
+        if (kTrain) {
+          f2_unpack(f2_add(b[0], b[1]), x0, x1);
+          lr += x0 + x1;
+        }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[t & 1]);
+        if (lane == 0) mbar_arrive(&sm.p_full[ss.at]);
+        last = ss;
+        ss.next();
+        vs.next();
         give_back();
       }
       if (!ok) break;
+      after = fwd_item(sh, item + gridDim.x, n_qt);  // while the last product runs
       // ---- output: O / l and lse
       const bool any = it.lo < it.hi;
       if (any) {
-        ok = wait(&sm.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
+        ok = wait(&sm.pv_done[last.at], last.phase);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
       }
       // no visible key: zeros (a NaN sum passes through). Rounded, P is not 0 where
       // l is not: the row's maximum is at least 2^0 of its reference.
       const bool none = l == 0.f;
-      const float inv_l = none ? 0.f : 1.f / lr;
+      const float inv_l = none ? 0.f : 1.f / (kTrain ? lr : l);
       const int64_t rows_all = (int64_t)sh.B * sh.Sq * sh.H;
       const int64_t orow = ((int64_t)it.b * sh.Sq + qi) * sh.H + it.h;
       const int64_t lrow = ((int64_t)it.b * sh.H + it.h) * sh.Sq + qi;
       if (any && sh.splits == 1) {
         uint8_t* block = sm.q[qs.at] + (warp & 3) * 4096;
-        if (out_res != nullptr) {  // the remainders first: the same memory
+        if (kTrain) {  // the remainders first: the same memory
 #pragma unroll 1
           for (int c = 0; c < kDP / 64; ++c)
             stage_rows<T, true>(t_o + c * 64, lane, !none, inv_l, block + c * kRows * 128);
@@ -685,7 +700,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         }
       } else {
         store_row<T>(t_o, sh.D, any, !none, qi < sh.Sq, inv_l, out + orow * sh.D,
-                     out_res != nullptr ? out_res + orow * sh.D : nullptr,
+                     kTrain ? out_res + orow * sh.D : nullptr,
                      sh.splits > 1 ? part_o + (it.split * rows_all + orow) * sh.D : nullptr);
       }
       if (any) {
@@ -696,7 +711,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       if (qi < sh.Sq) {
         if (sh.splits > 1)
           part_lse[it.split * rows_all + lrow] = none ? -INFINITY : m_ref + log2f(l);
-        else if (lse2)
+        else if (kTrain)
           lse2[lrow] = none ? INFINITY : m_ref + log2f(l);
       }
       tc_fence_before();
@@ -863,7 +878,8 @@ struct BwdItem {
 };
 template <bool kKeys>
 __device__ __forceinline__ BwdItem bwd_item(const Shape& s, int item, int n_rt) {
-  BwdItem it;
+  BwdItem it{};
+  if (item >= s.n_items) return it;  // asked for ahead of time
   const ItemAt at = item_at(s, item);
   it.split = at.split;
   // heaviest first under a causal mask: the last queries, the first keys
@@ -1157,25 +1173,29 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       }
       owed = nullptr;
     };
+    // row statistics (queries; negated) or the row's visibility (keys) of an item
+    auto row_of = [&](const BwdItem& x) {
+      float2 v = make_float2(-INFINITY, 0.f);
+      const int row = x.row0 + r;
+      if (!kKeys) {
+        if (x.lo < x.hi && row < sh.Sq)
+          v = __ldg(stats + ((int64_t)x.b * sh.H + x.head) * stat_pitch(sh.Sq) + row);
+      } else {
+        bool visible = row < sh.Sk;
+        if (visible && sh.words)
+          visible = (__ldg(sh.words + (int64_t)x.b * sh.nwords + row / 32) >> (row & 31)) & 1u;
+        v.y = visible ? 1.f : 0.f;
+      }
+      return v;
+    };
+    BwdItem after = bwd_item<kKeys>(sh, blockIdx.x, n_rt);
+    float2 after_row = row_of(after);
     for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-      const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
+      const BwdItem it = after;
       const int row = it.row0 + r;
       const bool any = it.lo < it.hi;
-      // row statistics (queries), or the row's visibility (keys)
-      uint64_t row_lse = f2_splat(-INFINITY), row_delta = f2_splat(0.f);  // negated
-      bool row_ok = true;
-      if (!kKeys) {
-        if (any && row < sh.Sq) {
-          const float2 v =
-              __ldg(stats + ((int64_t)it.b * sh.H + it.head) * stat_pitch(sh.Sq) + row);
-          row_lse = f2_splat(v.x);
-          row_delta = f2_splat(v.y);
-        }
-      } else {
-        row_ok = row < sh.Sk;
-        if (row_ok && sh.words)
-          row_ok = (__ldg(sh.words + (int64_t)it.b * sh.nwords + row / 32) >> (row & 31)) & 1u;
-      }
+      const uint64_t row_lse = f2_splat(after_row.x), row_delta = f2_splat(after_row.y);
+      const bool row_ok = !kKeys || after_row.y != 0.f;
       const bool rows_ok = __all_sync(0xffffffffu, row_ok);
       // the CTA's tiles alternate between the groups: mine is every second one
       int col0 = (kKeys ? it.first + (it.lo > 0 ? it.lo % it.n : 0) : it.lo) * kBN;
@@ -1267,6 +1287,9 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
         give_back();
       }
       if (!ok) break;
+      // the next item, and its row's load, while the last product runs
+      after = bwd_item<kKeys>(sh, item + gridDim.x, n_rt);
+      after_row = row_of(after);
       // ---- read the accumulators out
       if (any) {
         ok = wait(&sm.acc_full, n & 1);
@@ -1429,11 +1452,12 @@ cudaError_t cross_attn_opt_in(const void* kernel, size_t smem, std::atomic<uint6
 namespace {
 
 // `heads` of the rows that an item's index runs over.
-Shape shape_of(const CrossAttnArgs& a, int splits, int heads) {
+Shape shape_of(const CrossAttnArgs& a, int splits, int heads, int64_t items) {
   Shape s{};
   s.B = a.B; s.Sq = a.Sq; s.Sk = a.Sk; s.H = a.H; s.Hk = a.Hk; s.G = a.H / a.Hk; s.D = a.D;
   s.causal = a.causal;
   s.splits = splits;
+  s.n_items = (int)items;
   s.scale = a.scale;
   s.words = a.key_pad ? a.words : nullptr;
   s.vis_end = a.key_pad ? a.vis_end : nullptr;
@@ -1462,7 +1486,8 @@ int pieces(int64_t items, int64_t places, int64_t tiles) {
 int64_t row_tiles(int n) { return ((int64_t)n + kRows - 1) / kRows; }
 
 int fwd_splits(const CrossAttnArgs& a) {
-  return pieces(row_tiles(a.Sq) * a.H * a.B, 2ll * num_sms(), ((int64_t)a.Sk + kN - 1) / kN);
+  return pieces(row_tiles(a.Sq) * a.H * a.B, (int64_t)kFwdCtas * num_sms(),
+                ((int64_t)a.Sk + kN - 1) / kN);
 }
 int dq_splits(const CrossAttnArgs& a) {
   return pieces(row_tiles(a.Sq) * a.H * a.B, num_sms(), ((int64_t)a.Sk + kBN - 1) / kBN);
@@ -1472,7 +1497,7 @@ int dkv_splits(const CrossAttnArgs& a) {
                 ((int64_t)a.Sq + kBN - 1) / kBN * (a.H / a.Hk));
 }
 
-template <typename T, int kDP>
+template <typename T, int kDP, bool kTrain>
 cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   const int splits = fwd_splits(a);
   const int64_t rows = (int64_t)a.B * a.Sq * a.H;
@@ -1487,15 +1512,15 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
     return cudaErrorInvalidValue;
   static std::atomic<uint64_t> done{0};
   const int smem = (int)sizeof(FwdSmem<kDP>) + 1024;
-  auto kernel = cross_fwd_kernel<T, kDP>;
+  auto kernel = cross_fwd_kernel<T, kDP, kTrain>;
   cudaError_t e = cross_attn_opt_in((const void*)kernel, smem, done);
   if (e != cudaSuccess) return e;
   const int n_qt = (int)row_tiles(a.Sq);
   const int64_t items = (int64_t)n_qt * a.H * a.B * splits;
   if (items > 0x7fffffff - 4096) return cudaErrorInvalidValue;
-  const int grid = (int)std::min<int64_t>(items, 2ll * num_sms());
+  const int grid = (int)std::min<int64_t>(items, (int64_t)kFwdCtas * num_sms());
   e = launch_pdl(kernel, dim3(grid), dim3(kFwdThreads), smem, st, mq, mk, mv, mo,
-                 a.out_res ? mr : mo, shape_of(a, splits, a.H), (T*)a.out, (T*)a.out_res, a.lse2, a.partials, a.partials + splits * rows * a.D, (int)items, n_qt);
+                 a.out_res ? mr : mo, shape_of(a, splits, a.H, items), (T*)a.out, (T*)a.out_res, a.lse2, a.partials, a.partials + splits * rows * a.D, (int)items, n_qt);
   if (e != cudaSuccess) return e;
   note_launch();
   return splits > 1 ? launch_cross_attn_join(a, splits, st) : cudaGetLastError();
@@ -1536,7 +1561,7 @@ cudaError_t run_bwd_half(const CrossAttnArgs& a, cudaStream_t st) {
   o.part = a.partials;
   const int grid = (int)std::min<int64_t>(items, num_sms());
   e = launch_pdl(kernel, dim3(grid), dim3(BwdGeo<kDP, kKeys, kABufs>::kThreads), smem, st, kKeys ? mk : mq, kKeys ? mv : mo,
-                 kKeys ? mq : mk, kKeys ? mo : mv, m1, kKeys ? m2 : m1, shape_of(a, splits, heads), (const float2*)a.stats, o, (int)items, n_rt);
+                 kKeys ? mq : mk, kKeys ? mo : mv, m1, kKeys ? m2 : m1, shape_of(a, splits, heads, items), (const float2*)a.stats, o, (int)items, n_rt);
   if (e != cudaSuccess) return e;
   note_launch();
   if (splits > 1) {
@@ -1611,8 +1636,16 @@ cudaError_t launch_cross_attn_pack_mask(const CrossAttnArgs& a, cudaStream_t st)
 cudaError_t launch_cross_attn_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   if (bad_shape(a)) return cudaErrorInvalidValue;
   if (cross_attn_is_few(a)) return launch_cross_attn_few(a, st);
-  if (a.D <= 64) return a.half ? run_fwd<__half, 64>(a, st) : run_fwd<__nv_bfloat16, 64>(a, st);
-  return a.half ? run_fwd<__half, 128>(a, st) : run_fwd<__nv_bfloat16, 128>(a, st);
+  // a backward pass needs the lse and the remainders of O, both or neither
+  if ((a.lse2 != nullptr) != (a.out_res != nullptr)) return cudaErrorInvalidValue;
+  if (a.lse2 != nullptr) {
+    if (a.D <= 64)
+      return a.half ? run_fwd<__half, 64, true>(a, st) : run_fwd<__nv_bfloat16, 64, true>(a, st);
+    return a.half ? run_fwd<__half, 128, true>(a, st) : run_fwd<__nv_bfloat16, 128, true>(a, st);
+  }
+  if (a.D <= 64)
+    return a.half ? run_fwd<__half, 64, false>(a, st) : run_fwd<__nv_bfloat16, 64, false>(a, st);
+  return a.half ? run_fwd<__half, 128, false>(a, st) : run_fwd<__nv_bfloat16, 128, false>(a, st);
 }
 
 cudaError_t launch_cross_attn_bwd(const CrossAttnArgs& a, cudaStream_t st) {
