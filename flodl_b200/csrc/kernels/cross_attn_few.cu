@@ -55,7 +55,6 @@ struct FewSmem {
   static constexpr int kTile = kKeys * kDP * 2;
   static constexpr int kStages = kStageBytes / (2 * kTile);
   uint8_t k[kStages][kTile], v[kStages][kTile];  // the warps' outputs once all are read
-  uint8_t q[16 * kDP * 2];
   float m[kWarps][16], l[kWarps][16];
   uint64_t full[kStages], empty[kStages];
   uint32_t abort;
@@ -181,15 +180,6 @@ __global__ void __launch_bounds__(kThreads, 3)
   if (warp == kWarps && lane == 0)
     for (int i = 0; i < ahead; ++i) load(i);
 
-  // queries, rows (head, position) of the group; rows past the end are zero
-  for (int i = threadIdx.x; i < 16 * kDP / 8; i += kThreads) {
-    const int r = i / (kDP / 8), c = i - r * (kDP / 8);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < p.rows && c * 8 < p.D)
-      v = *reinterpret_cast<const uint4*>((const T*)p.q + b * p.qb + (int64_t)(r % p.Sq) * p.qs +
-                                          (int64_t)(kh * p.G + r / p.Sq) * p.qh + c * 8);
-    *reinterpret_cast<uint4*>(sm.q + chunk_at<16>(r, c)) = v;
-  }
   // visible keys, a bit each (keys past Sk count as hidden), and their end
   int n_load = t1 - t0;
   if (p.key_pad) {
@@ -205,8 +195,6 @@ __global__ void __launch_bounds__(kThreads, 3)
     if (lane == 0 && end) atomicMax(&sm.vis_end, end);
     __syncthreads();
     n_load = std::max(ahead, (sm.vis_end + 1) / 2);
-  } else {
-    __syncthreads();
   }
 
   float o[kDP / 8][4];
@@ -239,11 +227,23 @@ __global__ void __launch_bounds__(kThreads, 3)
     __syncwarp();
   } else {
     // ------------------------------------------------------------ consumers
+    // the queries as A fragments, rows (head, position) of the group; rows past the
+    // end are zero
     uint32_t qa[kSteps][4];
+    int row_q[2];
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-      ldsm4(qa[s], smem_u32(sm.q) + chunk_at<16>((lane & 7) + ((lane >> 3) & 1) * 8, 2 * s + (lane >> 4)));
-    const int row_q[2] = {g % p.Sq, (g + 8) % p.Sq};
+    for (int r2 = 0; r2 < 2; ++r2) {
+      const int r = g + 8 * r2, h = r / p.Sq;
+      row_q[r2] = r - h * p.Sq;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(
+          (const T*)p.q + b * p.qb + (int64_t)row_q[r2] * p.qs + (int64_t)(kh * p.G + h) * p.qh);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          qa[s][r2 + 2 * half] =
+              r < p.rows && 16 * s + 8 * half < p.D ? __ldg(src + 8 * s + 4 * half + t) : 0u;
+    }
     const int key0 = warp * 16;  // this warp's keys in a tile
     for (int i = 0; i < n_load; ++i) {
       const int st = i % kStages;
@@ -397,53 +397,81 @@ __global__ void __launch_bounds__(kThreads, 3)
 }
 
 // Joins the pieces of `splits` key ranges: a warp per query row, four columns
-// per lane (D <= 128), pieces in order. Weight of a piece: 2^(lse - max lse).
-template <typename T>
+// per lane, kLanes lanes for the row (16 for D <= 64: the warp's halves take every
+// other piece). Weight of a piece: 2^(lse - max lse); pieces in a fixed order.
+// Bound by latency: eight pieces' values and weights are in flight at once.
+template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part_o,
                                                    const float* __restrict__ part_lse,
                                                    T* __restrict__ out, T* __restrict__ out_res,
-                                                   float* __restrict__ lse2,
-                                                   int splits, int B, int Sq, int H, int D) {
+                                                   float* __restrict__ lse2, int splits,
+                                                   uint32_t rows, uint32_t Sq, uint32_t H, int D) {
+  constexpr int kHalves = 32 / kLanes, kAhead = 8;
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = (int64_t)B * Sq * H;
-  const int64_t nw = (int64_t)gridDim.x * 8;
-  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += nw) {
-    const int64_t bi = row / H;  // b * Sq + i
-    const int h = (int)(row - bi * H);
-    const int64_t b = bi / Sq;
-    const int64_t lrow = (b * H + h) * Sq + (bi - b * Sq);
-    float mm = -INFINITY;
-    for (int s = lane; s < splits; s += 32) mm = fmaxf(mm, part_lse[s * rows + lrow]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
-    const float base = mm == -INFINITY ? 0.f : mm;
-    float w = 0.f;
+  const int lane = threadIdx.x & 31, half = lane / kLanes, col = lane % kLanes * 4;
+  const bool mine = col < D;
+  for (uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8) {
+    const uint32_t bi = row / H, b = bi / Sq;  // bi = b * Sq + i
+    const uint32_t lrow = (b * H + (row - bi * H)) * Sq + (bi - b * Sq);
+    float mm = -INFINITY, w = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    const bool mine = lane * 4 < D;
-#pragma unroll 8
-    for (int s = 0; s < splits; ++s) {
-      const float f = ex2(part_lse[s * rows + lrow] - base);
-      w += f;
-      if (mine) {
-        const float4 v = *reinterpret_cast<const float4*>(part_o + (s * rows + row) * D + lane * 4);
-        a.x = fmaf(v.x, f, a.x);
-        a.y = fmaf(v.y, f, a.y);
-        a.z = fmaf(v.z, f, a.z);
-        a.w = fmaf(v.w, f, a.w);
+    auto scale = [&](float f) {
+      w *= f;
+      a.x *= f;
+      a.y *= f;
+      a.z *= f;
+      a.w *= f;
+    };
+    auto add = [&](const float4& v, float vw, float f) {
+      w = fmaf(vw, f, w);
+      a.x = fmaf(v.x, f, a.x);
+      a.y = fmaf(v.y, f, a.y);
+      a.z = fmaf(v.z, f, a.z);
+      a.w = fmaf(v.w, f, a.w);
+    };
+    for (int s0 = half; s0 < splits; s0 += kAhead * kHalves) {
+      float ls[kAhead];
+      float4 v[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int s = s0 + i * kHalves;
+        ls[i] = s < splits ? part_lse[(int64_t)s * rows + lrow] : -INFINITY;
+        v[i] = s < splits && mine
+                   ? *reinterpret_cast<const float4*>(part_o + ((int64_t)s * rows + row) * D + col)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
       }
+      float top = mm;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) top = fmaxf(top, ls[i]);
+      const float base = top == -INFINITY ? 0.f : top;
+      scale(ex2(mm - base));
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) add(v[i], 1.f, ex2(ls[i] - base));
+      mm = top;
+    }
+    if (kHalves == 2) {
+      const float om = __shfl_xor_sync(0xffffffffu, mm, 16), ow = __shfl_xor_sync(0xffffffffu, w, 16);
+      const float4 oa = make_float4(
+          __shfl_xor_sync(0xffffffffu, a.x, 16), __shfl_xor_sync(0xffffffffu, a.y, 16),
+          __shfl_xor_sync(0xffffffffu, a.z, 16), __shfl_xor_sync(0xffffffffu, a.w, 16));
+      const float top = fmaxf(mm, om), base = top == -INFINITY ? 0.f : top;
+      scale(ex2(mm - base));
+      add(oa, ow, ex2(om - base));
+      mm = top;
     }
     const bool none = w == 0.f;
     const float inv = none ? 0.f : 1.f / w;
+    if (half != 0) continue;
     if (mine) {
-      const uint2 w = make_uint2(pack<T>(a.x * inv, a.y * inv), pack<T>(a.z * inv, a.w * inv));
-      *reinterpret_cast<uint2*>(out + row * D + lane * 4) = w;
+      const int64_t at = (int64_t)row * D + col;
+      const uint2 o = make_uint2(pack<T>(a.x * inv, a.y * inv), pack<T>(a.z * inv, a.w * inv));
+      *reinterpret_cast<uint2*>(out + at) = o;
       if (out_res)
-        *reinterpret_cast<uint2*>(out_res + row * D + lane * 4) =
-            make_uint2(remainder2<T>(w.x, a.x * inv, a.y * inv), remainder2<T>(w.y, a.z * inv, a.w * inv));
+        *reinterpret_cast<uint2*>(out_res + at) =
+            make_uint2(remainder2<T>(o.x, a.x * inv, a.y * inv), remainder2<T>(o.y, a.z * inv, a.w * inv));
     }
-    if (lane == 0 && lse2) lse2[lrow] = none ? INFINITY : base + log2f(w);
+    if (lane == 0 && lse2) lse2[lrow] = none ? INFINITY : mm + log2f(w);
   }
 }
 
@@ -511,14 +539,20 @@ cudaError_t launch_cross_attn_few(const CrossAttnArgs& a, cudaStream_t st) {
 
 cudaError_t launch_cross_attn_join(const CrossAttnArgs& a, int splits, cudaStream_t st) {
   const int64_t rows = (int64_t)a.B * a.Sq * a.H;
+  if (rows > 0x7fffffff) return cudaErrorInvalidValue;
   const float* po = a.partials;
   const float* pl = a.partials + (int64_t)splits * rows * a.D;
   const int grid = (int)std::min<int64_t>((rows + 7) / 8, (int64_t)num_sms() * 8);
-  cudaError_t e =
-      a.half ? launch_pdl(join_kernel<__half>, dim3(grid), dim3(256), 0, st, po, pl, (__half*)a.out,
-                          (__half*)a.out_res, a.lse2, splits, a.B, a.Sq, a.H, a.D)
-             : launch_pdl(join_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, st, po, pl,
-                          (__nv_bfloat16*)a.out, (__nv_bfloat16*)a.out_res, a.lse2, splits, a.B, a.Sq, a.H, a.D);
+  auto launch = [&](auto t, auto kernel) {
+    using T = decltype(t);
+    return launch_pdl(kernel, dim3(grid), dim3(256), 0, st, po, pl, (T*)a.out, (T*)a.out_res, a.lse2,
+                      splits, (uint32_t)rows, (uint32_t)a.Sq, (uint32_t)a.H, a.D);
+  };
+  const bool wide = a.D > 64;
+  const cudaError_t e =
+      a.half ? launch(__half(), wide ? join_kernel<__half, 32> : join_kernel<__half, 16>)
+             : launch(__nv_bfloat16(),
+                      wide ? join_kernel<__nv_bfloat16, 32> : join_kernel<__nv_bfloat16, 16>);
   if (e != cudaSuccess) return e;
   note_launch();
   return cudaGetLastError();
