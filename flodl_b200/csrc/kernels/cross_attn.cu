@@ -37,6 +37,7 @@
 // All waits are bounded (see sm100_ptx.cuh).
 #include "sm100_ptx.cuh"
 #include "cross_attn.h"
+#include "cross_attn_join.cuh"
 
 #include <cuda_fp16.h>
 
@@ -112,8 +113,10 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
 constexpr uint32_t desc_hi(uint32_t sbo) {
   return ((sbo >> 4) & 0x3FFFu) | (1u << 14) | (2u << 29);  // version, 128-byte swizzle
 }
+// (In a cluster the bits above a CTA's own 256 KB of shared addresses hold its
+// rank; they would run into the stride's field.)
 __device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) {
-  return (addr >> 4) | ((lbo >> 4) << 16);
+  return ((addr & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16);
 }
 __device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id,
                                         uint32_t acc) {
@@ -402,6 +405,10 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const Waiter wait{&sm.abort, sh.err};
+  // a cluster's piece takes the memory of the keys and values once all are read
+  float* s_piece = reinterpret_cast<float*>(sm.k);
+  float* s_lse = reinterpret_cast<float*>(sm.q);
+  static_assert(sizeof(sm.k) + sizeof(sm.v) >= kRows * kDP * 4, "a piece in the stages");
 
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < kQBufs; ++i) {
@@ -698,6 +705,17 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
             tma_store_4d(&tm_o, block + c * kRows * 128, c * 64, qi - lane, it.h, it.b);
           bulk_commit_group();
         }
+      } else if (sh.splits > 1 && part_o == nullptr) {  // a cluster's piece
+#pragma unroll 1
+        for (int c = 0; c < kDP; c += 16) {
+          float v[16];
+          row16(t_o + c, any, !none, inv_l, v);
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(s_piece + piece_at<kDP>(r, (c + i) / 4)) =
+                make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+        s_lse[r] = none ? -INFINITY : m_ref + log2f(l);
       } else {
         store_row<T>(t_o, sh.D, any, !none, qi < sh.Sq, inv_l, out + orow * sh.D,
                      kTrain ? out_res + orow * sh.D : nullptr,
@@ -709,7 +727,9 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
         qs.next();
       }
       if (qi < sh.Sq) {
-        if (sh.splits > 1)
+        if (sh.splits > 1 && part_o == nullptr)
+          ;  // joined below
+        else if (sh.splits > 1)
           part_lse[it.split * rows_all + lrow] = none ? -INFINITY : m_ref + log2f(l);
         else if (kTrain)
           lse2[lrow] = none ? INFINITY : m_ref + log2f(l);
@@ -723,6 +743,27 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<256>(tmem);
+  }
+  if (sh.splits > 1 && part_o == nullptr) {  // one item per CTA
+    const FwdItem it = fwd_item(sh, blockIdx.x, n_qt);
+    const int q0 = it.qt * kRows;
+    cluster_join<kDP>(
+        s_piece, s_lse, min(kRows, sh.Sq - q0), sh.D, sh.splits,
+        [&](int r, int c, float4 v) {
+          const int64_t at = (((int64_t)it.b * sh.Sq + q0 + r) * sh.H + it.h) * sh.D + 4 * c;
+          const uint2 w = make_uint2(Type<T>::pack(v.x, v.y), Type<T>::pack(v.z, v.w));
+          *reinterpret_cast<uint2*>(out + at) = w;
+          if (kTrain) {
+            float4 f;
+            f2_unpack(Type<T>::unpack(w.x), f.x, f.y);
+            f2_unpack(Type<T>::unpack(w.y), f.z, f.w);
+            *reinterpret_cast<uint2*>(out_res + at) =
+                make_uint2(Type<T>::pack(v.x - f.x, v.y - f.y), Type<T>::pack(v.z - f.z, v.w - f.w));
+          }
+        },
+        [&](int r, float lse) {
+          if (kTrain) lse2[((int64_t)it.b * sh.H + it.h) * sh.Sq + q0 + r] = lse;
+        });
   }
 }
 
@@ -1449,6 +1490,33 @@ cudaError_t cross_attn_opt_in(const void* kernel, size_t smem, std::atomic<uint6
   return e;
 }
 
+int64_t cross_attn_clusters(const void* kernel, int threads, size_t smem, int size,
+                            CrossFits& fits) {
+  if (size < 2) return INT64_MAX;
+  int n = fits[size].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                         cudaSharedmemCarveoutMaxShared);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = -1;  // none
+    }
+    fits[size].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 namespace {
 
 // `heads` of the rows that an item's index runs over.
@@ -1485,9 +1553,25 @@ int pieces(int64_t items, int64_t places, int64_t tiles) {
 }
 int64_t row_tiles(int n) { return ((int64_t)n + kRows - 1) / kRows; }
 
-int fwd_splits(const CrossAttnArgs& a) {
-  return pieces(row_tiles(a.Sq) * a.H * a.B, (int64_t)kFwdCtas * num_sms(),
-                ((int64_t)a.Sk + kN - 1) / kN);
+// Clusters of the forward kernel that the GPU holds. The runtime counts one CTA per
+// SM (it rounds six warps up to eight); two fit, so twice as many clusters.
+template <int kDP>
+int64_t fwd_clusters(int size) {
+  static CrossFits fits{};
+  if (size < 2) return INT64_MAX;
+  return kFwdCtas * cross_attn_clusters((const void*)cross_fwd_kernel<__nv_bfloat16, kDP, false>,
+                                        kFwdThreads, sizeof(FwdSmem<kDP>) + 1024, size, fits);
+}
+CrossSplits fwd_splits(const CrossAttnArgs& a) {
+  const int64_t items = row_tiles(a.Sq) * a.H * a.B;
+  const int64_t tiles = ((int64_t)a.Sk + kN - 1) / kN;
+  const int want = pieces(items, (int64_t)kFwdCtas * num_sms(), tiles);
+  // as many as a cluster joins and the GPU holds at once (98 items of 128 x 1500 x 64:
+  // 21 us with two pieces each, 27 with three and a second kernel)
+  int s = std::min(want, kCrossCluster);
+  while (s > 1 && items > (a.D > 64 ? fwd_clusters<128>(s) : fwd_clusters<64>(s))) --s;
+  if (cross_attn_joins_more(items, s, want, tiles, num_sms())) return {want, false};
+  return {s, s > 1};
 }
 int dq_splits(const CrossAttnArgs& a) {
   return pieces(row_tiles(a.Sq) * a.H * a.B, num_sms(), ((int64_t)a.Sk + kBN - 1) / kBN);
@@ -1499,9 +1583,11 @@ int dkv_splits(const CrossAttnArgs& a) {
 
 template <typename T, int kDP, bool kTrain>
 cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
-  const int splits = fwd_splits(a);
+  const CrossSplits plan = fwd_splits(a);
+  const int splits = plan.n;
   const int64_t rows = (int64_t)a.B * a.Sq * a.H;
-  if (splits > 1 && !a.partials) return cudaErrorInvalidValue;
+  const bool joined = plan.joined();
+  if (joined && !a.partials) return cudaErrorInvalidValue;
   CUtensorMap mq, mk, mv, mo, mr;
   const int64_t o_st[3] = {(int64_t)a.Sq * a.H * a.D, (int64_t)a.H * a.D, a.D};
   if (!cross_attn_map(&mq, a.q, a.half, a.D, a.Sq, a.H, a.B, a.q_st, kRows) ||
@@ -1519,11 +1605,14 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   const int64_t items = (int64_t)n_qt * a.H * a.B * splits;
   if (items > 0x7fffffff - 4096) return cudaErrorInvalidValue;
   const int grid = (int)std::min<int64_t>(items, (int64_t)kFwdCtas * num_sms());
-  e = launch_pdl(kernel, dim3(grid), dim3(kFwdThreads), smem, st, mq, mk, mv, mo,
-                 a.out_res ? mr : mo, shape_of(a, splits, a.H, items), (T*)a.out, (T*)a.out_res, a.lse2, a.partials, a.partials + splits * rows * a.D, (int)items, n_qt);
+  // (several pieces: one item per CTA, as many items as places at most)
+  e = launch_pdl_cluster(kernel, dim3(grid), dim3(kFwdThreads), plan.clustered ? splits : 1, smem, st, mq,
+                         mk, mv, mo, a.out_res ? mr : mo, shape_of(a, splits, a.H, items), (T*)a.out,
+                         (T*)a.out_res, a.lse2, joined ? a.partials : nullptr,
+                         joined ? a.partials + splits * rows * a.D : nullptr, (int)items, n_qt);
   if (e != cudaSuccess) return e;
   note_launch();
-  return splits > 1 ? launch_cross_attn_join(a, splits, st) : cudaGetLastError();
+  return joined ? launch_cross_attn_join(a, splits, st) : cudaGetLastError();
 }
 
 template <typename T, int kDP, bool kKeys, int kABufs>
@@ -1613,8 +1702,8 @@ int64_t cross_attn_stats_floats(const CrossAttnArgs& a) {
   return 2ll * a.B * a.H * stat_pitch(a.Sq);
 }
 int64_t cross_attn_fwd_partials(const CrossAttnArgs& a) {
-  const int splits = cross_attn_is_few(a) ? cross_attn_few_splits(a) : fwd_splits(a);
-  return splits > 1 ? (int64_t)splits * a.B * a.Sq * a.H * (a.D + 1) : 0;
+  const CrossSplits s = cross_attn_is_few(a) ? cross_attn_few_splits(a) : fwd_splits(a);
+  return s.joined() ? (int64_t)s.n * a.B * a.Sq * a.H * (a.D + 1) : 0;
 }
 // The two halves run one after the other and use the same scratch.
 int64_t cross_attn_bwd_partials(const CrossAttnArgs& a) {

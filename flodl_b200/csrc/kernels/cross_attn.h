@@ -41,6 +41,8 @@ struct CrossAttnArgs {
 
 constexpr int kCrossFewRows = 16;  // query rows per memory head of the few-row form
 
+constexpr int kCrossCluster = 8;   // pieces of a split key axis that a cluster joins
+
 // Whether the forward takes the few-row form: all query rows of a memory head
 // (Sq * H / Hk) fit one 16-row tensor-core tile.
 bool cross_attn_is_few(const CrossAttnArgs& a);
@@ -60,7 +62,26 @@ bool cross_attn_map(CUtensorMap* m, const void* base, bool half, int D, int S, i
                     const int64_t (&st)[3], int rows);
 // Shared-memory opt-in of a kernel, once per device.
 cudaError_t cross_attn_opt_in(const void* kernel, size_t smem, std::atomic<uint64_t>& done);
-int cross_attn_few_splits(const CrossAttnArgs& a);
+// Pieces of the key axis, and whether a cluster joins them (else a second kernel).
+struct CrossSplits {
+  int n;
+  bool clustered;
+  bool joined() const { return n > 1 && !clustered; }
+};
+CrossSplits cross_attn_few_splits(const CrossAttnArgs& a);
+// Whether `want` pieces of a key axis of `tiles`, joined by a second kernel, beat the s
+// that a cluster joins. That kernel costs 3 to 4 us, a tile about 0.5 (64 keys, a CTA
+// to itself): where the s leave SMs idle and more than five tiles a piece go. (16 heads
+// x 128 rows x 64 columns each way, pieces 8 and 15 to 18: 13.6 us joined by
+// clusters and 14.3 by a kernel at 4001 keys, 42 and 29 at 20000.)
+inline bool cross_attn_joins_more(int64_t items, int64_t s, int64_t want, int64_t tiles, int sms) {
+  return want > kCrossCluster && items * s < sms && tiles / s - tiles / want > 5;
+}
+// Clusters of `size` CTAs of a kernel that the GPU holds at once (`fits`: a cache of
+// the kernel's own; a cluster's CTAs share a part of the GPU, so that fewer CTAs fit
+// in clusters than alone).
+using CrossFits = std::atomic<int>[kCrossCluster + 1];
+int64_t cross_attn_clusters(const void* kernel, int threads, size_t smem, int size, CrossFits& fits);
 cudaError_t launch_cross_attn_few(const CrossAttnArgs& a, cudaStream_t st);
 // out = the partial results of `splits` key ranges joined by their lse.
 cudaError_t launch_cross_attn_join(const CrossAttnArgs& a, int splits, cudaStream_t st);

@@ -20,6 +20,7 @@
 // joined by their lse in a second kernel, in a fixed order.
 #include "sm100_ptx.cuh"
 #include "cross_attn.h"
+#include "cross_attn_join.cuh"
 
 #include <cuda_fp16.h>
 
@@ -56,6 +57,7 @@ struct FewSmem {
   static constexpr int kStages = kStageBytes / (2 * kTile);
   uint8_t k[kStages][kTile], v[kStages][kTile];  // the warps' outputs once all are read
   float m[kWarps][16], l[kWarps][16];
+  float lse[16];  // of this CTA's piece
   uint64_t full[kStages], empty[kStages];
   uint32_t abort;
   int vis_end;  // of this CTA's words
@@ -339,6 +341,8 @@ __global__ void __launch_bounds__(kThreads, 3)
 
   // join the warps: o[n][2 r2 + j] is row g + 8 r2, column 8 n + 2 t + j
   float* s_o = reinterpret_cast<float*>(sm.k);
+  float* s_piece = s_o + kWarps * 16 * kDP;
+  static_assert((kWarps + 1) * 16 * kDP * 4 <= kStageBytes, "outputs in the stages");
   if (warp < kWarps) {
 #pragma unroll
     for (int r2 = 0; r2 < 2; ++r2) {
@@ -358,6 +362,13 @@ __global__ void __launch_bounds__(kThreads, 3)
     }
   }
   __syncthreads();
+  const int64_t rows_all = (int64_t)p.B * p.Sq * p.H;
+  auto orow_of = [&](int r) {
+    return ((int64_t)b * p.Sq + r % p.Sq) * p.H + kh * p.G + r / p.Sq;
+  };
+  auto lrow_of = [&](int r) {
+    return ((int64_t)b * p.H + kh * p.G + r / p.Sq) * p.Sq + r % p.Sq;
+  };
   const int pairs = p.D / 2;
   for (int i = threadIdx.x; i < p.rows * pairs; i += kThreads) {
     const int r = i / pairs, d = 2 * (i - r * pairs);
@@ -377,23 +388,38 @@ __global__ void __launch_bounds__(kThreads, 3)
     // no visible key: zeros. A NaN sum (NaN scores) passes through.
     const bool none = ll == 0.f;
     const float inv = none ? 0.f : 1.f / ll;
-    const int h = kh * p.G + r / p.Sq, iq = r % p.Sq;
-    const int64_t orow = ((int64_t)b * p.Sq + iq) * p.H + h;
-    const int64_t lrow = ((int64_t)b * p.H + h) * p.Sq + iq;
+    const int64_t orow = orow_of(r);
     if (p.splits == 1) {
       const uint32_t w = pack<T>(a0 * inv, a1 * inv);
       *reinterpret_cast<uint32_t*>((T*)p.out + orow * p.D + d) = w;
       if (p.out_res)
         *reinterpret_cast<uint32_t*>((T*)p.out_res + orow * p.D + d) =
             remainder2<T>(w, a0 * inv, a1 * inv);
-      if (d == 0 && p.lse2) p.lse2[lrow] = none ? INFINITY : top + log2f(ll);
+      if (d == 0 && p.lse2) p.lse2[lrow_of(r)] = none ? INFINITY : top + log2f(ll);
+    } else if (p.part_o == nullptr) {  // a cluster's piece, behind the warps' outputs
+      *reinterpret_cast<float2*>(s_piece + piece_at<kDP>(r, d / 4) + d % 4) =
+          make_float2(a0 * inv, a1 * inv);
+      if (d == 0) sm.lse[r] = none ? -INFINITY : top + log2f(ll);
     } else {
-      const int64_t rows_all = (int64_t)p.B * p.Sq * p.H;
       *reinterpret_cast<float2*>(p.part_o + (split * rows_all + orow) * p.D + d) =
           make_float2(a0 * inv, a1 * inv);
-      if (d == 0) p.part_lse[split * rows_all + lrow] = none ? -INFINITY : top + log2f(ll);
+      if (d == 0) p.part_lse[split * rows_all + lrow_of(r)] = none ? -INFINITY : top + log2f(ll);
     }
   }
+  if (p.splits > 1 && p.part_o == nullptr)
+    cluster_join<kDP>(
+        s_piece, sm.lse, p.rows, p.D, p.splits,
+        [&](int r, int c, float4 v) {
+          const int64_t at = orow_of(r) * p.D + 4 * c;
+          const uint2 w = make_uint2(pack<T>(v.x, v.y), pack<T>(v.z, v.w));
+          *reinterpret_cast<uint2*>((T*)p.out + at) = w;
+          if (p.out_res)
+            *reinterpret_cast<uint2*>((T*)p.out_res + at) =
+                make_uint2(remainder2<T>(w.x, v.x, v.y), remainder2<T>(w.y, v.z, v.w));
+        },
+        [&](int r, float lse) {
+          if (p.lse2) p.lse2[lrow_of(r)] = lse;
+        });
 }
 
 // Joins the pieces of `splits` key ranges: a warp per query row, four columns
@@ -489,11 +515,19 @@ cudaError_t run_few(const CrossAttnArgs& a, const FewParams& p, cudaStream_t st)
   constexpr size_t base = sizeof(FewSmem<kDP>) + 1024;
   cudaError_t e = cross_attn_opt_in((const void*)few_kernel<T, kDP>, base + 4 * kMaxWords, done);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(few_kernel<T, kDP>, dim3((unsigned)ctas), dim3(kThreads), base + 4 * words, st, mk,
-                 mv, p);
+  e = launch_pdl_cluster(few_kernel<T, kDP>, dim3((unsigned)ctas), dim3(kThreads),
+                         p.splits > 1 && p.part_o == nullptr ? p.splits : 1, base + 4 * words, st, mk,
+                         mv, p);
   if (e != cudaSuccess) return e;
   note_launch();
   return cudaSuccess;
+}
+
+template <int kDP>
+int64_t few_clusters(int size) {
+  static CrossFits fits{};
+  return cross_attn_clusters((const void*)few_kernel<__nv_bfloat16, kDP>, kThreads,
+                             sizeof(FewSmem<kDP>) + 1024 + 4 * kMaxWords, size, fits);
 }
 
 }  // namespace
@@ -505,12 +539,20 @@ bool cross_attn_is_few(const CrossAttnArgs& a) {
 // Key ranges per memory head: as many CTAs as fit the SMs at once (three each),
 // with four tiles or more in a range (a shorter one costs more in its join than
 // it saves), and no more mask words than a CTA's shared memory holds.
-int cross_attn_few_splits(const CrossAttnArgs& a) {
+CrossSplits cross_attn_few_splits(const CrossAttnArgs& a) {
   const int64_t units = (int64_t)a.B * a.Hk;
   const int64_t tiles = ((int64_t)a.Sk + kKeys - 1) / kKeys;
   const int64_t want = std::min(3ll * num_sms() / units, (long long)(tiles / 4));
   const int64_t need = (2 * tiles + kMaxWords - 1) / kMaxWords;
-  return (int)std::max<int64_t>({1, a.key_pad ? need : 1, want});
+  const int64_t least = a.key_pad ? std::max<int64_t>(1, need) : 1;
+  // as many as a cluster joins and the GPU holds at once (63 heads x 8192 x 64: 24 us
+  // with five or six pieces each, 34 with seven that wait for one another, 28 joined
+  // by a second kernel)
+  int64_t s = std::min<int64_t>(want, kCrossCluster);
+  while (s > 1 && units > (a.D > 64 ? few_clusters<128>((int)s) : few_clusters<64>((int)s))) --s;
+  if (s < least || cross_attn_joins_more(units, s, want, tiles, num_sms()))
+    return {(int)std::max<int64_t>(least, want), false};
+  return {(int)std::max<int64_t>(1, s), s > 1};
 }
 
 cudaError_t launch_cross_attn_few(const CrossAttnArgs& a, cudaStream_t st) {
@@ -520,11 +562,12 @@ cudaError_t launch_cross_attn_few(const CrossAttnArgs& a, cudaStream_t st) {
   p.B = a.B; p.Sq = a.Sq; p.Sk = a.Sk; p.H = a.H; p.Hk = a.Hk; p.D = a.D;
   p.G = a.H / a.Hk;
   p.rows = p.G * a.Sq;
-  p.splits = cross_attn_few_splits(a);
+  const CrossSplits splits = cross_attn_few_splits(a);
+  p.splits = splits.n;
   p.causal = a.causal;
   p.sl2 = a.scale * kLog2e;
   p.err = default_err_word();
-  if (p.splits > 1) {
+  if (splits.joined()) {
     if (!a.partials) return cudaErrorInvalidValue;
     p.part_o = a.partials;
     p.part_lse = a.partials + (int64_t)p.splits * a.B * a.Sq * a.H * a.D;
@@ -534,7 +577,7 @@ cudaError_t launch_cross_attn_few(const CrossAttnArgs& a, cudaStream_t st) {
       a.half ? (wide ? run_few<__half, 128>(a, p, st) : run_few<__half, 64>(a, p, st))
              : (wide ? run_few<__nv_bfloat16, 128>(a, p, st) : run_few<__nv_bfloat16, 64>(a, p, st));
   if (e != cudaSuccess) return e;
-  return p.splits > 1 ? launch_cross_attn_join(a, p.splits, st) : cudaGetLastError();
+  return splits.joined() ? launch_cross_attn_join(a, p.splits, st) : cudaGetLastError();
 }
 
 cudaError_t launch_cross_attn_join(const CrossAttnArgs& a, int splits, cudaStream_t st) {

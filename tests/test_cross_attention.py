@@ -239,6 +239,20 @@ def test_gpu_tiles(shape, dtype):
     check("cuda", dtype, *shape)
 
 
+SPLIT = [  # long key axes of few heads: 2 to 8 pieces, and more than that
+    (1, 128, 1, 1, 512, 128), (1, 128, 1, 1, 2048, 128), (1, 140, 1, 1, 2100, 64),
+    (2, 1, 1, 1, 2500, 64), (5, 3, 2, 1, 1300, 128), (1, 40, 2, 1, 9000, 72),
+    (1, 100, 1, 1, 16000, 64), (1, 2, 4, 2, 16000, 128),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mask", [None, "scattered", "empty", "one"])
+@pytest.mark.parametrize("shape", SPLIT)
+def test_gpu_split_keys(shape, mask):
+    check("cuda", torch.bfloat16, *shape, mask=mask)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("mask", ["right", "left", "scattered", "empty", "one"])
