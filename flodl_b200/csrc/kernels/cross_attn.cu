@@ -1331,6 +1331,10 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       // the next item, and its row's load, while the last product runs
       after = bwd_item<kKeys>(sh, item + gridDim.x, n_rt);
       after_row = row_of(after);
+      // A group without a tile in this item gives the buffer back here, before it waits
+      // for the products: of items of one tile each, these may come behind scores
+      // that need the buffer.
+      give_back();
       // ---- read the accumulators out
       if (any) {
         ok = wait(&sm.acc_full, n & 1);
@@ -1338,7 +1342,6 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
         tc_fence_after();
         ++n;
       }
-      give_back();
       // keys: group 0 takes dV, group 1 dK; queries: 64 of dQ's columns each (one
       // group at head size 64)
       const bool second = kKeys && group == 0;

@@ -239,6 +239,16 @@ def test_gpu_tiles(shape, dtype):
     check("cuda", dtype, *shape)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 72, 128])
+def test_gpu_many_items_of_one_tile(D):
+    # several items per CTA in every kernel, each with a single streamed tile
+    check("cuda", torch.bfloat16, 40, 17, 8, 8, 130, D)
+    check("cuda", torch.bfloat16, 40, 130, 8, 8, 17, D, mask="right")
+    check("cuda", torch.bfloat16, 50, 150, 8, 8, 150, D, causal=True)
+    check("cuda", torch.bfloat16, 100, 40, 8, 4, 50, D, mask="empty")
+
+
 SPLIT = [  # long key axes of few heads: 2 to 8 pieces, and more than that
     (1, 128, 1, 1, 512, 128), (1, 128, 1, 1, 2048, 128), (1, 140, 1, 1, 2100, 64),
     (2, 1, 1, 1, 2500, 64), (5, 3, 2, 1, 1300, 128), (1, 40, 2, 1, 9000, 72),
