@@ -224,6 +224,22 @@ __device__ __forceinline__ void stage_rows(uint32_t t, int lane, bool use, float
           pack8<T, kRes>(v + 8 * h);
   }
 }
+// Values to `block` and their remainders to `res`, 64 columns.
+template <typename T>
+__device__ __forceinline__ void stage_pair(uint32_t t, int lane, bool use, float f, uint8_t* block,
+                                           uint8_t* res) {
+#pragma unroll 2
+  for (int c = 0; c < 4; ++c) {
+    float v[16];
+    row16(t + c * 16, true, use, f, v);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = lane * 128 + (((2 * c + h) ^ (lane & 7)) << 4);
+      *reinterpret_cast<uint4*>(block + at) = pack8<T, false>(v + 8 * h);
+      *reinterpret_cast<uint4*>(res + at) = pack8<T, true>(v + 8 * h);
+    }
+  }
+}
 // The plain form: a row's columns below D as 16-bit values to out (and their
 // remainders to res), or as f32 to part (pieces of a split axis; rows without a
 // visible tile).
@@ -332,20 +348,22 @@ __device__ __forceinline__ void settle(uint64_t* bar, uint32_t issued) {
 // us on 8 x 16 heads, 1024 x 1024.)
 constexpr int kN = 64;
 constexpr int kFwdThreads = 192;
-template <int kDP>
+template <int kDP, bool kTrain>
 struct FwdGeo {
   static constexpr int kQBufs = kDP == 64 ? 2 : 1;
-  static constexpr int kStages = kDP == 64 ? 4 : 2;
+  static constexpr bool kResBuf = kTrain && kDP == 64;  // the remainders have a buffer
+  static constexpr int kStages = kDP == 64 ? (kResBuf ? 3 : 4) : 2;
 };
 constexpr int kFwdCtas = 2;       // per SM
 constexpr uint32_t kTmemO = 128;
 
-template <int kDP>
+template <int kDP, bool kTrain>
 struct FwdSmem {
-  using G = FwdGeo<kDP>;
+  using G = FwdGeo<kDP, kTrain>;
   uint8_t q[G::kQBufs][kRows * kDP * 2];
   uint8_t k[G::kStages][kN * kDP * 2];
   uint8_t v[G::kStages][kN * kDP * 2];
+  uint8_t res[G::kResBuf ? kRows * kDP * 2 : 16];  // (behind what needs 1024-byte alignment)
   uint64_t q_full[G::kQBufs], q_empty[G::kQBufs];
   uint64_t k_full[G::kStages], k_empty[G::kStages], v_full[G::kStages], v_empty[G::kStages];
   uint64_t s_full[2], p_full[2], pv_done[2], drain;  // [2]: by tile parity (a softmax warp
@@ -398,10 +416,10 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
                      const __grid_constant__ CUtensorMap tm_r, const __grid_constant__ Shape sh,
                      T* __restrict__ out, T* __restrict__ out_res, float* __restrict__ lse2, float* __restrict__ part_o,
                      float* __restrict__ part_lse, int n_items, int n_qt) {
-  using Geo = FwdGeo<kDP>;
+  using Geo = FwdGeo<kDP, kTrain>;
   constexpr uint32_t kStages = Geo::kStages, kQBufs = Geo::kQBufs;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  FwdSmem<kDP>& sm = *reinterpret_cast<FwdSmem<kDP>*>(
+  FwdSmem<kDP, kTrain>& sm = *reinterpret_cast<FwdSmem<kDP, kTrain>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const Waiter wait{&sm.abort, sh.err};
@@ -681,7 +699,11 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
       const int64_t lrow = ((int64_t)it.b * sh.H + it.h) * sh.Sq + qi;
       if (any && sh.splits == 1) {
         uint8_t* block = sm.q[qs.at] + (warp & 3) * 4096;
-        if (kTrain) {  // the remainders first: the same memory
+        if (Geo::kResBuf) {
+          if (lane == 0) bulk_wait_group_read<0>();  // the item before, long read
+          __syncwarp();
+          stage_pair<T>(t_o, lane, !none, inv_l, block, sm.res + (warp & 3) * 4096);
+        } else if (kTrain) {  // the remainders first: the same memory
 #pragma unroll 1
           for (int c = 0; c < kDP / 64; ++c)
             stage_rows<T, true>(t_o + c * 64, lane, !none, inv_l, block + c * kRows * 128);
@@ -695,12 +717,14 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
           }
           __syncwarp();
         }
+        if (!Geo::kResBuf)
 #pragma unroll 1
-        for (int c = 0; c < kDP / 64; ++c)
-          stage_rows<T, false>(t_o + c * 64, lane, !none, inv_l, block + c * kRows * 128);
+          for (int c = 0; c < kDP / 64; ++c)
+            stage_rows<T, false>(t_o + c * 64, lane, !none, inv_l, block + c * kRows * 128);
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) {
+          if (Geo::kResBuf) tma_store_4d(&tm_r, sm.res + (warp & 3) * 4096, 0, qi - lane, it.h, it.b);
           for (int c = 0; c * 64 < sh.D; ++c)
             tma_store_4d(&tm_o, block + c * kRows * 128, c * 64, qi - lane, it.h, it.b);
           bulk_commit_group();
@@ -1563,7 +1587,7 @@ int64_t fwd_clusters(int size) {
   static CrossFits fits{};
   if (size < 2) return INT64_MAX;
   return kFwdCtas * cross_attn_clusters((const void*)cross_fwd_kernel<__nv_bfloat16, kDP, false>,
-                                        kFwdThreads, sizeof(FwdSmem<kDP>) + 1024, size, fits);
+                                        kFwdThreads, sizeof(FwdSmem<kDP, false>) + 1024, size, fits);
 }
 CrossSplits fwd_splits(const CrossAttnArgs& a) {
   const int64_t items = row_tiles(a.Sq) * a.H * a.B;
@@ -1600,7 +1624,7 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
       !cross_attn_map(&mv, a.v, a.half, a.D, a.Sk, a.Hk, a.B, a.v_st, kN))
     return cudaErrorInvalidValue;
   static std::atomic<uint64_t> done{0};
-  const int smem = (int)sizeof(FwdSmem<kDP>) + 1024;
+  const int smem = (int)sizeof(FwdSmem<kDP, kTrain>) + 1024;
   auto kernel = cross_fwd_kernel<T, kDP, kTrain>;
   cudaError_t e = cross_attn_opt_in((const void*)kernel, smem, done);
   if (e != cudaSuccess) return e;
