@@ -849,7 +849,9 @@ struct Stride3 {
 };
 // The backward's row statistics: {-lse2, -delta} of every query, [B, H, pitch]
 // with the pitch Sq rounded up to 64 so that a streamed tile's 64 pairs are one
-// aligned 512-byte copy. Rows past Sq hold {-inf, 0}: their P is 0.
+// aligned 512-byte copy. Rows past Sq hold {-inf, 0}: their P is 0. (Made by the
+// queries' kernel instead, from tiles of O and its remainders, they cost a kernel
+// less, but a training step of 64 x 8 heads, 256 x 256 x 64, took 108 us instead of 101.)
 __host__ __device__ constexpr int stat_pitch(int Sq) { return (Sq + 63) / 64 * 64; }
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) cross_stats_kernel(const T* __restrict__ out,
@@ -974,7 +976,9 @@ struct BwdOut {
   float* part;         // [splits][1 or 2][rows][D] when splits > 1
 };
 
-template <typename T, int kDP, bool kKeys, int kABufs>
+// kSplit: pieces of the streamed axis (a template because the code that joins them
+// costs the others registers: 28.3 instead of 26.7 us on 64 x 8 heads, 256 x 256 x 64).
+template <typename T, int kDP, bool kKeys, int kABufs, bool kSplit>
 __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
     cross_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1,
                      const __grid_constant__ CUtensorMap tm_a2,
@@ -991,6 +995,9 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
                                       ~uintptr_t(1023));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const Waiter wait{&sm.abort, sh.err};
+
+  // a cluster's piece takes the stationary tiles' memory once all are read
+  static_assert(sizeof(sm.a1) + sizeof(sm.a2) >= (kKeys ? 2 : 1) * kRows * kDP * 4, "a piece there");
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kABufs; ++i) {
@@ -1371,7 +1378,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       const bool second = kKeys && group == 0;
       const uint32_t t_a = (second ? t_acc2 : t_acc1) + lanes;
       const float f = second ? unshift : sh.scale;
-      if (any && sh.splits == 1) {
+      if (any && !kSplit) {
         uint8_t* block = (second ? sm.a2[is.at] : sm.a1[is.at]) + (warp & 3) * 4096;
 #pragma unroll 1
         for (int c = kKeys ? 0 : group; c < kDP / 64; c += kKeys ? 1 : 2)
@@ -1384,13 +1391,25 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
                          it.b);
           bulk_commit_group();
         }
+      } else if (kSplit && outs.part == nullptr) {  // a cluster's piece
+        float* to = reinterpret_cast<float*>(sm.a1) + (second ? kRows * kDP : 0);
+        const int c1 = kKeys ? kDP : (group + 1) * (kDP / 2);
+#pragma unroll 1
+        for (int c = kKeys ? 0 : group * (kDP / 2); c < c1; c += 16) {
+          float v[16];
+          row16(t_a + c, any, true, f, v);
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(to + piece_at<kDP>(r, (c + i) / 4)) =
+                make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
       } else if (kKeys || group == 0) {
         const int rows_n = kKeys ? sh.Sk : sh.Sq, heads = kKeys ? sh.Hk : sh.H;
         const int64_t flat = ((int64_t)it.b * rows_n + row) * heads + it.head;
         const int64_t rows_all = (int64_t)sh.B * rows_n * heads;
         const Stride3 st3 = second ? outs.s2 : outs.s1;
         T* dst = (second ? outs.o2 : outs.o1) + it.b * st3.b + (int64_t)row * st3.s + it.head * st3.h;
-        float* part = sh.splits == 1 ? nullptr
+        float* part = !kSplit ? nullptr
                                      : outs.part + ((int64_t)it.split * (kKeys ? 2 : 1) + (second ? 1 : 0)) *
                                                        rows_all * sh.D + flat * sh.D;
         store_row<T>(t_a, sh.D, any, true, row < rows_n, f, dst, (T*)nullptr, part);
@@ -1413,6 +1432,22 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<512>(tmem);
+  }
+  if (kSplit && outs.part == nullptr) {  // one item per CTA
+    const BwdItem it = bwd_item<kKeys>(sh, blockIdx.x, n_rt);
+    const int rows = min(kRows, (kKeys ? sh.Sk : sh.Sq) - it.row0);
+    cluster_sync_all();
+    for (int which = 0; which < (kKeys ? 2 : 1); ++which) {
+      const Stride3& st3 = which ? outs.s2 : outs.s1;
+      T* dst = (which ? outs.o2 : outs.o1) + it.b * st3.b + (int64_t)it.row0 * st3.s + it.head * st3.h;
+      cluster_sum<kDP>(reinterpret_cast<float*>(sm.a1) + which * kRows * kDP, rows, sh.D, sh.splits,
+                       [&](int r, int c, float4 v) {
+                         *reinterpret_cast<uint2*>(dst + (int64_t)r * st3.s + 4 * c) =
+                             make_uint2(Type<T>::pack(v.x, v.y), Type<T>::pack(v.z, v.w));
+                       });
+    }
+    __syncwarp();
+    cluster_sync_all();  // no CTA leaves while others read its rows
   }
 }
 
@@ -1600,12 +1635,23 @@ CrossSplits fwd_splits(const CrossAttnArgs& a) {
   if (cross_attn_joins_more(items, s, want, tiles, num_sms())) return {want, false};
   return {s, s > 1};
 }
-int dq_splits(const CrossAttnArgs& a) {
-  return pieces(row_tiles(a.Sq) * a.H * a.B, num_sms(), ((int64_t)a.Sk + kBN - 1) / kBN);
+// Both halves of the backward have one CTA per SM.
+CrossSplits bwd_splits(int64_t items, int64_t tiles) {
+  static CrossFits fits{};
+  const int want = pieces(items, num_sms(), tiles);
+  int s = std::min(want, kCrossCluster);
+  using G = BwdGeo<64, true, 2>;
+  while (s > 1 && items > cross_attn_clusters((const void*)cross_bwd_kernel<__nv_bfloat16, 64, true, 2, true>,
+                                              G::kThreads, sizeof(BwdSmem<64, true, 2>) + 1024, s, fits))
+    --s;
+  if (cross_attn_joins_more(items, s, want, tiles, num_sms())) return {want, false};
+  return {s, s > 1};
 }
-int dkv_splits(const CrossAttnArgs& a) {
-  return pieces(row_tiles(a.Sk) * a.Hk * a.B, num_sms(),
-                ((int64_t)a.Sq + kBN - 1) / kBN * (a.H / a.Hk));
+CrossSplits dq_splits(const CrossAttnArgs& a) {
+  return bwd_splits(row_tiles(a.Sq) * a.H * a.B, ((int64_t)a.Sk + kBN - 1) / kBN);
+}
+CrossSplits dkv_splits(const CrossAttnArgs& a) {
+  return bwd_splits(row_tiles(a.Sk) * a.Hk * a.B, ((int64_t)a.Sq + kBN - 1) / kBN * (a.H / a.Hk));
 }
 
 template <typename T, int kDP, bool kTrain>
@@ -1642,10 +1688,10 @@ cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   return joined ? launch_cross_attn_join(a, splits, st) : cudaGetLastError();
 }
 
-template <typename T, int kDP, bool kKeys, int kABufs>
-cudaError_t run_bwd_half(const CrossAttnArgs& a, cudaStream_t st) {
-  const int splits = kKeys ? dkv_splits(a) : dq_splits(a);
-  if (splits > 1 && !a.partials) return cudaErrorInvalidValue;
+template <typename T, int kDP, bool kKeys, int kABufs, bool kSplit>
+cudaError_t run_bwd_half(const CrossAttnArgs& a, const CrossSplits& plan, cudaStream_t st) {
+  const int splits = plan.n;
+  if (plan.joined() && !a.partials) return cudaErrorInvalidValue;
   const int rb = kRows, cb = kBN;
   CUtensorMap mq, mk, mv, mo;
   if (!cross_attn_map(&mq, a.q, a.half, a.D, a.Sq, a.H, a.B, a.q_st, kKeys ? cb : rb) ||
@@ -1661,7 +1707,7 @@ cudaError_t run_bwd_half(const CrossAttnArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   constexpr int smem = (int)sizeof(BwdSmem<kDP, kKeys, kABufs>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory");
-  auto kernel = cross_bwd_kernel<T, kDP, kKeys, kABufs>;
+  auto kernel = cross_bwd_kernel<T, kDP, kKeys, kABufs, kSplit>;
   cudaError_t e = cross_attn_opt_in((const void*)kernel, smem, done);
   if (e != cudaSuccess) return e;
   const int S = kKeys ? a.Sk : a.Sq, heads = kKeys ? a.Hk : a.H;
@@ -1674,13 +1720,15 @@ cudaError_t run_bwd_half(const CrossAttnArgs& a, cudaStream_t st) {
   o.s1 = kKeys ? s3(a.dk_st) : s3(a.dq_st);
   o.o2 = kKeys ? (T*)a.dv : o.o1;
   o.s2 = kKeys ? s3(a.dv_st) : o.s1;
-  o.part = a.partials;
+  o.part = plan.joined() ? a.partials : nullptr;
   const int grid = (int)std::min<int64_t>(items, num_sms());
-  e = launch_pdl(kernel, dim3(grid), dim3(BwdGeo<kDP, kKeys, kABufs>::kThreads), smem, st, kKeys ? mk : mq, kKeys ? mv : mo,
-                 kKeys ? mq : mk, kKeys ? mo : mv, m1, kKeys ? m2 : m1, shape_of(a, splits, heads, items), (const float2*)a.stats, o, (int)items, n_rt);
+  e = launch_pdl_cluster(kernel, dim3(grid), dim3(BwdGeo<kDP, kKeys, kABufs>::kThreads),
+                         plan.clustered ? splits : 1, smem, st, kKeys ? mk : mq, kKeys ? mv : mo,
+                         kKeys ? mq : mk, kKeys ? mo : mv, m1, kKeys ? m2 : m1,
+                         shape_of(a, splits, heads, items), (const float2*)a.stats, o, (int)items, n_rt);
   if (e != cudaSuccess) return e;
   note_launch();
-  if (splits > 1) {
+  if (plan.joined()) {
     const int n_out = kKeys ? 2 : 1;
     const int64_t total = (int64_t)a.B * S * heads * (a.D / 8) * n_out;
     e = launch_pdl(cross_sum_kernel<T>,
@@ -1707,19 +1755,35 @@ cudaError_t run_stats(const CrossAttnArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-constexpr int kLongItem = 1024;  // keys
+constexpr int kLongItem = 1024;  // keys of a query tile (half of them under a causal mask)
+template <typename T, int kDP>
+cudaError_t run_dq(const CrossAttnArgs& a, cudaStream_t st) {
+  const CrossSplits plan = dq_splits(a);
+  // At head size 128 the queries' kernel has room for two stationary pairs and
+  // three stages or for one and five: the second where items are long (96 instead of
+  // 105 us on 32 x 12 heads, 256 x 1024, but 60.7 instead of 59.5 at 256 x 512; causal 207
+  // instead of 219 at 4096, 82 instead of 79 at 1024), or one to a CTA.
+  if constexpr (kDP == 128) {
+    if (plan.n > 1) return run_bwd_half<T, kDP, false, 1, true>(a, plan, st);
+    return (a.causal ? a.Sk / 2 : a.Sk) >= kLongItem
+               ? run_bwd_half<T, kDP, false, 1, false>(a, plan, st)
+               : run_bwd_half<T, kDP, false, 2, false>(a, plan, st);
+  } else {
+    return plan.n > 1 ? run_bwd_half<T, kDP, false, 2, true>(a, plan, st)
+                      : run_bwd_half<T, kDP, false, 2, false>(a, plan, st);
+  }
+}
+template <typename T, int kDP>
+cudaError_t run_dkv(const CrossAttnArgs& a, cudaStream_t st) {
+  const CrossSplits plan = dkv_splits(a);
+  return plan.n > 1 ? run_bwd_half<T, kDP, true, 2, true>(a, plan, st)
+                    : run_bwd_half<T, kDP, true, 2, false>(a, plan, st);
+}
 template <typename T, int kDP>
 cudaError_t run_bwd(const CrossAttnArgs& a, cudaStream_t st) {
   cudaError_t e = run_stats<T>(a, st);
-  if (e != cudaSuccess) return e;
-  // At head size 128 the queries' kernel has room for two stationary pairs and
-  // three stages or for one and five: the second where items are long.
-  if constexpr (kDP == 128) {
-    e = a.Sk >= kLongItem ? run_bwd_half<T, kDP, false, 1>(a, st) : run_bwd_half<T, kDP, false, 2>(a, st);
-  } else {
-    e = run_bwd_half<T, kDP, false, 2>(a, st);
-  }
-  if (e == cudaSuccess) e = run_bwd_half<T, kDP, true, 2>(a, st);
+  if (e == cudaSuccess) e = run_dq<T, kDP>(a, st);
+  if (e == cudaSuccess) e = run_dkv<T, kDP>(a, st);
   return e;
 }
 
@@ -1734,9 +1798,9 @@ int64_t cross_attn_fwd_partials(const CrossAttnArgs& a) {
 }
 // The two halves run one after the other and use the same scratch.
 int64_t cross_attn_bwd_partials(const CrossAttnArgs& a) {
-  const int sq = dq_splits(a), sk = dkv_splits(a);
-  const int64_t nq = sq > 1 ? (int64_t)sq * a.B * a.Sq * a.H * a.D : 0;
-  const int64_t nk = sk > 1 ? (int64_t)sk * 2 * a.B * a.Sk * a.Hk * a.D : 0;
+  const CrossSplits sq = dq_splits(a), sk = dkv_splits(a);
+  const int64_t nq = sq.joined() ? (int64_t)sq.n * a.B * a.Sq * a.H * a.D : 0;
+  const int64_t nk = sk.joined() ? (int64_t)sk.n * 2 * a.B * a.Sk * a.Hk * a.D : 0;
   return std::max(nq, nk);
 }
 
