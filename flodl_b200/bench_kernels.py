@@ -147,6 +147,56 @@ def case_flash_bert(kind):
     return fn, 2.5 * f_fwd, (Bb * Sb * 3 * Db * 2 + 2 * Bb * Sb * Db) * 2
 
 
+def case_cross(kind):
+    """Attention to a memory: the LM's heads over 256 encoder states, BERT-base
+    heads over padded ones, and a serving batch's next tokens."""
+    from ._ext import cuda_ext
+    C = cuda_ext()
+    shapes = {"cross_fwd": (B, S, S, H), "cross_bwd": (B, S, S, H),
+              "cross_fwd_bert": (32, 256, 512, 12), "cross_step": (B, 1, 4096, H)}
+    Bc, Sq, Sk, Hc = shapes[kind]
+    d = D // H
+    q, dout = _bf(Bc, Sq, Hc, d), _bf(Bc, Sq, Hc, d)
+    k, v = _bf(Bc, Sk, 2, Hc, d).unbind(2)
+    pad = None
+    if kind == "cross_fwd_bert":
+        pad = torch.arange(Sk, device="cuda")[None] >= Sk - torch.arange(Bc, device="cuda")[:, None] * 8
+    sc = 1.0 / math.sqrt(d)
+    flops, io = 4.0 * Bc * Hc * Sq * Sk * d, 2 * (2 * q.numel() + 2 * k.numel())
+    if pad is not None:
+        flops *= 1 - pad.float().mean().item()
+    if kind != "cross_bwd":
+        return (lambda: C.cross_attn_fwd(q, k, v, pad, False, sc, False)), flops, io
+    out, res, lse, _ = C.cross_attn_fwd(q, k, v, None, False, sc, True)
+    grads = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+
+    def fn():
+        C.cross_attn_bwd(dout, q, k, v, out, res, lse, None, None, False, sc, *grads)
+    return fn, 2.5 * flops, io + 2 * (2 * q.numel() + 2 * k.numel())
+
+
+def case_qk_norm_rope(kind):
+    """Norms and rotation of the LM's query and key heads, read from the packed
+    projection; "long" is 4 x 8192 tokens, 16 query and 4 key heads of 128."""
+    from ._ext import cuda_ext
+    C = cuda_ext()
+    Bc, Sc, Hq, Hk, d = (4, 8192, 16, 4, 128) if kind == "qk_norm_rope_long" else (B, S, H, H, D // H)
+    x = _bf(Bc, Sc, Hq + 2 * Hk, d)
+    q, k = x[:, :, :Hq], x[:, :, Hq:Hq + Hk]
+    w = torch.rand(d, device="cuda") + 0.5
+    t = torch.arange(Sc, device="cuda")[:, None] * 0.01 * torch.arange(1, 33, device="cuda")
+    cos, sin = t.cos(), t.sin()
+    yq, yk = q.contiguous(), k.contiguous()
+    n = q.numel() + k.numel()
+    if kind != "qk_norm_rope_bwd":
+        return (lambda: C.qk_norm_rope_fwd(q, k, w, w, cos, sin, None, 0, yq, yk, 1e-5)), 0.0, 4 * n
+    dq, dk = torch.empty_like(yq), torch.empty_like(yk)
+
+    def fn():
+        C.qk_norm_rope_backward(yq, yk, q, k, w, w, cos, sin, None, 0, 1e-5, dq, dk)
+    return fn, 0.0, 6 * n
+
+
 def case_ln(kind):
     from ._ext import cuda_ext
     C = cuda_ext()
@@ -338,6 +388,9 @@ CASES = {
     "gemm_fc1_nogelu": case_gemm,
     "flash_fwd": case_flash, "flash_bwd": case_flash,
     "flash_fwd_bert": case_flash_bert, "flash_bwd_bert": case_flash_bert,
+    "cross_fwd": case_cross, "cross_bwd": case_cross, "cross_fwd_bert": case_cross,
+    "cross_step": case_cross, "qk_norm_rope_fwd": case_qk_norm_rope,
+    "qk_norm_rope_bwd": case_qk_norm_rope, "qk_norm_rope_long": case_qk_norm_rope,
     "ln_fwd": case_ln, "ln_bwd": case_ln, "adamw": case_adamw, "sgd": case_sgd,
     "softmax_ce": case_softmax_ce, "embed_fwd": case_embed, "embed_bwd": case_embed,
     "im2col": case_conv, "col2im": case_conv, "bn_stats": case_conv, "bn_apply": case_conv,

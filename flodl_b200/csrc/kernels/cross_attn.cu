@@ -24,8 +24,24 @@
 // dQ has a kernel of its own, which recomputes S and dP (seven products instead
 // of five), so that no gradient is summed by atomics: results do not depend on
 // the order of execution. Where the items are fewer than the SMs, the streamed
-// axis is split and the pieces are added (the forward's joined by lse) in order
-// by a second kernel.
+// axis is split; the CTAs of an item's pieces form a cluster and add them (the
+// forward's joined by lse) in order, or a second kernel does.
+//
+// What bounds it, and what it takes (bf16; us, TFLOP/s of the products named above; the
+// library's 16-bit product reaches 1653):
+//   heads x queries x keys x D    forward     for training   dQ           dK/dV
+//   512 x 256 x 256 x 64          21.4 (400)  25.3 (340)     26.3 (490)   34.9 (490)
+//   384 x 256 x 512 x 64          28.3 (455)  31.9 (404)     33.9 (570)   50.7 (508)
+//   128 x 1024 x 1024 x 64        62.3 (551)  68.8 (499)     67.0 (770)   90.2 (760)
+//   64 x 2048^2 x 128, causal     89 (773)    101 (680)      124 (830)    162 (850)
+//   32 x 2048 x 8192 x 128        238 (1155)  260 (1058)     356 (1160)   505 (1090)
+// At head size 128 and long axes the tensor pipe is busy two thirds of the time: the
+// products of a tile and its elementwise work overlap but for the tile's round trip.
+// At head size 64 and a few tiles per item the round trip bounds it (scores, TMEM
+// loads, maximum, exponentials, TMEM stores, product: a warp's tile takes about 2100
+// cycles with another CTA's warp beside it, of which 512 are exponentials): tensor
+// pipe 15 to 20% busy, exponentials 31 to 38%, instruction issue 33 to 43%, DRAM 22 to 28%.
+// The seventh product and the statistics' pass are the price of sums in a fixed order.
 //
 // Hidden keys: a packing kernel turns the padding mask into a bit per key and
 // the end of the visible keys of each sample; tiles past it are not visited.
@@ -414,8 +430,9 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
                      const __grid_constant__ CUtensorMap tm_v,
                      const __grid_constant__ CUtensorMap tm_o,
                      const __grid_constant__ CUtensorMap tm_r, const __grid_constant__ Shape sh,
-                     T* __restrict__ out, T* __restrict__ out_res, float* __restrict__ lse2, float* __restrict__ part_o,
-                     float* __restrict__ part_lse, int n_items, int n_qt) {
+                     T* __restrict__ out, T* __restrict__ out_res, float* __restrict__ lse2,
+                     float* __restrict__ part_o, float* __restrict__ part_lse, int n_items,
+                     int n_qt) {
   using Geo = FwdGeo<kDP, kTrain>;
   constexpr uint32_t kStages = Geo::kStages, kQBufs = Geo::kQBufs;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -986,7 +1003,8 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
                      const __grid_constant__ CUtensorMap tm_b2,
                      const __grid_constant__ CUtensorMap tm_o1,
                      const __grid_constant__ CUtensorMap tm_o2, const __grid_constant__ Shape sh,
-                     const float2* __restrict__ stats, const __grid_constant__ BwdOut<T> outs, int n_items, int n_rt) {
+                     const float2* __restrict__ stats,
+                     const __grid_constant__ BwdOut<T> outs, int n_items, int n_rt) {
   using Geo = BwdGeo<kDP, kKeys, kABufs>;
   using Smem = BwdSmem<kDP, kKeys, kABufs>;
   constexpr uint32_t kStages = Geo::kStages, kBufs = Geo::kBufs;

@@ -17,7 +17,13 @@
 // the tensor pipe is not the limit. (A first version loaded the fragments
 // straight from global memory: 680 instructions per 16 keys, 2.5 TB/s.)
 // The key axis is split over CTAs until the SMs are covered; the pieces are
-// joined by their lse in a second kernel, in a fixed order.
+// joined by their lse, in a fixed order, by a cluster of up to eight CTAs through
+// distributed shared memory or by a second kernel. Measured (one query per head, bf16): 512
+// heads x 4096 x 64 in 86.7 us, 6.2 TB/s (0.96 of a copy's rate); 384 padded heads x
+// 512 x 64 in 8.4; 16 memory heads x 32768 x 128 (64 query heads) in 49, 5.5 TB/s with
+// its join; one sequence's 8 heads x 100 in 2.8, a launch. (17 to 64 rows as two to
+// four groups of 16, a warp to each: 21 us at 37 rows x 4001 keys of 16 heads, where
+// the 128-row tiles of tcgen05 take 13.)
 #include "sm100_ptx.cuh"
 #include "cross_attn.h"
 #include "cross_attn_join.cuh"
@@ -545,6 +551,11 @@ CrossSplits cross_attn_few_splits(const CrossAttnArgs& a) {
   const int64_t want = std::min(3ll * num_sms() / units, (long long)(tiles / 4));
   const int64_t need = (2 * tiles + kMaxWords - 1) / kMaxWords;
   const int64_t least = a.key_pad ? std::max<int64_t>(1, need) : 1;
+  // Between one and one and a half times the CTAs that fit, a second wave would leave
+  // most SMs idle: three shorter waves instead (512 heads x 4096 x 64: 104 -> 89 us;
+  // 448 x 1500 x 128: 66.5 -> 65; 512 x 1024 x 64 would go from 30 to 36).
+  const int64_t places = 3ll * num_sms();
+  if (units > places && 2 * units < 3 * places && tiles >= 24 && least <= 3) return {3, true};
   // as many as a cluster joins and the GPU holds at once (63 heads x 8192 x 64: 24 us
   // with five or six pieces each, 34 with seven that wait for one another, 28 joined
   // by a second kernel)

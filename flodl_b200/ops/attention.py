@@ -7,6 +7,11 @@ O += PV on tcgen05 with the accumulators in TMEM, online softmax, causal tile
 skipping. Q/K/V are read straight out of the packed ``[T, 3C]`` projection
 output and O is written as ``[T, C]`` (token-major), so no transposes run
 around the kernel.
+
+:func:`cross_attention` takes queries, keys and values in tensors of their own
+(another sequence's states, shared memory heads, single tokens of serving) and
+:func:`attention_qk_norm` norms and rotates the heads of a packed projection
+before either form.
 """
 from __future__ import annotations
 

@@ -254,6 +254,7 @@ SPLIT = [  # long key axes of few heads: 2 to 8 pieces, and more than that
     (2, 1, 1, 1, 2500, 64), (5, 3, 2, 1, 1300, 128), (1, 40, 2, 1, 9000, 72),
     (1, 100, 1, 1, 16000, 64), (1, 2, 4, 2, 16000, 128),
     (1, 9000, 1, 1, 100, 128), (2, 700, 1, 1, 90, 64),
+    (60, 1, 8, 8, 1600, 64),
 ]
 
 
