@@ -180,17 +180,22 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> cross_attn_fwd(
   return {out, res, lse, bits};
 }
 
-// Gradients into dq, dk, dv (any strides of 16 bytes).
+optional<Tensor> if_defined(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
+
+// Gradients into dq, dk, dv (any strides of 16 bytes); without dq, or without dk
+// and dv, that half is left out.
 void cross_attn_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v,
                     const Tensor& out, const Tensor& res, const Tensor& lse2,
                     const optional<Tensor>& key_pad,
-                    const optional<Tensor>& mask_bits, bool causal, double scale, Tensor& dq,
-                    Tensor& dk, Tensor& dv) {
+                    const optional<Tensor>& mask_bits, bool causal, double scale,
+                    const optional<Tensor>& dq, const optional<Tensor>& dk,
+                    const optional<Tensor>& dv) {
   auto a = cross_args(q, k, v, key_pad, mask_bits, causal, scale);
   cross_strides(dout, "dout", a.B, a.Sq, a.H, a.D, q, a.do_st);
-  cross_strides(dq, "dq", a.B, a.Sq, a.H, a.D, q, a.dq_st);
-  cross_strides(dk, "dk", a.B, a.Sk, a.Hk, a.D, q, a.dk_st);
-  cross_strides(dv, "dv", a.B, a.Sk, a.Hk, a.D, q, a.dv_st);
+  FL_CHECK(dk.has_value() == dv.has_value(), "cross_attn: dk and dv come together");
+  if (dq) cross_strides(*dq, "dq", a.B, a.Sq, a.H, a.D, q, a.dq_st);
+  if (dk) cross_strides(*dk, "dk", a.B, a.Sk, a.Hk, a.D, q, a.dk_st);
+  if (dv) cross_strides(*dv, "dv", a.B, a.Sk, a.Hk, a.D, q, a.dv_st);
   for (const Tensor* t : {&out, &res})
     FL_CHECK(t->sizes() == q.sizes() && t->is_contiguous() && t->scalar_type() == q.scalar_type() &&
                  t->device() == q.device(), "cross_attn: out and its remainders must be the forward's");
@@ -202,9 +207,9 @@ void cross_attn_bwd(const Tensor& dout, const Tensor& q, const Tensor& k, const 
   a.out = out.data_ptr();
   a.out_res = res.data_ptr();
   a.lse2 = lse2.data_ptr<float>();
-  a.dq = dq.data_ptr();
-  a.dk = dk.data_ptr();
-  a.dv = dv.data_ptr();
+  a.dq = dq ? dq->data_ptr() : nullptr;
+  a.dk = dk ? dk->data_ptr() : nullptr;
+  a.dv = dv ? dv->data_ptr() : nullptr;
   Tensor bits;
   if (a.key_pad && !a.words) {
     bits = cross_attn_mask(*key_pad);
@@ -225,8 +230,6 @@ Tensor tma_ready(const Tensor& t) {
   for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
-
-optional<Tensor> if_defined(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
 
 struct CrossAttn : public torch::autograd::Function<CrossAttn> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q0, const Tensor& k0,
@@ -249,12 +252,14 @@ struct CrossAttn : public torch::autograd::Function<CrossAttn> {
     {
       at::NoGradGuard no_grad;
       const Tensor dout = tma_ready(grads[0].to(q.scalar_type()));
-      dq = at::empty(q.sizes(), q.options());
-      dk = at::empty(k.sizes(), k.options());
-      dv = at::empty(v.sizes(), v.options());
+      if (ctx->needs_input_grad(0)) dq = at::empty(q.sizes(), q.options());
+      if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
+        dk = at::empty(k.sizes(), k.options());
+        dv = at::empty(v.sizes(), v.options());
+      }
       cross_attn_bwd(dout, q, k, v, s[3], s[4], s[5], if_defined(s[6]), if_defined(s[7]),
-                     ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), dq, dk,
-                     dv);
+                     ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(),
+                     if_defined(dq), if_defined(dk), if_defined(dv));
     }
     return once_differentiable({dq, dk, dv, Tensor(), Tensor(), Tensor()}, "cross_attention");
   }

@@ -1800,8 +1800,8 @@ cudaError_t run_dkv(const CrossAttnArgs& a, cudaStream_t st) {
 template <typename T, int kDP>
 cudaError_t run_bwd(const CrossAttnArgs& a, cudaStream_t st) {
   cudaError_t e = run_stats<T>(a, st);
-  if (e == cudaSuccess) e = run_dq<T, kDP>(a, st);
-  if (e == cudaSuccess) e = run_dkv<T, kDP>(a, st);
+  if (e == cudaSuccess && a.dq) e = run_dq<T, kDP>(a, st);
+  if (e == cudaSuccess && a.dk) e = run_dkv<T, kDP>(a, st);
   return e;
 }
 
@@ -1817,8 +1817,8 @@ int64_t cross_attn_fwd_partials(const CrossAttnArgs& a) {
 // The two halves run one after the other and use the same scratch.
 int64_t cross_attn_bwd_partials(const CrossAttnArgs& a) {
   const CrossSplits sq = dq_splits(a), sk = dkv_splits(a);
-  const int64_t nq = sq.joined() ? (int64_t)sq.n * a.B * a.Sq * a.H * a.D : 0;
-  const int64_t nk = sk.joined() ? (int64_t)sk.n * 2 * a.B * a.Sk * a.Hk * a.D : 0;
+  const int64_t nq = a.dq && sq.joined() ? (int64_t)sq.n * a.B * a.Sq * a.H * a.D : 0;
+  const int64_t nk = a.dk && sk.joined() ? (int64_t)sk.n * 2 * a.B * a.Sk * a.Hk * a.D : 0;
   return std::max(nq, nk);
 }
 
@@ -1847,7 +1847,7 @@ cudaError_t launch_cross_attn_fwd(const CrossAttnArgs& a, cudaStream_t st) {
 }
 
 cudaError_t launch_cross_attn_bwd(const CrossAttnArgs& a, cudaStream_t st) {
-  if (bad_shape(a) || !a.lse2 || !a.stats || (a.key_pad && (!a.words || !a.vis_end)))
+  if (bad_shape(a) || !a.lse2 || !a.out_res || !a.stats || !a.dk != !a.dv || (a.key_pad && (!a.words || !a.vis_end)))
     return cudaErrorInvalidValue;
   if (a.D <= 64) return a.half ? run_bwd<__half, 64>(a, st) : run_bwd<__nv_bfloat16, 64>(a, st);
   return a.half ? run_bwd<__half, 128>(a, st) : run_bwd<__nv_bfloat16, 128>(a, st);

@@ -717,7 +717,11 @@ class RotaryEmbedding(Module):
         if positions is None:
             y = self.forward(x[..., :R])
         else:
-            cos, sin = (t[positions][:, None].to(x.dtype) for t in (self.cos, self.sin))
+            if positions.dtype != torch.int64 or positions.shape != (x.shape[0], x.shape[2]) or \
+                    positions.device != x.device:
+                raise ValueError(f"positions must be int64 {[x.shape[0], x.shape[2]]} on {x.device}")
+            cos, sin = (t[:, None].to(x.dtype)
+                        for t in ops.norm.rotary_rows(self.cos, self.sin, positions))
             x1, x2 = x[..., 0:R:2], x[..., 1:R:2]
             y = torch.stack((x1 * cos - x2 * sin, x1 * sin + x2 * cos), dim=-1).flatten(-2)
         return torch.cat((y, x[..., R:]), -1) if R < x.shape[-1] else y

@@ -170,8 +170,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     copied. Up to 16 query rows per memory head (``Sq * H / Hk``; the single
     tokens of serving) take a form that streams the memory once. Scores and
     sums are f32, probabilities are rounded to the inputs' type for the
-    products. Gradients are the same from run to run. Other inputs run the
-    composed form in f32 or f64.
+    products, and score gradients likewise in the backward (in f16 those beyond
+    65504 become infinite: scale the loss as for any f16 training). Gradients are
+    the same from run to run. Other inputs run the composed form in f32 or f64.
     """
     if use_kernels(q):
         out = C().cross_attention(q, k, v, key_padding, causal, scale)
@@ -227,9 +228,11 @@ class _CrossPackedFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, kv, out, res, lse, key_padding, bits = ctx.saved_tensors
-        dq, dkv = torch.empty_like(q), torch.empty_like(kv)
+        dq = torch.empty_like(q) if ctx.needs_input_grad[0] else None
+        dkv = torch.empty_like(kv) if ctx.needs_input_grad[1] else None
         C().cross_attn_bwd(_fresh(dout.to(q.dtype)), q, kv[:, :, 0], kv[:, :, 1], out, res, lse,
-                           key_padding, bits, *ctx.consts, dq, dkv[:, :, 0], dkv[:, :, 1])
+                           key_padding, bits, *ctx.consts, dq,
+                           *((dkv[:, :, 0], dkv[:, :, 1]) if dkv is not None else (None, None)))
         return dq, dkv, None, None, None
 
 

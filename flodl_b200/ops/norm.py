@@ -198,6 +198,21 @@ def check_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, offset):
                          f"{cos.shape[0]} rows")
 
 
+def rotary_rows(cos, sin, positions):
+    """The tables' rows of ``positions``. One outside the tables raises on the CPU;
+    on CUDA, where the check would wait for the device, its row is NaN."""
+    rows = cos.shape[0]
+    if not positions.is_cuda:
+        if positions.numel() and (int(positions.min()) < 0 or int(positions.max()) >= rows):
+            raise IndexError(f"a position is outside the tables' {rows} rows")
+        return cos[positions], sin[positions]
+    if rows == 0:
+        return tuple(t.new_full((*positions.shape, t.shape[1]), float("nan")) for t in (cos, sin))
+    bad = ((positions < 0) | (positions >= rows))[..., None]
+    at = positions.clamp(0, rows - 1)
+    return tuple(t[at].masked_fill(bad, float("nan")) for t in (cos, sin))
+
+
 def _qk_norm_rope_composed(x, w, cos, sin, eps):
     at_least = torch.float64 if x.dtype == torch.float64 else torch.float32
     y = x.to(at_least)
@@ -244,14 +259,6 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     if cos is not None and positions is None:
         c, s = cos[offset:offset + q.shape[1]], sin[offset:offset + q.shape[1]]
     elif cos is not None:
-        rows = cos.shape[0]
-        if not q.is_cuda:
-            if positions.numel() and (int(positions.min()) < 0 or int(positions.max()) >= rows):
-                raise IndexError(f"a position is outside the tables' {rows} rows")
-            c, s = cos[positions], sin[positions]
-        else:
-            bad = ((positions < 0) | (positions >= rows))[..., None]
-            at = positions.clamp(0, max(rows - 1, 0))
-            c, s = (t[at].masked_fill(bad, float("nan")) for t in (cos, sin))
+        c, s = rotary_rows(cos, sin, positions)
     return (_qk_norm_rope_composed(q, q_weight, c, s, eps),
             _qk_norm_rope_composed(k, k_weight, c, s, eps))

@@ -295,3 +295,32 @@ def test_gpu_decoder_block_trains_captured():
     for p, e, n in zip(params, eager_grads, names[2:]):
         # the projections' weight gradients are split-K sums in any order
         torch.testing.assert_close(p.grad, e, rtol=1e-3, atol=1e-3 * float(e.abs().max()), msg=n)
+
+
+def test_rotary_positions_are_checked():
+    rope = RotaryEmbedding(8, 16)
+    x = torch.randn(2, 3, 4, 8)
+    at = torch.tensor([[0, 15, 3, 3], [1, 2, 3, 4]])
+    y = rope.rotate(x, at)
+    for b in range(2):
+        for s in range(4):
+            one = x.new_zeros(1, 3, 16, 8)
+            one[:, :, at[b, s]] = x[b, :, s]
+            assert torch.allclose(rope.rotate(one)[0, :, at[b, s]], y[b, :, s], atol=1e-6)
+    for bad in (at + 1, at - 1):
+        with pytest.raises(IndexError):
+            rope.rotate(x, bad)
+    for bad in (at.int(), at[:1], at[:, :3]):
+        with pytest.raises(ValueError):
+            rope.rotate(x, bad)
+
+
+@pytest.mark.gpu
+def test_gpu_rotary_position_outside_the_tables_is_nan():
+    rope = RotaryEmbedding(8, 16, device="cuda")
+    x = torch.randn(2, 3, 4, 8, device="cuda")
+    at = torch.tensor([[0, 15, 16, 3], [1, -1, 1 << 40, 4]], device="cuda")
+    y = rope.rotate(x, at)
+    assert torch.isnan(y).all(1).all(-1).tolist() == [[False, False, True, False],
+                                                     [False, True, True, False]]
+    assert not torch.isnan(y[0, :, :2]).any()

@@ -247,6 +247,31 @@ def test_gpu_many_items_of_one_tile(D):
     check("cuda", torch.bfloat16, 40, 130, 8, 8, 17, D, mask="right")
     check("cuda", torch.bfloat16, 50, 150, 8, 8, 150, D, causal=True)
     check("cuda", torch.bfloat16, 100, 40, 8, 4, 50, D, mask="empty")
+    check("cuda", torch.bfloat16, 40, 130, 8, 8, 1100, D, mask="one")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+def test_gpu_gradients_of_one_side(packed):
+    # frozen memories, frozen queries: the wanted side's gradient is the same
+    q, k, v, do = make(2, 70, 4, 2, 90, 64, torch.bfloat16, "cuda")
+    kv = torch.stack((k, v), 2)
+
+    def grads(wants_q, wants_kv):
+        a, b = q.clone().requires_grad_(wants_q), kv.clone().requires_grad_(wants_kv)
+        out = (ops.cross_attention_packed(a, b) if packed
+               else ops.cross_attention(a, b[:, :, 0], b[:, :, 1]))
+        out.backward(do)
+        return a.grad, b.grad
+
+    both = grads(True, True)
+    only_q, none = grads(True, False)
+    assert none is None and torch.equal(only_q, both[0])
+    none, only_kv = grads(False, True)
+    assert none is None and torch.equal(only_kv, both[1])
+    x = v.clone().requires_grad_()
+    ops.cross_attention(q, k, x).backward(do)
+    assert torch.equal(x.grad, both[1][:, :, 1])
 
 
 SPLIT = [  # long key axes of few heads: 2 to 8 pieces, and more than that
