@@ -32,8 +32,8 @@
 //   heads x queries x keys x D    forward     for training   dQ           dK/dV
 //   512 x 256 x 256 x 64          21.4 (400)  25.3 (340)     26.3 (490)   34.9 (490)
 //   384 x 256 x 512 x 64          28.3 (455)  31.9 (404)     33.9 (570)   50.7 (508)
-//   128 x 1024 x 1024 x 64        62.3 (551)  68.8 (499)     67.0 (770)   90.2 (760)
-//   64 x 2048^2 x 128, causal     89 (773)    101 (680)      124 (830)    162 (850)
+//   128 x 1024 x 1024 x 64        60 (577)    66 (518)       67 (770)     92 (745)
+//   64 x 2048^2 x 128, causal     80 (863)    91 (757)       117 (880)    154 (894)
 //   32 x 2048 x 8192 x 128        238 (1155)  260 (1058)     356 (1160)   505 (1090)
 // At head size 128 and long axes the tensor pipe is busy two thirds of the time: the
 // products of a tile and its elementwise work overlap but for the tile's round trip.
@@ -293,10 +293,24 @@ struct Shape {
   int nwords, n_items;
   uint32_t* err;
   // item -> (row tile, batch, head, piece): divisors of an item's index
-  FastDiv by_splits, by_bh, by_heads, by_group;
+  FastDiv by_splits, by_outer, by_heads, by_group;
 };
 
-// An item's coordinates: the piece fastest, then heads, batches, row tiles.
+// The items of a CTA, one of each round of gridDim.x: every second round is dealt
+// backwards, so that a CTA with one of the heaviest items gets one of the lightest
+// next (causal 2 x 16 heads, 4096 x 4096 x 64: forward 136 -> 113 us, dQ 137 -> 124, dK/dV
+// 195 -> 178).
+struct Walk {
+  int at = blockIdx.x, step = 2 * (int)(gridDim.x - blockIdx.x) - 1;
+  __device__ __forceinline__ int after() const { return at + step; }
+  __device__ __forceinline__ void next() {
+    at += step;
+    step = 2 * (int)gridDim.x - step;
+  }
+};
+
+// An item's coordinates: the piece fastest, then heads; samples slowest (a sample
+// with few visible keys has light items), or under a causal mask row tiles.
 struct ItemAt {
   int rt, b, head, split;
 };
@@ -304,10 +318,11 @@ __device__ __forceinline__ ItemAt item_at(const Shape& s, int item) {
   ItemAt a;
   const uint32_t i = s.by_splits.div(item);
   a.split = item - i * s.by_splits.d;
-  a.rt = s.by_bh.div(i);
-  const uint32_t bh = i - a.rt * s.by_bh.d;
-  a.b = s.by_heads.div(bh);
-  a.head = bh - a.b * s.by_heads.d;
+  const uint32_t outer = s.by_outer.div(i), rest = i - outer * s.by_outer.d;
+  const uint32_t inner = s.by_heads.div(rest);
+  a.head = rest - inner * s.by_heads.d;
+  a.rt = s.causal ? outer : inner;
+  a.b = s.causal ? inner : outer;
   return a;
 }
 // Streamed tiles [lo, hi) of piece `split` of nt.
@@ -387,8 +402,7 @@ struct FwdSmem {
   uint32_t tmem_base, abort;
 };
 
-// Items run from the last query tile to the first (under a causal mask the
-// heaviest first), heads and batches fastest.
+// Query tiles run from the last to the first: under a causal mask the heaviest first.
 struct FwdItem {
   int qt, h, b, split, lo, hi;  // key tiles [lo, hi)
 };
@@ -484,8 +498,8 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
       tma_prefetch_desc(&tm_v);
       uint32_t n = 0, t = 0;
       bool ok = true;
-      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-        const FwdItem it = fwd_item(sh, item, n_qt);
+      for (Walk item; item.at < n_items && ok; item.next()) {
+        const FwdItem it = fwd_item(sh, item.at, n_qt);
         if (it.lo >= it.hi) continue;
         const uint32_t qb = n % kQBufs;
         if (!(ok = wait(&sm.q_empty[qb], ((n / kQBufs) & 1) ^ 1))) break;
@@ -538,10 +552,10 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
       // where the next item's Q has a buffer of its own
       bool behind = false, behind_acc = false;
       FwdItem after = fwd_item(sh, blockIdx.x, n_qt);
-      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+      for (Walk item; item.at < n_items && ok; item.next()) {
         const FwdItem it = after;
         if (it.lo >= it.hi) {
-          after = fwd_item(sh, item + gridDim.x, n_qt);
+          after = fwd_item(sh, item.after(), n_qt);
           continue;
         }
         if (kQBufs == 1 && behind) {
@@ -560,7 +574,7 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
           umma_commit(&sm.k_empty[ks.at]);
           ks.next();
           ss.next();
-          if (j == it.hi - 1) after = fwd_item(sh, item + gridDim.x, n_qt);  // while products run
+          if (j == it.hi - 1) after = fwd_item(sh, item.after(), n_qt);  // while products run
           if (behind && !(ok = issue_pv(behind_acc))) break;
           behind = true;
           behind_acc = j > it.lo;
@@ -596,7 +610,7 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
       owed = nullptr;
     };
     FwdItem after = fwd_item(sh, blockIdx.x, n_qt);
-    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+    for (Walk item; item.at < n_items && ok; item.next()) {
       const FwdItem it = after;
       const int qi = it.qt * kRows + r;
       // tiles before `plain` hold no hidden score
@@ -699,7 +713,7 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
         give_back();
       }
       if (!ok) break;
-      after = fwd_item(sh, item + gridDim.x, n_qt);  // while the last product runs
+      after = fwd_item(sh, item.after(), n_qt);  // while the last product runs
       // ---- output: O / l and lse
       const bool any = it.lo < it.hi;
       if (any) {
@@ -1059,8 +1073,8 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       tma_prefetch_desc(&tm_b2);
       uint32_t n = 0, u = 0;
       bool ok = true;
-      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-        const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
+      for (Walk item; item.at < n_items && ok; item.next()) {
+        const BwdItem it = bwd_item<kKeys>(sh, item.at, n_rt);
         if (it.lo >= it.hi) continue;
         const uint32_t ab = n % kABufs;
         if (!(ok = wait(&sm.a_empty[ab], ((n / kABufs) & 1) ^ 1))) break;
@@ -1135,8 +1149,8 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
         as.next();
         return true;
       };
-      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-        const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
+      for (Walk item; item.at < n_items && ok; item.next()) {
+        const BwdItem it = bwd_item<kKeys>(sh, item.at, n_rt);
         if (it.lo >= it.hi) continue;
         if (!(ok = wait(&sm.a_full[is.at], is.phase))) break;
         const uint32_t a1 = a10 + is.at * Geo::kABytes, a2 = a20 + is.at * Geo::kABytes;
@@ -1174,8 +1188,8 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       Ring<kBufs> sb;
       Ring<kABufs> is;
       bool ok = true, issued = false;
-      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-        const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
+      for (Walk item; item.at < n_items && ok; item.next()) {
+        const BwdItem it = bwd_item<kKeys>(sh, item.at, n_rt);
         if (it.lo >= it.hi) continue;
         if (!(ok = wait(&sm.a_full[is.at], is.phase))) break;
         const uint32_t a1 = a10 + is.at * Geo::kABytes, a2 = a20 + is.at * Geo::kABytes;
@@ -1209,8 +1223,8 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       Ring<kBufs> sb;
       uint32_t n = 0;
       bool ok = true, issued = false;
-      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-        const BwdItem it = bwd_item<kKeys>(sh, item, n_rt);
+      for (Walk item; item.at < n_items && ok; item.next()) {
+        const BwdItem it = bwd_item<kKeys>(sh, item.at, n_rt);
         if (it.lo >= it.hi) continue;
         // the item before has been read out
         if (!(ok = wait(&sm.acc_free, (n & 1) ^ 1))) break;
@@ -1280,7 +1294,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
     };
     BwdItem after = bwd_item<kKeys>(sh, blockIdx.x, n_rt);
     float2 after_row = row_of(after);
-    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+    for (Walk item; item.at < n_items && ok; item.next()) {
       const BwdItem it = after;
       const int row = it.row0 + r;
       const bool any = it.lo < it.hi;
@@ -1378,7 +1392,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       }
       if (!ok) break;
       // the next item, and its row's load, while the last product runs
-      after = bwd_item<kKeys>(sh, item + gridDim.x, n_rt);
+      after = bwd_item<kKeys>(sh, item.after(), n_rt);
       after_row = row_of(after);
       // A group without a tile in this item gives the buffer back here, before it waits
       // for the products: of items of one tile each, these may come behind scores
@@ -1612,7 +1626,9 @@ Shape shape_of(const CrossAttnArgs& a, int splits, int heads, int64_t items) {
   s.nwords = (a.Sk + 31) / 32;
   s.err = default_err_word();
   s.by_splits = FastDiv((uint32_t)splits);
-  s.by_bh = FastDiv((uint32_t)(heads * a.B));
+  // row tiles of an item's head: items / (pieces * heads * samples)
+  const int64_t tiles = items / ((int64_t)splits * heads * a.B);
+  s.by_outer = FastDiv((uint32_t)(heads * (a.causal ? a.B : tiles)));
   s.by_heads = FastDiv((uint32_t)heads);
   s.by_group = FastDiv((uint32_t)s.G);
   return s;
