@@ -30,11 +30,11 @@
 // What bounds it, and what it takes (bf16; us, TFLOP/s of the products named above; the
 // library's 16-bit product reaches 1653):
 //   heads x queries x keys x D    forward     for training   dQ           dK/dV
-//   512 x 256 x 256 x 64          21.4 (400)  25.3 (340)     26.3 (490)   34.9 (490)
-//   384 x 256 x 512 x 64          28.3 (455)  31.9 (404)     33.9 (570)   50.7 (508)
-//   128 x 1024 x 1024 x 64        60 (577)    66 (518)       67 (770)     92 (745)
-//   64 x 2048^2 x 128, causal     80 (863)    91 (757)       117 (880)    154 (894)
-//   32 x 2048 x 8192 x 128        238 (1155)  260 (1058)     356 (1160)   505 (1090)
+//   512 x 256 x 256 x 64          20.6 (416)  24.9 (345)     24.9 (518)   35.0 (490)
+//   384 x 256 x 512 x 64          27.1 (476)  31.5 (409)     32.9 (588)   51.5 (500)
+//   128 x 1024 x 1024 x 64        57 (603)    65 (531)       62 (830)     89 (771)
+//   64 x 2048^2 x 128, causal     79 (873)    92 (751)       113 (914)    150 (915)
+//   32 x 2048 x 8192 x 128        231 (1192)  252 (1093)     344 (1197)   520 (1060)
 // At head size 128 and long axes the tensor pipe is busy two thirds of the time: the
 // products of a tile and its elementwise work overlap but for the tile's round trip.
 // At head size 64 and a few tiles per item the round trip bounds it (scores, TMEM
@@ -77,6 +77,7 @@ template <>
 struct Type<__nv_bfloat16> {
   static constexpr uint32_t kIdesc = 1;  // tcgen05 kind::f16 operand format
   static constexpr float kShift = 0.f;
+  static constexpr bool kCubic = true;  // (see f2_exp2_cubic)
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
   static __device__ __forceinline__ uint64_t unpack(uint32_t v) {
     const float2 f = unpack_bf16x2(v);
@@ -89,6 +90,7 @@ struct Type<__half> {
   // P of a long row lies below f16's normal range (2^-14): the backward's P^T
   // is formed at 2^7 times its value and dV scaled back
   static constexpr float kShift = 7.f;
+  static constexpr bool kCubic = false;
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -107,6 +109,40 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^x of a pair on the FMA pipe, for x <= 128 (below -126.5: zero; NaN stays NaN):
+// 2^n by the exponent bits times a cubic for 2^f, |f| <= 1/2, fitted by Remez' exchange
+// for relative error (7.5e-5). The exponential unit takes 8 cycles for a warp's 32
+// values; every fourth pair done this way shortens a tile's round trip (128 heads,
+// 1024 x 1024 x 64: forward 61.9 -> 58.1 us, dQ 66.5 -> 62.6; every second pair 66.6 and 72,
+// issue then bounds it; dK/dV, which needs an addition more per pair, 90 -> 94).
+// Only for P that is rounded to bf16 (half a step: 2e-3): f16 would want a degree more,
+// and gains nothing then.
+__device__ __forceinline__ uint64_t f2_exp2_cubic(uint64_t x) {
+  float a, b;
+  f2_unpack(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
+  x = f2_pack(a, b);
+  const uint64_t t = f2_add(x, f2_splat(12582912.f));  // 1.5 * 2^23: n in the low bits
+  const uint64_t f = f2_fma(f2_add(t, f2_splat(-12582912.f)), f2_splat(-1.f), x);
+  uint64_t p = f2_fma(f, f2_splat(0.0551716685f), f2_splat(0.242611125f));
+  p = f2_fma(p, f, f2_splat(0.693260968f));
+  p = f2_fma(p, f, f2_splat(0.999928057f));
+  f2_unpack(t, a, b);
+  return f2_mul(p, f2_pack(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u),
+                           __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
+}
+// 2^x of a pair, the kind by the pair's index.
+template <bool kCubic>
+__device__ __forceinline__ void exp2_pair(uint64_t x, int pair, float& p0, float& p1) {
+  if (kCubic && pair % 4 == 0) {
+    f2_unpack(f2_exp2_cubic(x), p0, p1);
+  } else {
+    f2_unpack(x, p0, p1);
+    p0 = ex2(p0);
+    p1 = ex2(p1);
+  }
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
@@ -686,10 +722,10 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
           uint32_t pw[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            float a0, a1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c * 16 + 2 * i]),
-                                     __uint_as_float(v[c * 16 + 2 * i + 1])), sl2x2, neg_m), a0, a1);
-            const float p0 = ex2(a0), p1 = ex2(a1);
+            float p0, p1;
+            exp2_pair<Type<T>::kCubic>(
+                f2_fma(f2_pack(__uint_as_float(v[c * 16 + 2 * i]),
+                               __uint_as_float(v[c * 16 + 2 * i + 1])), sl2x2, neg_m), i, p0, p1);
             pw[i] = Type<T>::pack(p0, p1);
             a[i & 1] = f2_add(a[i & 1], f2_pack(p0, p1));
             if (kTrain) b[i & 1] = f2_add(b[i & 1], Type<T>::unpack(pw[i]));
@@ -1354,9 +1390,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
                   f2_fma(f2_pack(__uint_as_float(s16[i]), __uint_as_float(s16[i + 1])), sl2x2, nl);
               if (kShift != 0.f) e = f2_add(e, f2_splat(kShift));
               float p0, p1, d0, d1;
-              f2_unpack(e, p0, p1);
-              p0 = ex2(p0);
-              p1 = ex2(p1);
+              exp2_pair<!kKeys && Type<T>::kCubic>(e, i / 2, p0, p1);
               uint64_t d = f2_add(f2_pack(__uint_as_float(d16[i]), __uint_as_float(d16[i + 1])), nd);
               if (kShift != 0.f) d = f2_mul(d, f2_splat(unshift));
               f2_unpack(f2_mul(f2_pack(p0, p1), d), d0, d1);
