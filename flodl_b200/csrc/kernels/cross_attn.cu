@@ -1502,6 +1502,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
   if (kSplit && outs.part == nullptr) {  // one item per CTA
     const BwdItem it = bwd_item<kKeys>(sh, blockIdx.x, n_rt);
     const int rows = min(kRows, (kKeys ? sh.Sk : sh.Sq) - it.row0);
+    __syncwarp();  // an aligned barrier
     cluster_sync_all();
     for (int which = 0; which < (kKeys ? 2 : 1); ++which) {
       const Stride3& st3 = which ? outs.s2 : outs.s1;

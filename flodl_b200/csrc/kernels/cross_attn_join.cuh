@@ -29,6 +29,7 @@ __device__ __forceinline__ int piece_at(int r, int c) {
 template <int kDP, typename Store, typename StoreLse>
 __device__ __forceinline__ void cluster_join(const float* o, const float* lse, int rows, int D,
                                              int pieces, Store store, StoreLse store_lse) {
+  __syncwarp();  // an aligned barrier
   cluster_sync_all();
   const int chunks = D / 4;
   const uint32_t o0 = smem_u32(o), lse0 = smem_u32(lse);
