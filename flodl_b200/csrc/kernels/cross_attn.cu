@@ -920,41 +920,56 @@ struct Stride3 {
 // queries' kernel instead, from tiles of O and its remainders, they cost a kernel
 // less, but a training step of 64 x 8 heads, 256 x 256 x 64, took 108 us instead of 101.)
 __host__ __device__ constexpr int stat_pitch(int Sq) { return (Sq + 63) / 64 * 64; }
+// Bound by the bytes of dO, O and its remainders (which the forward leaves in L2 where
+// they fit). kLanes lanes take a row; two rows of each are in flight, and indexes are 32
+// bits (64-bit divisions for every row took 10.6 instead of 7.3 us on 64 x 8 heads,
+// 256 rows of 64; 19.9 instead of 13.4 on 4 x 16 heads, 2048 rows of 128).
+constexpr int kRowsAhead = 2;
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) cross_stats_kernel(const T* __restrict__ out,
                                                           const T* __restrict__ out_res,
                                                           const T* __restrict__ dout, Stride3 ds,
                                                           const float* __restrict__ lse2,
                                                           float2* __restrict__ stats, int B, int Sq,
-                                                          int H, int D) {
+                                                          FastDiv by_heads, int D) {
   pdl_wait();
   pdl_trigger();
   constexpr int kPer = 256 / kLanes;
   const int part = threadIdx.x % kLanes, sub = threadIdx.x / kLanes;
-  const int pitch = stat_pitch(Sq);
-  const int64_t rows = (int64_t)B * pitch * H;
-  for (int64_t base = (int64_t)blockIdx.x * kPer; base < rows; base += (int64_t)gridDim.x * kPer) {
-    const int64_t row = base + sub;  // (b * pitch + i) * H + h
-    const int64_t bi = row / H;
-    const int h = (int)(row - bi * H);
-    const int64_t b = bi / pitch;
-    const int i = (int)(bi - b * pitch);
-    float s = 0.f;
-    if (row < rows && i < Sq && part * 8 < D) {
-      const int64_t at = ((b * Sq + i) * H + h) * D + part * 8;
-      const uint4 g =
-          __ldg(reinterpret_cast<const uint4*>(dout + b * ds.b + i * ds.s + h * ds.h + part * 8));
-      s = dot8<T>(__ldg(reinterpret_cast<const uint4*>(out + at)), g);
-      // with what O's rounding left off: in a row that one key dominates, dP and
-      // delta nearly cancel, and the rounding of O would be the largest error
-      if (out_res != nullptr) s += dot8<T>(__ldg(reinterpret_cast<const uint4*>(out_res + at)), g);
-    }
+  const int pitch = stat_pitch(Sq), H = by_heads.d;
+  const uint32_t rows = (uint32_t)pitch * H;  // of a sample
+  const bool mine = part * 8 < D;
+  for (int b = blockIdx.y; b < B; b += gridDim.y)
+    for (uint32_t base = blockIdx.x * (kPer * kRowsAhead); base < rows;
+         base += gridDim.x * (kPer * kRowsAhead)) {
+      uint4 g[kRowsAhead], o[kRowsAhead], r[kRowsAhead];
+      uint32_t i[kRowsAhead], h[kRowsAhead];
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (row < rows && part == 0)
-      stats[(b * H + h) * pitch + i] =
-          make_float2(i < Sq ? -__ldg(lse2 + (b * H + h) * Sq + i) : -INFINITY, -s);
-  }
+      for (int k = 0; k < kRowsAhead; ++k) {
+        const uint32_t row = base + k * kPer + sub;  // i * H + h
+        i[k] = by_heads.div(row);
+        h[k] = row - i[k] * H;
+        g[k] = o[k] = r[k] = make_uint4(0, 0, 0, 0);
+        if (i[k] < (uint32_t)Sq && mine) {
+          const int64_t at = (((int64_t)b * Sq + i[k]) * H + h[k]) * D + part * 8;
+          g[k] = __ldg(reinterpret_cast<const uint4*>(dout + b * ds.b + i[k] * ds.s + h[k] * ds.h +
+                                                      part * 8));
+          o[k] = __ldg(reinterpret_cast<const uint4*>(out + at));
+          r[k] = __ldg(reinterpret_cast<const uint4*>(out_res + at));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kRowsAhead; ++k) {
+        // with what O's rounding left off: in a row that one key dominates, dP and
+        // delta nearly cancel, and the rounding of O would be the largest error
+        float s = dot8<T>(o[k], g[k]) + dot8<T>(r[k], g[k]);
+#pragma unroll
+        for (int x = kLanes / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+        if (part == 0 && i[k] < (uint32_t)pitch)
+          stats[((int64_t)b * H + h[k]) * pitch + i[k]] = make_float2(
+              i[k] < (uint32_t)Sq ? -__ldg(lse2 + ((int64_t)b * H + h[k]) * Sq + i[k]) : -INFINITY, -s);
+      }
+    }
 }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
@@ -1811,14 +1826,18 @@ cudaError_t run_bwd_half(const CrossAttnArgs& a, const CrossSplits& plan, cudaSt
 
 template <typename T>
 cudaError_t run_stats(const CrossAttnArgs& a, cudaStream_t st) {
-  const int64_t rows = (int64_t)a.B * stat_pitch(a.Sq) * a.H;
-  const int per = a.D <= 64 ? 32 : 16;
-  const dim3 grid((unsigned)std::min<int64_t>((rows + per - 1) / per, num_sms() * 16ll));
+  const int64_t rows = (int64_t)stat_pitch(a.Sq) * a.H;  // of a sample
+  if (rows >= kMaxFlatIndex - (1 << 24)) return cudaErrorInvalidValue;  // (over 170 GB of tensors)
+  const int per = (a.D <= 64 ? 32 : 16) * kRowsAhead;
+  const int64_t x = std::min<int64_t>((rows + per - 1) / per, num_sms() * 16ll);
+  const int64_t y = std::min<int64_t>({a.B, std::max<int64_t>(1, num_sms() * 16ll / x), 65535});
+  const dim3 grid((unsigned)x, (unsigned)y);
   const Stride3 ds{a.do_st[0], a.do_st[1], a.do_st[2]};
   auto k = a.D <= 64 ? cross_stats_kernel<T, 8> : cross_stats_kernel<T, 16>;
   cudaError_t e = launch_pdl(k, grid, dim3(256), 0, st, (const T*)a.out,
                              (const T*)a.out_res, (const T*)a.dout, ds,
-                             (const float*)a.lse2, (float2*)a.stats, a.B, a.Sq, a.H, a.D);
+                             (const float*)a.lse2, (float2*)a.stats, a.B, a.Sq, FastDiv((uint32_t)a.H),
+                             a.D);
   if (e != cudaSuccess) return e;
   note_launch();
   return cudaGetLastError();
