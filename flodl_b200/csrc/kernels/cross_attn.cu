@@ -1917,7 +1917,8 @@ cudaError_t launch_cross_attn_fwd(const CrossAttnArgs& a, cudaStream_t st) {
 }
 
 cudaError_t launch_cross_attn_bwd(const CrossAttnArgs& a, cudaStream_t st) {
-  if (bad_shape(a) || !a.lse2 || !a.out_res || !a.stats || !a.dk != !a.dv || (a.key_pad && (!a.words || !a.vis_end)))
+  if (bad_shape(a) || !a.lse2 || !a.out_res || !a.stats || !a.dk != !a.dv ||
+      (a.key_pad && (!a.words || !a.vis_end)))
     return cudaErrorInvalidValue;
   if (a.D <= 64) return a.half ? run_bwd<__half, 64>(a, st) : run_bwd<__nv_bfloat16, 64>(a, st);
   return a.half ? run_bwd<__half, 128>(a, st) : run_bwd<__nv_bfloat16, 128>(a, st);
