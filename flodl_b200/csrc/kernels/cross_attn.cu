@@ -1630,6 +1630,8 @@ cudaError_t cross_attn_opt_in(const void* kernel, size_t smem, std::atomic<uint6
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                              cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess)  // clusters of more than 8 CTAs
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess) done.fetch_or(bit);
   return e;
 }
@@ -1642,6 +1644,7 @@ int64_t cross_attn_clusters(const void* kernel, int threads, size_t smem, int si
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                          cudaSharedmemCarveoutMaxShared);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = size;
@@ -1714,21 +1717,21 @@ CrossSplits fwd_splits(const CrossAttnArgs& a) {
   const int want = pieces(items, (int64_t)kFwdCtas * num_sms(), tiles);
   // as many as a cluster joins and the GPU holds at once (98 items of 128 x 1500 x 64:
   // 21 us with two pieces each, 27 with three and a second kernel)
-  int s = std::min(want, kCrossCluster);
+  int s = std::min(want, kCrossTileCluster);
   while (s > 1 && items > (a.D > 64 ? fwd_clusters<128>(s) : fwd_clusters<64>(s))) --s;
-  if (cross_attn_joins_more(items, s, want, tiles, num_sms())) return {want, false};
+  if (cross_attn_joins_more(items, s, kCrossTileCluster, want, tiles, num_sms())) return {want, false};
   return {s, s > 1};
 }
 // Both halves of the backward have one CTA per SM.
 CrossSplits bwd_splits(int64_t items, int64_t tiles) {
   static CrossFits fits{};
   const int want = pieces(items, num_sms(), tiles);
-  int s = std::min(want, kCrossCluster);
+  int s = std::min(want, kCrossTileCluster);
   using G = BwdGeo<64, true, 2>;
   while (s > 1 && items > cross_attn_clusters((const void*)cross_bwd_kernel<__nv_bfloat16, 64, true, 2, true>,
                                               G::kThreads, sizeof(BwdSmem<64, true, 2>) + 1024, s, fits))
     --s;
-  if (cross_attn_joins_more(items, s, want, tiles, num_sms())) return {want, false};
+  if (cross_attn_joins_more(items, s, kCrossTileCluster, want, tiles, num_sms())) return {want, false};
   return {s, s > 1};
 }
 CrossSplits dq_splits(const CrossAttnArgs& a) {

@@ -41,7 +41,12 @@ struct CrossAttnArgs {
 
 constexpr int kCrossFewRows = 16;  // query rows per memory head of the few-row form
 
-constexpr int kCrossCluster = 8;   // pieces of a split key axis that a cluster joins
+// Pieces of a split axis that a cluster joins, at most: of the few-row form (one sample's
+// 8 heads x 8192 x 64 8.6 us, 9.4 with 8; 16 memory heads x 32768 x 128 45.6, 49.5 with 8
+// or a second kernel), and of the others, whose CTAs are larger (100 x 4000 x 128, 8
+// heads: 17 us with 16, 13.2 with 8).
+constexpr int kCrossCluster = 16;
+constexpr int kCrossTileCluster = 8;
 
 // Whether the forward takes the few-row form: all query rows of a memory head
 // (Sq * H / Hk) fit one 16-row tensor-core tile.
@@ -69,13 +74,14 @@ struct CrossSplits {
   bool joined() const { return n > 1 && !clustered; }
 };
 CrossSplits cross_attn_few_splits(const CrossAttnArgs& a);
-// Whether `want` pieces of a key axis of `tiles`, joined by a second kernel, beat the s
-// that a cluster joins. That kernel costs 3 to 4 us, a tile about 0.5 (64 keys, a CTA
-// to itself): where the s leave SMs idle and more than five tiles a piece go. (16 heads
-// x 128 rows x 64 columns each way, pieces 8 and 15 to 18: 13.6 us joined by
+// Whether `want` pieces of an axis of `tiles`, joined by a second kernel, beat the s that
+// a cluster joins (at most `most`). That kernel costs 3 to 4 us, a tile about 0.5 (64
+// keys, a CTA to itself): where the s leave SMs idle and more than five tiles a piece
+// go. (16 heads x 128 rows x 64 columns, pieces 8 and 15 to 18: 13.6 us joined by
 // clusters and 14.3 by a kernel at 4001 keys, 42 and 29 at 20000.)
-inline bool cross_attn_joins_more(int64_t items, int64_t s, int64_t want, int64_t tiles, int sms) {
-  return want > kCrossCluster && items * s < sms && tiles / s - tiles / want > 5;
+inline bool cross_attn_joins_more(int64_t items, int64_t s, int64_t most, int64_t want,
+                                  int64_t tiles, int sms) {
+  return want > most && items * s < sms && tiles / s - tiles / want > 5;
 }
 // Clusters of `size` CTAs of a kernel that the GPU holds at once (`fits`: a cache of
 // the kernel's own; a cluster's CTAs share a part of the GPU, so that fewer CTAs fit

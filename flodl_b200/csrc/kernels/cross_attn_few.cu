@@ -17,11 +17,10 @@
 // the tensor pipe is not the limit. (A first version loaded the fragments
 // straight from global memory: 680 instructions per 16 keys, 2.5 TB/s.)
 // The key axis is split over CTAs until the SMs are covered; the pieces are
-// joined by their lse, in a fixed order, by a cluster of up to eight CTAs through
+// joined by their lse, in a fixed order, by a cluster of up to sixteen CTAs through
 // distributed shared memory or by a second kernel. Measured (one query per head, bf16): 512
 // heads x 4096 x 64 in 86.7 us, 6.2 TB/s (0.96 of a copy's rate); 384 padded heads x
-// 512 x 64 in 8.4; 16 memory heads x 32768 x 128 (64 query heads) in 49, 5.5 TB/s with
-// its join; one sequence's 8 heads x 100 in 2.8, a launch. (17 to 64 rows as two to
+// 512 x 64 in 8.4; 16 memory heads x 32768 x 128 (64 query heads) in 45.6, 5.9 TB/s; one sequence's 8 heads x 100 in 2.8, a launch. (17 to 64 rows as two to
 // four groups of 16, a warp to each: 21 us at 37 rows x 4001 keys of 16 heads, where
 // the 128-row tiles of tcgen05 take 13.)
 #include "sm100_ptx.cuh"
@@ -561,7 +560,7 @@ CrossSplits cross_attn_few_splits(const CrossAttnArgs& a) {
   // by a second kernel)
   int64_t s = std::min<int64_t>(want, kCrossCluster);
   while (s > 1 && units > (a.D > 64 ? few_clusters<128>((int)s) : few_clusters<64>((int)s))) --s;
-  if (s < least || cross_attn_joins_more(units, s, want, tiles, num_sms()))
+  if (s < least || cross_attn_joins_more(units, s, kCrossCluster, want, tiles, num_sms()))
     return {(int)std::max<int64_t>(least, want), false};
   return {(int)std::max<int64_t>(1, s), s > 1};
 }

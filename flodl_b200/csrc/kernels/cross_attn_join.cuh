@@ -16,6 +16,8 @@
 
 namespace flodl {
 
+constexpr int kAhead = 8;  // pieces in flight
+
 // Offset (in floats) of columns 4c..4c+3 of row r: 16-byte chunks rotated by the row, so
 // that rows written by a lane each do not meet in the same banks.
 template <int kDP>
@@ -36,31 +38,37 @@ __device__ __forceinline__ void cluster_join(const float* o, const float* lse, i
   for (int i = cluster_ctarank() * blockDim.x + threadIdx.x; i < rows * chunks;
        i += pieces * blockDim.x) {
     const int r = i / chunks, c = i - r * chunks;
-    float ls[kCrossCluster];
-    float4 v[kCrossCluster];
-#pragma unroll
-    for (int p = 0; p < kCrossCluster; ++p) {
-      ls[p] = -INFINITY;
-      v[p] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (p < pieces) {
-        ls[p] = ld_cluster(lse0 + 4 * r, p);
-        v[p] = ld_cluster4(o0 + 4 * piece_at<kDP>(r, c), p);
-      }
-    }
-    float top = ls[0];
-#pragma unroll
-    for (int p = 1; p < kCrossCluster; ++p) top = fmaxf(top, ls[p]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float w = 0.f;
+    float top = -INFINITY, w = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int p0 = 0; p0 < pieces; p0 += kAhead) {
+      float ls[kAhead];
+      float4 v[kAhead];
 #pragma unroll
-    for (int p = 0; p < kCrossCluster; ++p) {
-      const float f = exp2f(ls[p] - base);
-      w += f;
-      a.x = fmaf(v[p].x, f, a.x);
-      a.y = fmaf(v[p].y, f, a.y);
-      a.z = fmaf(v[p].z, f, a.z);
-      a.w = fmaf(v[p].w, f, a.w);
+      for (int p = 0; p < kAhead; ++p) {
+        ls[p] = -INFINITY;
+        v[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p0 + p < pieces) {
+          ls[p] = ld_cluster(lse0 + 4 * r, p0 + p);
+          v[p] = ld_cluster4(o0 + 4 * piece_at<kDP>(r, c), p0 + p);
+        }
+      }
+      const float before = top;
+#pragma unroll
+      for (int p = 0; p < kAhead; ++p) top = fmaxf(top, ls[p]);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float f0 = exp2f(before - base);
+      w *= f0;
+      a = make_float4(a.x * f0, a.y * f0, a.z * f0, a.w * f0);
+#pragma unroll
+      for (int p = 0; p < kAhead; ++p) {
+        const float f = exp2f(ls[p] - base);
+        w += f;
+        a.x = fmaf(v[p].x, f, a.x);
+        a.y = fmaf(v[p].y, f, a.y);
+        a.z = fmaf(v[p].z, f, a.z);
+        a.w = fmaf(v[p].w, f, a.w);
+      }
     }
     // no visible key: zeros. A NaN sum (NaN scores) passes through.
     const bool none = w == 0.f;
@@ -80,15 +88,18 @@ __device__ __forceinline__ void cluster_sum(const float* o, int rows, int D, int
   for (int i = cluster_ctarank() * blockDim.x + threadIdx.x; i < rows * chunks;
        i += pieces * blockDim.x) {
     const int r = i / chunks, c = i - r * chunks;
-    float4 v[kCrossCluster];
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int p0 = 0; p0 < pieces; p0 += kAhead) {
+      float4 v[kAhead];
 #pragma unroll
-    for (int p = 0; p < kCrossCluster; ++p)
-      v[p] = p < pieces ? ld_cluster4(o0 + 4 * piece_at<kDP>(r, c), p)
-                        : make_float4(0.f, 0.f, 0.f, 0.f);
-    float4 a = v[0];
+      for (int p = 0; p < kAhead; ++p)
+        v[p] = p0 + p < pieces ? ld_cluster4(o0 + 4 * piece_at<kDP>(r, c), p0 + p)
+                               : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int p = 1; p < kCrossCluster; ++p)
-      a = make_float4(a.x + v[p].x, a.y + v[p].y, a.z + v[p].z, a.w + v[p].w);
+      for (int p = 0; p < kAhead; ++p)
+        a = make_float4(a.x + v[p].x, a.y + v[p].y, a.z + v[p].z, a.w + v[p].w);
+    }
     store(r, c, a);
   }
 }
