@@ -7,6 +7,8 @@ use of a GPU op), never a silent fallback to eager PyTorch.
 from __future__ import annotations
 
 import importlib
+import pathlib
+import re
 
 _C = None
 _C_ERR: Exception | None = None
@@ -42,3 +44,16 @@ def native():
             f"{_NATIVE_ERR!r}. Run `python setup.py build_ext --inplace`."
         )
     return _native
+
+
+def missing_names() -> list[str]:
+    """Names that the package's modules call in the extensions and that these do
+    not export (an extension of another version of the package)."""
+    missing = set()
+    for path in pathlib.Path(__file__).parent.rglob("*.py"):
+        text = path.read_text()
+        for pattern, ext in ((r"\b(?:C|cuda_ext)\(\)\.(\w+)", cuda_ext), (r"\bnative\(\)\.(\w+)", native)):
+            for name in re.findall(pattern, text):
+                if not hasattr(ext(), name):
+                    missing.add(f"{ext().__name__}.{name} ({path.name})")
+    return sorted(missing)

@@ -10,11 +10,14 @@ Two extensions:
   balancer, CPU averaging reducer and the batch prefetcher.
 
 Usage: ``python setup.py build_ext --inplace -t /tmp/flodl_b200_build`` (``__graft_entry__.build()`` runs
-exactly this).
+exactly this). Objects are kept per tree under the ``-t`` directory and reused only while what they were
+compiled from is the same, whatever the files' times say.
 """
 import glob
+import hashlib
 import os
 
+import torch
 from setuptools import setup
 from torch.utils.cpp_extension import BuildExtension, CppExtension, CUDAExtension
 
@@ -83,10 +86,60 @@ ext_modules = [
     ),
 ]
 
+def _digest(*parts):
+    h = hashlib.sha256()
+    for p in parts:
+        h.update(len(p).to_bytes(8, "little") + p)
+    return h.hexdigest()
+
+
+def _read(path):
+    with open(path, "rb") as f:
+        return f.read()
+
+
+class Build(BuildExtension.with_options(use_ninja=True)):
+    """Objects by content.
+
+    ninja compares modification times only: where another version of the tree
+    was built at this path before, and the files here carry older times (a
+    commit's, as archives and time-preserving copies keep them), it would link
+    the other version's objects. So every object has a key beside it, of its
+    source, of all headers and of the toolkit, and one whose key differs is
+    removed first. Trees do not share a directory.
+    """
+
+    def finalize_options(self):
+        super().finalize_options()
+        self.build_temp = os.path.join(self.build_temp,
+                                       "tree-" + _digest(os.path.realpath(ROOT).encode())[:16])
+
+    def build_extension(self, ext):
+        headers = sorted(f for f in glob.glob(os.path.join(CSRC, "**", "*"), recursive=True)
+                         if os.path.isfile(f) and not f.endswith((".cpp", ".cu")))
+        common = [f"{torch.__version__} {torch.version.cuda}".encode()]
+        for f in headers:
+            common += [f.encode(), _read(f)]
+        common = _digest(*common).encode()
+        keys = {}
+        for src in ext.sources:
+            obj = os.path.join(self.build_temp, os.path.splitext(src)[0] + ".o")
+            keys[obj] = _digest(common, src.encode(), _read(src)).encode()
+            known = os.path.exists(obj + ".key") and _read(obj + ".key") == keys[obj]
+            if os.path.exists(obj) and not known:
+                os.remove(obj)
+        super().build_extension(ext)
+        for obj, key in keys.items():
+            if not os.path.exists(obj):
+                raise RuntimeError(f"{obj} was not built")
+            with open(obj + ".key", "wb") as f:
+                f.write(key)
+
+
 setup(
     name="flodl_b200",
     version="0.1.0",
     packages=["flodl_b200"],
     ext_modules=ext_modules,
-    cmdclass={"build_ext": BuildExtension.with_options(use_ninja=True)},
+    cmdclass={"build_ext": Build},
 )
