@@ -231,6 +231,7 @@ __device__ __forceinline__ void zero_hidden_rows(uint8_t* tile, uint2 words, int
     }
   }
   fence_proxy_async_shared();
+  __syncwarp();  // the caller's next TMEM instruction is aligned
 }
 
 // Sixteen columns of a row that lies in TMEM from t on, times f (`use` false:
@@ -302,21 +303,21 @@ __device__ __forceinline__ void store_row(uint32_t t, int D, bool there, bool us
   for (int c = 0; c < D; c += 16) {
     float v[16];
     row16(t + c, there, use, f, v);
-    if (!row) continue;
-    if (part == nullptr) {
+    if (row && part == nullptr) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         if (c + 8 * h < D) {
           *reinterpret_cast<uint4*>(out + c + 8 * h) = pack8<T, false>(v + 8 * h);
           if (res != nullptr) *reinterpret_cast<uint4*>(res + c + 8 * h) = pack8<T, true>(v + 8 * h);
         }
-    } else {
+    } else if (row) {
 #pragma unroll
       for (int h = 0; h < 4; ++h)
         if (c + 4 * h < D)
           *reinterpret_cast<float4*>(part + c + 4 * h) =
               make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
     }
+    __syncwarp();  // a tile may end inside a warp: the next TMEM load is aligned
   }
 }
 
@@ -825,9 +826,11 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas)
         else if (kTrain)
           lse2[lrow] = none ? INFINITY : m_ref + log2f(l);
       }
+      __syncwarp();
       tc_fence_before();
     }
     if (lane == 0) bulk_wait_group<0>();
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -1507,6 +1510,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       }
     }
     if (lane == 0) bulk_wait_group<0>();
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();

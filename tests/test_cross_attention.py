@@ -291,6 +291,17 @@ def test_gpu_split_keys(shape, mask):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 96])
+@pytest.mark.parametrize("rows", [17, 45, 100, 129])
+def test_gpu_row_tiles_that_end_inside_a_warp(rows, D):
+    # pieces of long axes that a second kernel joins (their rows are stored lane by
+    # lane), and hidden keys in tiles of every kernel
+    check("cuda", torch.bfloat16, 1, rows, 1, 1, 16000, D, mask="scattered")
+    check("cuda", torch.bfloat16, 1, 9000, 1, 1, rows, D, mask="scattered")
+    check("cuda", torch.float16, 3, rows, 2, 1, 200, D, mask="scattered")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("mask", ["right", "left", "scattered", "empty", "one"])
 def test_gpu_tiles_masks(mask, dtype):
