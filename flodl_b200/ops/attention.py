@@ -71,7 +71,7 @@ def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, causal: bool = F
     """Self-attention over packed ``qkv [B*S, 3C]``; returns ``[B*S, C]``.
 
     ``key_padding`` (bool ``[B, S]``, True = masked key) implements the padding
-    mask used by BERT-style encoders.
+    mask used by BERT-style encoders; with ``causal`` both apply.
     """
     if not use_kernels(qkv):
         D = qkv.shape[1] // (3 * H)
@@ -79,6 +79,8 @@ def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, causal: bool = F
         mask = None
         if key_padding is not None:
             mask = ~key_padding[:, None, None, :]
+            if causal:
+                mask = mask & torch.ones(S, S, dtype=torch.bool, device=qkv.device).tril()
         o = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, is_causal=causal and mask is None)
         return o.permute(0, 2, 1, 3).reshape(B * S, H * D)
     q16 = qkv if qkv.dtype == torch.bfloat16 else qkv.to(torch.bfloat16)

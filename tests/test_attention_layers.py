@@ -84,6 +84,19 @@ def test_cpu_self_attention(kind, causal):
         torch.testing.assert_close(m(x, key_padding_mask=pad), plain(m, x, pad=pad), rtol=1e-5, atol=1e-5)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_cpu_causal_with_padding(kind):
+    """Both masks at once: right padding, left padding (rows that see no key), all hidden."""
+    m = layer(kind, causal=True)
+    x = torch.randn(3, 7, 32)
+    pad = torch.tensor([[False] * 5 + [True] * 2, [True] * 3 + [False] * 4, [True] * 7])
+    y = m(x, key_padding_mask=pad)
+    torch.testing.assert_close(y, plain(m, x, pad=pad), rtol=1e-5, atol=1e-5)
+    later = x.clone()
+    later[:, 4:] += 1.0  # what comes after a query has no effect on it
+    torch.testing.assert_close(m(later, key_padding_mask=pad)[:, :4], y[:, :4], rtol=0, atol=0)
+
+
 @pytest.mark.parametrize("kind", ["plain", "norm"])
 def test_cpu_cross_attention_and_serving_form(kind):
     m = layer(kind)
