@@ -225,6 +225,21 @@ def test_gpu_self_attention(kind, causal, C, H):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("C,H", [(256, 4), (192, 2), (160, 4), (256, 2), (60, 3), (320, 2)])
+def test_gpu_plain_self_attention(causal, C, H):
+    """Head sizes 64, 96, 40, 128, and those that no kernel takes (20, 160)."""
+    m = layer("plain", C, H, causal, "cuda")
+    x = torch.randn(3, 150, C, device="cuda")
+    compare(m, lambda a: m(a), lambda a: plain(m, a), [x])
+    at = torch.arange(150, device="cuda")[None, :]
+    pad = at >= torch.tensor([150, 70, 3], device="cuda")[:, None]
+    compare(m, lambda a: m(a, key_padding_mask=pad), lambda a: plain(m, a, pad=pad), [x])
+    pad = at < torch.tensor([0, 70, 150], device="cuda")[:, None]  # rows that see no key
+    compare(m, lambda a: m(a, key_padding_mask=pad), lambda a: plain(m, a, pad=pad), [x])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["plain", "norm"])
 @pytest.mark.parametrize("C,H,S,Sm", [(256, 4, 40, 170), (192, 2, 130, 90), (160, 4, 1, 300), (512, 8, 300, 300)])
 def test_gpu_cross_attention(kind, C, H, S, Sm):
