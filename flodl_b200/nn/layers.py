@@ -592,6 +592,14 @@ class LSTMCell(Module):
 
 
 # ---------------------------------------------------------------- attention
+def _mask_of(mask, batch: int, keys: int):
+    """A padding mask shared by the samples (or by a sample's keys), as ``[batch, keys]``."""
+    if (mask is not None and mask.dim() == 2 and mask.shape[0] in (1, batch)
+            and mask.shape[1] in (1, keys)):
+        return mask.expand(batch, keys).contiguous()
+    return mask  # the operators refuse other shapes
+
+
 class MultiheadAttention(NamedInputModule):
     """Multi-head attention (flodl/src/nn/attention.rs:28,136-230).
 
@@ -633,7 +641,8 @@ class MultiheadAttention(NamedInputModule):
         return self.attend(x, memory)
 
     def forward(self, x, refs=None, key_padding_mask=None, positions=None):
-        """``positions`` (int64 ``[B, S]``) are the rotary positions of a batch
+        """``key_padding_mask`` (bool, True = hidden key) is ``[B, keys]``, or ``[1, keys]``
+        for all samples. ``positions`` (int64 ``[B, S]``) are the rotary positions of a batch
         whose sequences do not start at 0 (left padding)."""
         if isinstance(refs, torch.Tensor):
             return self.attend(x, refs, key_padding_mask, positions)
@@ -655,6 +664,7 @@ class MultiheadAttention(NamedInputModule):
         H = self.num_heads
         if positions is not None and (memory is not None or self.rotary is None):
             raise ValueError("positions need self-attention with a rotary embedding")
+        key_padding_mask = _mask_of(key_padding_mask, B, S if memory is None else memory.shape[1])
         if memory is not None:
             q, kv = ops.cross_projection(x, memory, self.qkv.weight, self.qkv.bias)
             o = self._cross(x, q, kv, key_padding_mask, self.causal and S == memory.shape[1])
@@ -685,7 +695,7 @@ class MultiheadAttention(NamedInputModule):
         :meth:`project_memory`'s result."""
         B, S, Cd = x.shape
         q = ops.project_rows(x, self.qkv.weight, self.qkv.bias, 0, self.embed_dim)
-        o = self._cross(x, q, memory_kv, key_padding_mask)
+        o = self._cross(x, q, memory_kv, _mask_of(key_padding_mask, B, memory_kv.shape[1]))
         return self.out_proj(o).reshape(B, S, Cd).to(x.dtype)
 
 

@@ -111,6 +111,34 @@ def test_cpu_cross_attention_and_serving_form(kind):
     assert not kv.requires_grad and not steps[0].requires_grad
 
 
+def shared_masks(device):
+    """One mask for all samples, and one flag for all keys of a sample."""
+    x, mem = torch.randn(2, 3, 32, device=device), torch.randn(2, 9, 32, device=device)
+    for kind in KINDS:
+        m = layer(kind, device=device)
+        for y, keys in ((None, 3), (mem, 9)):
+            one = torch.zeros(1, keys, dtype=torch.bool, device=device)
+            one[0, 2] = True
+            flags = torch.tensor([[False], [True]], device=device)
+            for mask in (one, flags):
+                full = mask.expand(2, keys).contiguous()
+                assert torch.equal(m(x, y, key_padding_mask=mask), m(x, y, key_padding_mask=full))
+                if y is not None:
+                    kv = m.project_memory(y)
+                    assert torch.equal(m.attend_memory(x[:, :1], kv, mask), m.attend_memory(x[:, :1], kv, full))
+        with pytest.raises(ValueError):
+            m(x, mem, key_padding_mask=torch.zeros(2, 4, dtype=torch.bool, device=device))
+
+
+def test_cpu_masks_shared_by_the_batch():
+    shared_masks("cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_masks_shared_by_the_batch():
+    shared_masks("cuda")
+
+
 @pytest.mark.parametrize("kind", ["plain", "both"])
 def test_cpu_gradients_by_differences(kind):
     m = layer(kind, C=8, H=2).double()
