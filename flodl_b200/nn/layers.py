@@ -648,15 +648,16 @@ class MultiheadAttention(NamedInputModule):
             return self.attend(x, refs, key_padding_mask, positions)
         return self.attend(x, next(iter(refs.values())) if refs else None, key_padding_mask, positions)
 
-    def _cross(self, x, q, kv, key_padding_mask, causal=False):
+    def _cross(self, x, q, kv, key_padding_mask, causal=False, normed_keys=False):
         B, S, Cd = x.shape
         H = self.num_heads
         q = q.view(B, S, H, Cd // H)
         kv = kv.view(B, kv.shape[1], 2, H, Cd // H)
         if self.q_norm is not None:
-            k = ops.rms_norm(kv[:, :, 0], self.k_norm.weight, self.k_norm.eps)
             q = ops.rms_norm(q, self.q_norm.weight, self.q_norm.eps)
-            return ops.cross_attention(q, k, kv[:, :, 1], key_padding_mask, causal).view(B * S, Cd)
+            if not normed_keys:
+                k = ops.rms_norm(kv[:, :, 0], self.k_norm.weight, self.k_norm.eps)
+                return ops.cross_attention(q, k, kv[:, :, 1], key_padding_mask, causal).view(B * S, Cd)
         return ops.cross_attention_packed(q, kv, key_padding_mask, causal).view(B * S, Cd)
 
     def attend(self, x, memory=None, key_padding_mask=None, positions=None):
@@ -684,10 +685,14 @@ class MultiheadAttention(NamedInputModule):
 
     @torch.no_grad()
     def project_memory(self, memory):
-        """Keys and values ``[B, Sm, 2C]`` of a memory, for :meth:`attend_memory`
-        at every step of serving (no gradients)."""
+        """Keys (normed, with ``qk_norm``) and values ``[B, Sm, 2C]`` of a memory, for
+        :meth:`attend_memory` at every step of serving (no gradients)."""
         n = self.embed_dim
-        return ops.project_rows(memory, self.qkv.weight, self.qkv.bias, n, 3 * n)
+        kv = ops.project_rows(memory, self.qkv.weight, self.qkv.bias, n, 3 * n)
+        if self.k_norm is not None:
+            k = kv.unflatten(-1, (2, self.num_heads, n // self.num_heads))[..., 0, :, :]
+            k.copy_(ops.rms_norm(k, self.k_norm.weight, self.k_norm.eps))
+        return kv
 
     @torch.no_grad()
     def attend_memory(self, x, memory_kv, key_padding_mask=None):
@@ -695,7 +700,8 @@ class MultiheadAttention(NamedInputModule):
         :meth:`project_memory`'s result."""
         B, S, Cd = x.shape
         q = ops.project_rows(x, self.qkv.weight, self.qkv.bias, 0, self.embed_dim)
-        o = self._cross(x, q, memory_kv, _mask_of(key_padding_mask, B, memory_kv.shape[1]))
+        o = self._cross(x, q, memory_kv, _mask_of(key_padding_mask, B, memory_kv.shape[1]),
+                        normed_keys=True)
         return self.out_proj(o).reshape(B, S, Cd).to(x.dtype)
 
 

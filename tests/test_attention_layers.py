@@ -111,6 +111,31 @@ def test_cpu_cross_attention_and_serving_form(kind):
     assert not kv.requires_grad and not steps[0].requires_grad
 
 
+def norms_once(device, monkeypatch):
+    """A step over a projected memory norms the new queries only."""
+    m = layer("norm", device=device)
+    x, mem = torch.randn(2, 1, 32, device=device), torch.randn(2, 90, 32, device=device)
+    with torch.no_grad():
+        want = m(x, mem)
+    sizes, rms_norm = [], ops.rms_norm
+    monkeypatch.setattr(ops, "rms_norm", lambda t, *a: (sizes.append(t.numel()), rms_norm(t, *a))[1])
+    kv = m.project_memory(mem)
+    assert sizes == [mem.numel()]
+    y = m.attend_memory(x, kv)
+    assert sizes[1:] == [x.numel()]
+    # the same values in the same kernels; only the library's small products may differ
+    torch.testing.assert_close(y, want, rtol=0, atol=4 * T * float(want.abs().max()) if x.is_cuda else 1e-5)
+
+
+def test_cpu_serving_norms_the_memory_once(monkeypatch):
+    norms_once("cpu", monkeypatch)
+
+
+@pytest.mark.gpu
+def test_gpu_serving_norms_the_memory_once(monkeypatch):
+    norms_once("cuda", monkeypatch)
+
+
 def shared_masks(device):
     """One mask for all samples, and one flag for all keys of a sample."""
     x, mem = torch.randn(2, 3, 32, device=device), torch.randn(2, 9, 32, device=device)
