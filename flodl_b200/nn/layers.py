@@ -728,16 +728,20 @@ class RotaryEmbedding(Module):
 
     def rotate(self, x, positions=None):
         """The first ``dim`` values of each head of ``x [B, H, S, D]``, turned by
-        positions 0.. or ``positions [B, S]``; the others as they are."""
-        R = 2 * self.cos.shape[1]
+        positions 0.. or ``positions [B, S]``; the others as they are. Tables and
+        products are f32 whatever the type of ``x``, and rounded once."""
+        R, rows, S = 2 * self.cos.shape[1], self.cos.shape[0], x.shape[2]
         if positions is None:
-            y = self.forward(x[..., :R])
+            if S > rows:
+                raise ValueError(f"positions 0 to {S - 1} are outside the tables' {rows} rows")
+            cos, sin = self.cos[:S], self.sin[:S]
         else:
-            if positions.dtype != torch.int64 or positions.shape != (x.shape[0], x.shape[2]) or \
+            if positions.dtype != torch.int64 or positions.shape != (x.shape[0], S) or \
                     positions.device != x.device:
-                raise ValueError(f"positions must be int64 {[x.shape[0], x.shape[2]]} on {x.device}")
-            cos, sin = (t[:, None].to(x.dtype)
-                        for t in ops.norm.rotary_rows(self.cos, self.sin, positions))
-            x1, x2 = x[..., 0:R:2], x[..., 1:R:2]
-            y = torch.stack((x1 * cos - x2 * sin, x1 * sin + x2 * cos), dim=-1).flatten(-2)
+                raise ValueError(f"positions must be int64 {[x.shape[0], S]} on {x.device}")
+            cos, sin = (t[:, None] for t in ops.norm.rotary_rows(self.cos, self.sin, positions))
+        work = torch.float64 if x.dtype == torch.float64 else torch.float32
+        cos, sin = cos.to(work), sin.to(work)
+        x1, x2 = x[..., 0:R:2].to(work), x[..., 1:R:2].to(work)
+        y = torch.stack((x1 * cos - x2 * sin, x1 * sin + x2 * cos), dim=-1).flatten(-2).to(x.dtype)
         return torch.cat((y, x[..., R:]), -1) if R < x.shape[-1] else y

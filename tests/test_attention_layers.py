@@ -396,6 +396,27 @@ def test_rotary_positions_are_checked():
             rope.rotate(x, bad)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rotary_rounds_once(dtype):
+    """Off from the tables' rotation by half a step of the type, and for the two
+    products and their sum in f32 by 2 u of their magnitudes."""
+    rope = RotaryEmbedding(32, 4096)
+    x = torch.randn(2, 3, 700, 40).to(dtype)
+    at = torch.randint(0, 4096, (2, 700))
+    for pos in (None, at):
+        rows = pos if pos is not None else torch.arange(700).expand(2, 700)
+        c, s = rope.cos.double()[rows][:, None], rope.sin.double()[rows][:, None]
+        a, d = x.double()[..., 0:32:2], x.double()[..., 1:32:2]
+        want = torch.cat((torch.stack((a * c - d * s, a * s + d * c), -1).flatten(-2), x.double()[..., 32:]), -1)
+        mag = torch.cat((torch.stack(((a * c).abs() + (d * s).abs(), (a * s).abs() + (d * c).abs()),
+                                     -1).flatten(-2), 0 * x.double()[..., 32:]), -1)
+        tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-38
+        bound = torch.finfo(dtype).eps / 2 * (want.abs() + 2 * 2.0 ** -24 * mag) + 2 * 2.0 ** -24 * mag + tiny
+        assert ((rope.rotate(x, pos).double() - want).abs() <= bound).all()
+    with pytest.raises(ValueError):
+        RotaryEmbedding(32, 699).rotate(x)
+
+
 @pytest.mark.gpu
 def test_gpu_rotary_position_outside_the_tables_is_nan():
     rope = RotaryEmbedding(8, 16, device="cuda")
