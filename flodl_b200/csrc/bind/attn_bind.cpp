@@ -267,7 +267,7 @@ struct CrossAttn : public torch::autograd::Function<CrossAttn> {
 
 // Attention over a memory: argument errors are ValueErrors. Nothing comes back
 // where the kernels do not apply (another dtype or head size, an empty
-// dimension); the caller then checks and composes.
+// dimension, a forward-mode tangent); the caller then checks and composes.
 optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor& v,
                                  const optional<Tensor>& key_pad, bool causal, optional<double> scale) {
   if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || !q.is_cuda() ||
@@ -277,7 +277,7 @@ optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor&
     return c10::nullopt;
   const int64_t B = q.size(0), D = q.size(3);
   if (k.size(0) != B || k.size(3) != D || D % 8 || D > 128 || q.numel() == 0 || k.numel() == 0 ||
-      q.size(2) % k.size(2))
+      q.size(2) % k.size(2) || has_tangent(q) || has_tangent(k) || has_tangent(v))
     return c10::nullopt;
   TORCH_CHECK_VALUE(!key_pad || (key_pad->scalar_type() == at::kBool && key_pad->dim() == 2 &&
                                  key_pad->size(0) == B && key_pad->size(1) == k.size(1) &&

@@ -59,6 +59,11 @@ inline torch::autograd::variable_list once_differentiable(torch::autograd::varia
   return grads;
 }
 
+// A tensor with a forward-mode tangent: the kernels have none to give, so that an
+// operator which also has a composed form takes that one.
+inline bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+inline bool has_tangent(const c10::optional<at::Tensor>& t) { return t && has_tangent(*t); }
+
 namespace py = pybind11;
 void register_gemm(py::module& m);
 void register_norm(py::module& m);

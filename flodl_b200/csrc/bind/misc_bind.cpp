@@ -283,8 +283,8 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
 };
 
 // The operator: argument errors are ValueErrors. Nothing comes back where the
-// kernels do not apply (another dtype or head size, an empty input); the caller
-// then checks and composes.
+// kernels do not apply (another dtype or head size, an empty input, a forward-mode
+// tangent); the caller then checks and composes.
 optional<std::pair<Tensor, Tensor>> qk_norm_rope(const Tensor& q, const Tensor& k,
                                                  const optional<Tensor>& q_weight,
                                                  const optional<Tensor>& k_weight,
@@ -294,6 +294,9 @@ optional<std::pair<Tensor, Tensor>> qk_norm_rope(const Tensor& q, const Tensor& 
                                                  double eps) {
   if (!q.is_cuda() || dtype_code(q) < 0 || q.dim() != 4 || k.dim() != 4 || q.size(3) < 2 ||
       q.size(3) > flodl::kQkNormRopeMaxD || q.numel() == 0 || k.numel() == 0)
+    return c10::nullopt;
+  if (has_tangent(q) || has_tangent(k) || has_tangent(q_weight) || has_tangent(k_weight) ||
+      has_tangent(cos) || has_tangent(sin))
     return c10::nullopt;
   const int64_t B = q.size(0), S = q.size(1), D = q.size(3);
   TORCH_CHECK_VALUE(k.size(0) == B && k.size(1) == S && k.size(3) == D, "queries ", q.sizes(),

@@ -18,9 +18,9 @@ from __future__ import annotations
 from typing import Callable, List
 
 import torch
+from torch.autograd import forward_ad
 
 from .._ext import cuda_ext
-
 
 
 def use_kernels(t: torch.Tensor) -> bool:
@@ -29,6 +29,11 @@ def use_kernels(t: torch.Tensor) -> bool:
 
 def C():
     return cuda_ext()
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether one of them carries a forward-mode tangent, which the kernels would drop."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 # ----------------------------------------------------------------- shadows

@@ -22,7 +22,7 @@ import torch
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
-from ._common import C, use_kernels
+from ._common import C, has_tangent, use_kernels
 from .norm import qk_norm_rope
 
 
@@ -178,7 +178,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     sums are f32, probabilities are rounded to the inputs' type for the
     products, and score gradients likewise in the backward (in f16 those beyond
     65504 become infinite: scale the loss as for any f16 training). Gradients are
-    the same from run to run. Other inputs run the composed form in f32 or f64.
+    the same from run to run. Other inputs, and those with forward-mode tangents, run
+    the composed form in f32 or f64.
     """
     if use_kernels(q):
         out = C().cross_attention(q, k, v, key_padding, causal, scale)
@@ -258,7 +259,8 @@ def cross_attention_packed(q: torch.Tensor, kv: torch.Tensor,
     if (torch.is_grad_enabled() and (q.requires_grad or kv.requires_grad) and q.dim() == 4
             and _kernels_take(q) and kv.numel() > 0 and kv.dtype == q.dtype and kv.device == q.device
             and kv.shape[0] == q.shape[0] and kv.shape[4] == q.shape[3]
-            and q.shape[2] % kv.shape[3] == 0 and not (causal and q.shape[1] != kv.shape[1])):
+            and q.shape[2] % kv.shape[3] == 0 and not (causal and q.shape[1] != kv.shape[1])
+            and not has_tangent(q, kv)):
         pad = key_padding
         ok = pad is None or (pad.dtype == torch.bool and pad.shape == kv.shape[:2]
                              and pad.device == q.device)
@@ -317,7 +319,8 @@ def attention_qk_norm(qkv: torch.Tensor, B: int, S: int, H: int, q_weight: Optio
     D = qkv.shape[1] // (3 * H)
     packed = qkv.view(B, S, 3, H, D) if qkv.is_contiguous() else qkv.reshape(B, S, 3, H, D)
     needs = any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight))
-    if torch.is_grad_enabled() and needs and _kernels_take(packed):
+    if (torch.is_grad_enabled() and needs and _kernels_take(packed)
+            and not has_tangent(packed, q_weight, k_weight, cos, sin)):
         # the checks of both operators, on views (nothing is launched for them)
         from .norm import check_qk_norm_rope
         check_qk_norm_rope(packed[:, :, 0], packed[:, :, 1], q_weight, k_weight, cos, sin, positions, 0)

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
-from ._common import (C, as_bf16_2d, bf16_shadow, grad_buffer, grad_ready, splitk_for,
+from ._common import (C, as_bf16_2d, bf16_shadow, grad_buffer, grad_ready, has_tangent, splitk_for,
                       use_kernels, wants_grad)
 
 
@@ -321,6 +321,9 @@ def project_rows(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     part = (lambda t: t[lo:hi] if t is not None else None)
     if not use_kernels(x):
         return F.linear(x, weight[lo:hi], part(bias))
+    if has_tangent(x, weight, bias):
+        b = part(bias)
+        return F.linear(x.bfloat16(), weight[lo:hi].bfloat16(), b.bfloat16() if b is not None else None)
     b16 = bf16_shadow(bias) if bias is not None else None
     w16 = bf16_shadow(weight)[lo:hi]
     x2 = as_bf16_2d(x)

@@ -426,3 +426,58 @@ def test_gpu_rotary_position_outside_the_tables_is_nan():
     assert torch.isnan(y).all(1).all(-1).tolist() == [[False, False, True, False],
                                                      [False, True, True, False]]
     assert not torch.isnan(y[0, :, :2]).any()
+
+
+# ------------------------------------------------------------------ forward mode
+def tangents(device, dtype):
+    """Forward-mode tangents of the operators against the same in 64 bits on the CPU:
+    norm-wise off by no more than half a step of the type for every rounding (one at
+    the end; in attention_qk_norm also of the normed queries and keys and of their
+    tangents), and by f32 sums of up to 64 terms."""
+    from torch.autograd import forward_ad
+    g = torch.Generator().manual_seed(4)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(dtype)
+    q, k, v, kv, qkv = rnd(2, 5, 4, 16), rnd(2, 9, 2, 16), rnd(2, 9, 2, 16), rnd(2, 9, 2, 2, 16), rnd(10, 96)
+    x, W, w = rnd(3, 32), rnd(96, 32).bfloat16().float(), torch.rand(16, generator=g) + 0.5
+    rope = RotaryEmbedding(16, 8)
+    calls = [  # dual inputs, the others, the operator, its roundings
+        ((q, k, v), (), lambda a, b, c: ops.cross_attention(a, b, c), 1),
+        ((v,), (q, k), lambda c, a, b: ops.cross_attention(a, b, c), 1),
+        ((kv,), (q,), lambda b, a: ops.cross_attention_packed(a, b), 1),
+        ((q, k[:, :5]), (w, rope.cos, rope.sin), lambda a, b, w, c, s: ops.qk_norm_rope(a, b, w, w, c, s)[1], 1),
+        ((w,), (q, k[:, :5]), lambda w, a, b: ops.qk_norm_rope(a, b, w, w)[0], 1),
+        ((qkv,), (w, rope.cos, rope.sin), lambda a, w, c, s: ops.attention_qk_norm(a, 2, 5, 2, w, w, c, s), 5),
+        ((x,), (W,), lambda a, W: ops.project_rows(a, W, None, 32, 96), 1),
+    ]
+    for duals, others, f, roundings in calls:
+        steps = [rnd(*t.shape) for t in duals]
+
+        def run(dev, wide, leaves):
+            cast = lambda t: (t.double() if wide else t).to(dev)
+            with forward_ad.dual_level():
+                made = [forward_ad.make_dual(cast(t).detach().requires_grad_(leaves), cast(d.to(t.dtype)))
+                        for t, d in zip(duals, steps)]
+                y = f(*made, *(cast(t) for t in others))
+                t = forward_ad.unpack_dual(y).tangent
+                return None if t is None else t.detach()
+
+        want = run("cpu", True, False)
+        for leaves in (False, True):
+            got = run(device, False, leaves)
+            assert got is not None, "the tangent is lost"
+            close(got.cpu(), want, roundings * torch.finfo(got.dtype).eps / 2 + 64 * 2.0 ** -24, "tangent")
+
+
+def test_cpu_tangents():
+    tangents("cpu", torch.float32)
+
+
+@pytest.mark.gpu
+def test_gpu_tangents():
+    tangents("cuda", torch.bfloat16)
+    with pytest.raises(Exception):  # the fused projections have no forward mode, and say so
+        from torch.autograd import forward_ad
+        m = layer("plain", device="cuda")
+        with forward_ad.dual_level():
+            x = torch.randn(1, 3, 32, device="cuda")
+            m(forward_ad.make_dual(x, x), x)
