@@ -7,6 +7,7 @@
 //   backward, from the base-2 log-sum-exp and delta = rowsum(dO * O):
 //   P = 2^(c log2e S - lse2),  dS = P (dO V^T - delta),
 //   dQ = c dS K,  dK = c dS^T Q,  dV = P^T dO
+// (in f16 dS is formed at a power of two of its value, see range_shift)
 //
 // Tiles come by 4-D TMA maps {D, position, head, batch} straight from the
 // strided tensors: no copy for packed projections, rows past the end and
@@ -78,6 +79,7 @@ struct Type<__nv_bfloat16> {
   static constexpr uint32_t kIdesc = 1;  // tcgen05 kind::f16 operand format
   static constexpr float kShift = 0.f;
   static constexpr bool kCubic = true;  // (see f2_exp2_cubic)
+  static constexpr bool kRanged = false;
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
   static __device__ __forceinline__ uint64_t unpack(uint32_t v) {
     const float2 f = unpack_bf16x2(v);
@@ -91,6 +93,7 @@ struct Type<__half> {
   // is formed at 2^7 times its value and dV scaled back
   static constexpr float kShift = 7.f;
   static constexpr bool kCubic = false;
+  static constexpr bool kRanged = true;  // dS is formed at a power of two (see range_shift)
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -917,6 +920,27 @@ __device__ __forceinline__ float dot8<__half>(uint4 a, uint4 b) {
 struct Stride3 {
   int64_t b, s, h;
 };
+// f16 has no normal numbers below 2^-14, and dS = P (dP - delta) of a long row or of
+// a small dO lies below (8192 keys, D = 64: with dO of 1e-3 the input gradients were off
+// by 0.010 of their norm, where rounding them once is off by 0.0009). So f16 dS is formed
+// at 2^k of its value and the products scaled back in f32. k comes from
+//   |dP - delta| <= 2 |dO_i| max_j |V_j|   (norms; j over the visible keys; O is a mean of V)
+// so that 2^k |dS| stays within 2^15: for dQ from its row's dO, for dK, which sums rows, from
+// the largest dO of the memory head's queries. The power is folded into exponents
+// and factors that are there anyway; what it costs is a pass over V in front.
+struct Range {
+  const float* norms;     // |dO_i|^2 [B, H, stat_pitch]
+  const uint32_t* d_max;  // [B, Hk] the largest, as bits (of numbers >= 0 in their order; NaN above)
+  const uint32_t* v_max;  // [B, Hk, parts] the largest |V_j|^2 of a range's parts
+  int parts;              // 32 at most
+};
+constexpr int kRangeParts = 32;
+__device__ __forceinline__ int range_shift(float d2, float v2) {
+  const float p = d2 * v2;
+  if (!(p > 0.f && p < INFINITY)) return 0;  // nothing to scale, or no finite result
+  const int e = (int)(__float_as_uint(p) >> 23) - 127;  // sqrt(p) < 2^ceil((e + 1) / 2)
+  return 14 - ((e + 2) >> 1);
+}
 // The backward's row statistics: {-lse2, -delta} of every query, [B, H, pitch]
 // with the pitch Sq rounded up to 64 so that a streamed tile's 64 pairs are one
 // aligned 512-byte copy. Rows past Sq hold {-inf, 0}: their P is 0. (Made by the
@@ -933,8 +957,10 @@ __global__ void __launch_bounds__(256) cross_stats_kernel(const T* __restrict__ 
                                                           const T* __restrict__ out_res,
                                                           const T* __restrict__ dout, Stride3 ds,
                                                           const float* __restrict__ lse2,
-                                                          float2* __restrict__ stats, int B, int Sq,
-                                                          FastDiv by_heads, int D) {
+                                                          float2* __restrict__ stats,
+                                                          float* __restrict__ norms,
+                                                          uint32_t* __restrict__ d_max, int B, int Sq,
+                                                          FastDiv by_heads, FastDiv by_group, int D) {
   pdl_wait();
   pdl_trigger();
   constexpr int kPer = 256 / kLanes;
@@ -971,8 +997,63 @@ __global__ void __launch_bounds__(256) cross_stats_kernel(const T* __restrict__ 
         if (part == 0 && i[k] < (uint32_t)pitch)
           stats[((int64_t)b * H + h[k]) * pitch + i[k]] = make_float2(
               i[k] < (uint32_t)Sq ? -__ldg(lse2 + ((int64_t)b * H + h[k]) * Sq + i[k]) : -INFINITY, -s);
+        if constexpr (Type<T>::kRanged) {
+          float n = dot8<T>(g[k], g[k]);
+#pragma unroll
+          for (int x = kLanes / 2; x > 0; x >>= 1) n += __shfl_xor_sync(0xffffffffu, n, x);
+          if (part == 0 && i[k] < (uint32_t)pitch) {
+            norms[((int64_t)b * H + h[k]) * pitch + i[k]] = n;
+            uint32_t* top = d_max + (int64_t)b * by_group.div(H) + by_group.div(h[k]);
+            if (__float_as_uint(n) > *(volatile uint32_t*)top) atomicMax(top, __float_as_uint(n));
+          }
+        }
       }
     }
+}
+
+// The largest |V_j|^2 over the visible keys of a part of each (sample, memory head), and
+// zeros to the maxima of dO that the statistics' kernel raises. kLanes lanes a row.
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(256) cross_range_kernel(const T* __restrict__ v, Stride3 vs,
+                                                          const uint32_t* __restrict__ words,
+                                                          const int* __restrict__ vis_end, int Sk,
+                                                          FastDiv by_heads, uint32_t units, int D,
+                                                          uint32_t* __restrict__ v_max,
+                                                          uint32_t* __restrict__ d_max) {
+  __shared__ uint32_t s_top[8];
+  pdl_wait();
+  pdl_trigger();
+  constexpr int kPer = 256 / kLanes;
+  const int part = threadIdx.x % kLanes, sub = threadIdx.x / kLanes;
+  const bool mine = part * 8 < D;
+  const int nwords = (Sk + 31) / 32;
+  for (uint32_t unit = blockIdx.y; unit < units; unit += gridDim.y) {
+    const uint32_t b = by_heads.div(unit), kh = unit - b * by_heads.d;
+    const int end = vis_end ? __ldg(vis_end + b) : Sk;
+    const T* base = v + b * vs.b + kh * vs.h + part * 8;
+    uint32_t top = 0;
+#pragma unroll 4
+    for (int j0 = blockIdx.x * kPer; j0 < end; j0 += gridDim.x * kPer) {
+      const int j = j0 + sub;
+      const bool seen =
+          j < end && (!words || ((__ldg(words + (int64_t)b * nwords + j / 32) >> (j & 31)) & 1u));
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (seen && mine) x = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)j * vs.s));
+      float n = dot8<T>(x, x);
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+      top = max(top, __float_as_uint(n));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (threadIdx.x % 32 == 0) s_top[threadIdx.x / 32] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 8; ++w) top = max(top, s_top[w]);
+      v_max[(int64_t)unit * gridDim.x + blockIdx.x] = top;
+      if (blockIdx.x == 0) d_max[unit] = 0;
+    }
+    __syncthreads();
+  }
 }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
@@ -1059,10 +1140,12 @@ struct BwdOut {
   T *o1, *o2;          // dQ, or dK and dV
   Stride3 s1, s2;
   float* part;         // [splits][1 or 2][rows][D] when splits > 1
+  Range range;
 };
 
 // kSplit: pieces of the streamed axis (a template because the code that joins them
-// costs the others registers: 28.3 instead of 26.7 us on 64 x 8 heads, 256 x 256 x 64).
+// costs the others registers: 28.3 instead of 26.7 us on 64 x 8 heads, 256 x 256 x 64; the
+// split queries' kernels, at the 168 registers of a thread, spill 4 to 60 bytes).
 template <typename T, int kDP, bool kKeys, int kABufs, bool kSplit>
 __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
     cross_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1,
@@ -1346,13 +1429,35 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       }
       return v;
     };
+    // the exponent at which dS of an item (queries: of its row) is formed
+    auto shift_of = [&](const BwdItem& x) {
+      if constexpr (Type<T>::kRanged) {
+        if (x.lo >= x.hi) return 0;
+        const int64_t unit = (int64_t)x.b * sh.Hk + (kKeys ? (uint32_t)x.head : sh.by_group.div(x.head));
+        const uint32_t v2 = __reduce_max_sync(
+            0xffffffffu,
+            lane < outs.range.parts ? __ldg(outs.range.v_max + unit * outs.range.parts + lane) : 0u);
+        float d2 = 0.f;
+        if (kKeys)
+          d2 = __uint_as_float(__ldg(outs.range.d_max + unit));
+        else if (x.row0 + r < sh.Sq)
+          d2 = __ldg(outs.range.norms + ((int64_t)x.b * sh.H + x.head) * stat_pitch(sh.Sq) + x.row0 + r);
+        return range_shift(d2, __uint_as_float(v2));
+      }
+      return 0;
+    };
     BwdItem after = bwd_item<kKeys>(sh, blockIdx.x, n_rt);
     float2 after_row = row_of(after);
+    int after_shift = shift_of(after);
     for (Walk item; item.at < n_items && ok; item.next()) {
       const BwdItem it = after;
       const int row = it.row0 + r;
       const bool any = it.lo < it.hi;
-      const uint64_t row_lse = f2_splat(after_row.x), row_delta = f2_splat(after_row.y);
+      // 2^shift dS: queries by P's exponent, keys (where P is wanted too) by dP's factor
+      const int shift = after_shift;
+      const uint64_t row_lse = f2_splat(kKeys ? after_row.x : after_row.x + (float)shift);
+      const uint64_t row_delta = f2_splat(after_row.y);
+      const uint64_t d_factor = f2_splat(kShift != 0.f ? exp2f((float)shift - kShift) : 1.f);
       const bool row_ok = !kKeys || after_row.y != 0.f;
       const bool rows_ok = __all_sync(0xffffffffu, row_ok);
       // the CTA's tiles alternate between the groups: mine is every second one
@@ -1410,7 +1515,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
               float p0, p1, d0, d1;
               exp2_pair<!kKeys && Type<T>::kCubic>(e, i / 2, p0, p1);
               uint64_t d = f2_add(f2_pack(__uint_as_float(d16[i]), __uint_as_float(d16[i + 1])), nd);
-              if (kShift != 0.f) d = f2_mul(d, f2_splat(unshift));
+              if (kShift != 0.f) d = f2_mul(d, d_factor);
               f2_unpack(f2_mul(f2_pack(p0, p1), d), d0, d1);
               if (decltype(masked)::value) {
                 bool v0 = row_ok && ((wc >> i) & 1u), v1 = row_ok && ((wc >> (i + 1)) & 1u);
@@ -1446,6 +1551,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       // the next item, and its row's load, while the last product runs
       after = bwd_item<kKeys>(sh, item.after(), n_rt);
       after_row = row_of(after);
+      after_shift = shift_of(after);
       // A group without a tile in this item gives the buffer back here, before it waits
       // for the products: of items of one tile each, these may come behind scores
       // that need the buffer.
@@ -1461,7 +1567,7 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       // group at head size 64)
       const bool second = kKeys && group == 0;
       const uint32_t t_a = (second ? t_acc2 : t_acc1) + lanes;
-      const float f = second ? unshift : sh.scale;
+      const float f = second ? unshift : Type<T>::kRanged ? sh.scale * exp2f((float)-shift) : sh.scale;
       if (any && !kSplit) {
         uint8_t* block = (second ? sm.a2[is.at] : sm.a1[is.at]) + (warp & 3) * 4096;
 #pragma unroll 1
@@ -1745,6 +1851,26 @@ CrossSplits dkv_splits(const CrossAttnArgs& a) {
   return bwd_splits(row_tiles(a.Sk) * a.Hk * a.B, ((int64_t)a.Sq + kBN - 1) / kBN * (a.H / a.Hk));
 }
 
+// Parts of the keys in cross_range_kernel: as many CTAs as eight to an SM, with four
+// rows a lane or more.
+int range_parts(const CrossAttnArgs& a) {
+  const int64_t units = (int64_t)a.B * a.Hk, rows = (a.D <= 64 ? 32 : 16) * 4;
+  return (int)std::max<int64_t>(
+      1, std::min<int64_t>({kRangeParts, num_sms() * 8 / units, (a.Sk + rows - 1) / rows}));
+}
+// The scratch of `stats`: the row statistics, then (f16) the norms of dO's rows, their
+// maxima and those of V's.
+Range range_of(const CrossAttnArgs& a) {
+  Range r{};
+  if (!a.half) return r;
+  const int64_t rows = (int64_t)a.B * a.H * stat_pitch(a.Sq);
+  r.norms = a.stats + 2 * rows;
+  r.d_max = reinterpret_cast<const uint32_t*>(r.norms + rows);
+  r.v_max = r.d_max + (int64_t)a.B * a.Hk;
+  r.parts = range_parts(a);
+  return r;
+}
+
 template <typename T, int kDP, bool kTrain>
 cudaError_t run_fwd(const CrossAttnArgs& a, cudaStream_t st) {
   const CrossSplits plan = fwd_splits(a);
@@ -1812,6 +1938,7 @@ cudaError_t run_bwd_half(const CrossAttnArgs& a, const CrossSplits& plan, cudaSt
   o.o2 = kKeys ? (T*)a.dv : o.o1;
   o.s2 = kKeys ? s3(a.dv_st) : o.s1;
   o.part = plan.joined() ? a.partials : nullptr;
+  o.range = range_of(a);
   const int grid = (int)std::min<int64_t>(items, num_sms());
   e = launch_pdl_cluster(kernel, dim3(grid), dim3(BwdGeo<kDP, kKeys, kABufs>::kThreads),
                          plan.clustered ? splits : 1, smem, st, kKeys ? mk : mq, kKeys ? mv : mo,
@@ -1832,19 +1959,39 @@ cudaError_t run_bwd_half(const CrossAttnArgs& a, const CrossSplits& plan, cudaSt
 }
 
 template <typename T>
+cudaError_t run_range(const CrossAttnArgs& a, const Range& r, cudaStream_t st) {
+  const uint32_t units = (uint32_t)a.B * (uint32_t)a.Hk;
+  auto k = a.D <= 64 ? cross_range_kernel<T, 8> : cross_range_kernel<T, 16>;
+  cudaError_t e = launch_pdl(k, dim3(r.parts, std::min(units, 65535u)), dim3(256), 0, st, (const T*)a.v,
+                             Stride3{a.v_st[0], a.v_st[1], a.v_st[2]},
+                             (const uint32_t*)(a.key_pad ? a.words : nullptr),
+                             (const int*)(a.key_pad ? a.vis_end : nullptr), a.Sk, FastDiv((uint32_t)a.Hk),
+                             units, a.D, const_cast<uint32_t*>(r.v_max), const_cast<uint32_t*>(r.d_max));
+  if (e != cudaSuccess) return e;
+  note_launch();
+  return cudaGetLastError();
+}
+
+template <typename T>
 cudaError_t run_stats(const CrossAttnArgs& a, cudaStream_t st) {
   const int64_t rows = (int64_t)stat_pitch(a.Sq) * a.H;  // of a sample
   if (rows >= kMaxFlatIndex - (1 << 24)) return cudaErrorInvalidValue;  // (over 170 GB of tensors)
   const int per = (a.D <= 64 ? 32 : 16) * kRowsAhead;
   const int64_t x = std::min<int64_t>((rows + per - 1) / per, num_sms() * 16ll);
   const int64_t y = std::min<int64_t>({a.B, std::max<int64_t>(1, num_sms() * 16ll / x), 65535});
+  const Range r = range_of(a);
+  if constexpr (Type<T>::kRanged) {
+    const cudaError_t e = run_range<T>(a, r, st);
+    if (e != cudaSuccess) return e;
+  }
   const dim3 grid((unsigned)x, (unsigned)y);
   const Stride3 ds{a.do_st[0], a.do_st[1], a.do_st[2]};
   auto k = a.D <= 64 ? cross_stats_kernel<T, 8> : cross_stats_kernel<T, 16>;
   cudaError_t e = launch_pdl(k, grid, dim3(256), 0, st, (const T*)a.out,
                              (const T*)a.out_res, (const T*)a.dout, ds,
-                             (const float*)a.lse2, (float2*)a.stats, a.B, a.Sq, FastDiv((uint32_t)a.H),
-                             a.D);
+                             (const float*)a.lse2, (float2*)a.stats, const_cast<float*>(r.norms),
+                             const_cast<uint32_t*>(r.d_max), a.B, a.Sq, FastDiv((uint32_t)a.H),
+                             FastDiv((uint32_t)(a.H / a.Hk)), a.D);
   if (e != cudaSuccess) return e;
   note_launch();
   return cudaGetLastError();
@@ -1885,7 +2032,9 @@ cudaError_t run_bwd(const CrossAttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 int64_t cross_attn_stats_floats(const CrossAttnArgs& a) {
-  return 2ll * a.B * a.H * stat_pitch(a.Sq);
+  const int64_t rows = (int64_t)a.B * a.H * stat_pitch(a.Sq);
+  if (!a.half) return 2 * rows;
+  return 3 * rows + ((int64_t)a.B * a.Hk * (1 + range_parts(a)) + 3) / 4 * 4;  // (what follows is 16-byte aligned)
 }
 int64_t cross_attn_fwd_partials(const CrossAttnArgs& a) {
   const CrossSplits s = cross_attn_is_few(a) ? cross_attn_few_splits(a) : fwd_splits(a);

@@ -29,7 +29,7 @@ struct CrossAttnArgs {
   // backward
   const void* dout = nullptr;
   int64_t do_st[3] = {};
-  float* stats = nullptr;              // scratch of cross_attn_stats_floats
+  float* stats = nullptr;              // scratch of cross_attn_stats_floats, 16-byte aligned
   void *dq = nullptr, *dk = nullptr, *dv = nullptr;  // null dq, or null dk and dv: not wanted
   int64_t dq_st[3] = {}, dk_st[3] = {}, dv_st[3] = {};
   int B = 0, Sq = 0, Sk = 0, H = 0, Hk = 0, D = 0;

@@ -176,9 +176,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     copied. Up to 16 query rows per memory head (``Sq * H / Hk``; the single
     tokens of serving) take a form that streams the memory once. Scores and
     sums are f32, probabilities are rounded to the inputs' type for the
-    products, and score gradients likewise in the backward (in f16 those beyond
-    65504 become infinite: scale the loss as for any f16 training). Gradients are
-    the same from run to run. Other inputs, and those with forward-mode tangents, run
+    products, and score gradients likewise in the backward (in f16 at a power of two
+    that the data gives, so that small ones do not vanish nor large ones overflow; the
+    gradients returned have f16's own range). Gradients are the same from run to run. Other inputs, and those with forward-mode tangents, run
     the composed form in f32 or f64.
     """
     if use_kernels(q):

@@ -251,6 +251,60 @@ def test_gpu_many_items_of_one_tile(D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gains", [  # of queries and keys, values, output gradients
+    (1.0, 1.0, 1.0), (1.0, 1.0, 1e-2), (1.0, 1.0, 1e-3), (1.0, 1.0, 1e-4), (1.0, 1e-2, 1e-2),
+    (0.01, 300.0, 1e3)])
+@pytest.mark.parametrize("shape,mask,causal", [
+    ((1, 130, 2, 1, 8192, 64), None, False), ((2, 70, 4, 2, 9000, 128), "scattered", False),
+    ((2, 3, 4, 2, 9001, 64), "right", False), ((2, 200, 2, 2, 200, 96), None, True),
+    ((3, 40, 2, 1, 60, 64), "empty", False), ((40, 150, 8, 4, 700, 64), "right", False)])
+def test_gpu_f16_gradients_keep_their_range(shape, mask, causal, gains):
+    """Long rows and small or large output gradients in f16. Two roundings to f16 are
+    behind a gradient, of P or dS and of the result. Each is a relative error of the
+    same distribution, independent from term to term, so that in the norm of a sum of
+    many terms of either sign each counts as the rounding of the exact gradient does:
+    sqrt(2) of it together. 2 leaves room for f32's errors and O's rounding in delta."""
+    q, k, v, do = make(*shape, torch.float16, "cuda")
+    q, k, v, do = q * gains[0], k * gains[0], v * gains[1], do * gains[2]
+    pad = mask_of(mask, shape[0], shape[4], "cuda")
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    ops.cross_attention(*leaves, key_padding=pad, causal=causal).backward(do)
+    want = reference(q, k, v, pad, causal, None, do)
+    for x, i, n in zip(leaves, (2, 4, 6), ("dq", "dk", "dv")):
+        once = (want[i].half().double() - want[i]).norm().item()
+        err = (x.grad.double() - want[i]).norm().item()
+        assert err <= 2 * once, f"{n}: {err / want[i].norm():.3g}, rounding once {once / want[i].norm():.3g}"
+
+
+@pytest.mark.gpu
+def test_gpu_f16_gradients_of_unlike_heads_and_rows():
+    """Output gradients of very different sizes by sample, head and row, values by head,
+    rows without any gradient; a sample whose gradient is infinite stays to itself."""
+    shape = (3, 150, 4, 2, 600, 64)
+    q, k, v, do = make(*shape, torch.float16, "cuda")
+    do[0] *= 1e-4
+    do[1, :, 1] *= 1e-3
+    do[1, ::3] = 0
+    do[1, 1::3, 2:] *= 1e-2
+    v[1, :, 1] *= 100
+    want = reference(q, k, v, None, False, None, do)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    out = ops.cross_attention(*leaves)
+    grads = torch.autograd.grad(out, leaves, do, retain_graph=True)
+    for g, i, n in zip(grads, (2, 4, 6), ("dq", "dk", "dv")):
+        for b in range(3):
+            for h in range(g.shape[2]):
+                w = want[i][b, :, h]
+                once = (w.half().double() - w).norm().item()
+                assert (g[b, :, h].double() - w).norm().item() <= 2 * once, (n, b, h)
+    assert (grads[0][1, ::3] == 0).all()
+    do[2, 5] = float("inf")
+    again = torch.autograd.grad(out, leaves, do)
+    for a, b in zip(grads, again):
+        assert torch.equal(a[:2], b[:2]) and not torch.isfinite(b[2]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("packed", [False, True])
 def test_gpu_gradients_of_one_side(packed):
     # frozen memories, frozen queries: the wanted side's gradient is the same
