@@ -72,7 +72,8 @@ def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, causal: bool = F
 
     ``key_padding`` (bool ``[B, S]``, True = masked key) implements the padding
     mask used by BERT-style encoders; with ``causal`` both apply. On CUDA the flash kernel takes
-    head size 64, :func:`cross_attention` the others; the result is bf16.
+    head size 64, :func:`cross_attention` the others and empty inputs; the result
+    is bf16.
     """
     if not use_kernels(qkv):
         D = qkv.shape[1] // (3 * H)
@@ -85,7 +86,7 @@ def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, causal: bool = F
         o = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, is_causal=causal and mask is None)
         return o.permute(0, 2, 1, 3).reshape(B * S, H * D)
     q16 = qkv if qkv.dtype == torch.bfloat16 else qkv.to(torch.bfloat16)
-    if qkv.shape[1] != 3 * H * 64:
+    if qkv.shape[1] != 3 * H * 64 or q16.numel() == 0:
         q, k, v = q16.reshape(B, S, 3, H, qkv.shape[1] // (3 * H)).unbind(2)
         return cross_attention(q, k, v, key_padding, causal).view(B * S, qkv.shape[1] // 3)
     return _PackedAttnFn.apply(q16.contiguous(), B, S, H, causal, key_padding)

@@ -288,11 +288,14 @@ class _CrossProjFn(torch.autograd.Function):
         dx = _rows_dgrad(dq2, w16[:n], ctx.like[0]) if ctx.needs_input_grad[0] else None
         dm = _rows_dgrad(dkv2, w16[n:], ctx.like[1]) if ctx.needs_input_grad[1] else None
         for dy2, in2, lo, hi in ((dq2, x2, 0, n), (dkv2, m2, n, 3 * n)):
-            if wants_grad(weight):
-                C().gemm(dy2, in2, grad_buffer(weight)[lo:hi], hi - lo, K, in2.shape[0], True, True,
+            gw, gb = (grad_buffer(t)[lo:hi] if wants_grad(t) else None for t in (weight, bias))
+            if in2.shape[0] == 0:  # an empty memory: zeros, where nothing was before
+                continue
+            if gw is not None:
+                C().gemm(dy2, in2, gw, hi - lo, K, in2.shape[0], True, True,
                          flags=C().EPI_ACCUMULATE, k_splits=splitk_for(hi - lo, K, in2.shape[0]))
-            if wants_grad(bias):
-                C().colsum(dy2, grad_buffer(bias)[lo:hi])
+            if gb is not None:
+                C().colsum(dy2, gb)
         for t in (weight, bias):
             if wants_grad(t):
                 grad_ready(t)

@@ -105,7 +105,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-5)
     (flodl/src/nn/rmsnorm.rs:54-62). On CUDA one kernel forward and one
     backward (which also accumulates ``weight.grad``); f32 and bf16 inputs keep
     their dtype, statistics are f32."""
-    if not use_kernels(x) or x.dtype not in (torch.float32, torch.bfloat16) or (
+    if not use_kernels(x) or x.dtype not in (torch.float32, torch.bfloat16) or x.numel() == 0 or (
             x.shape[-1] > 8192 and wants_grad(weight)):
         xf = x.float() if x.dtype in (torch.float16, torch.bfloat16) else x  # at least f32
         y = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)

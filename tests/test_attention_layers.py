@@ -136,6 +136,36 @@ def test_gpu_serving_norms_the_memory_once(monkeypatch):
     norms_once("cuda", monkeypatch)
 
 
+def empty_sequences(device, dtype):
+    """A memory without positions gives the output bias and no gradient but its own;
+    a batch without samples gives an empty output."""
+    for kind in KINDS:
+        m = layer(kind, 128, 2, device=device)
+        x = torch.randn(2, 3, 128, device=device).to(dtype).requires_grad_()
+        mem = torch.randn(2, 0, 128, device=device).to(dtype)
+        y = m(x, mem)
+        bias = m.out_proj.bias.detach()
+        t = T if x.is_cuda else 0.0  # the projection rounds
+        assert ((y.detach().float() - bias).abs() <= t * bias.abs()).all()
+        y.float().sum().backward()
+        assert (x.grad == 0).all() and (m.qkv.weight.grad == 0).all() and (m.qkv.bias.grad == 0).all()
+        serve = m.attend_memory(x.detach()[:, :1], m.project_memory(mem))
+        assert torch.equal(serve, y.detach()[:, :1])
+        with torch.no_grad():
+            none = torch.randn(0, 3, 128, device=device).to(dtype)
+            assert m(none).shape == (0, 3, 128) and m(none, none).shape == (0, 3, 128)
+
+
+def test_cpu_empty_sequences():
+    empty_sequences("cpu", torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gpu_empty_sequences(dtype):
+    empty_sequences("cuda", dtype)
+
+
 def shared_masks(device):
     """One mask for all samples, and one flag for all keys of a sample."""
     x, mem = torch.randn(2, 3, 32, device=device), torch.randn(2, 9, 32, device=device)
