@@ -27,7 +27,8 @@ void flash_fwd(const Tensor& qkv, Tensor& out, Tensor& lse2, int64_t B, int64_t 
   a.lse2 = lse2.data_ptr<float>();
   if (key_pad) {
     FL_CHECK(key_pad->scalar_type() == at::kBool && key_pad->is_contiguous() &&
-                 key_pad->numel() == B * S, "key_pad must be bool [B, S]");
+                 key_pad->numel() == B * S && key_pad->device() == qkv.device(),
+             "key_pad must be bool [B, S] on ", qkv.device());
     a.key_pad = reinterpret_cast<const uint8_t*>(key_pad->data_ptr());
   }
   a.B = (int)B; a.S = (int)S; a.H = (int)H; a.D = (int)D;
@@ -56,7 +57,12 @@ void flash_bwd(const Tensor& dout, const Tensor& qkv, const Tensor& out, const T
   a.dqkv = reinterpret_cast<__nv_bfloat16*>(dqkv.data_ptr());
   a.delta = delta.data_ptr<float>();
   a.dq_acc = dq_acc.defined() ? dq_acc.data_ptr<float>() : nullptr;
-  if (key_pad) a.key_pad = reinterpret_cast<const uint8_t*>(key_pad->data_ptr());
+  if (key_pad) {
+    FL_CHECK(key_pad->scalar_type() == at::kBool && key_pad->is_contiguous() &&
+                 key_pad->numel() == B * S && key_pad->device() == qkv.device(),
+             "key_pad must be bool [B, S] on ", qkv.device());
+    a.key_pad = reinterpret_cast<const uint8_t*>(key_pad->data_ptr());
+  }
   if (dbias) {
     FL_CHECK_F32(*dbias);
     FL_CHECK(dbias->is_contiguous() && dbias->numel() == 3 * H * D, "dbias must be f32 [3*H*D]");

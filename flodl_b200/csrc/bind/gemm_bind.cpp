@@ -15,6 +15,9 @@ void gemm(const at::Tensor& A, const at::Tensor& B, at::Tensor& out, int64_t M, 
   FL_CHECK_CUDA(A);
   FL_CHECK_CUDA(B);
   FL_CHECK_CUDA(out);
+  FL_CHECK(B.device() == A.device() && out.device() == A.device(), "gemm operands on one device");
+  for (const c10::optional<at::Tensor>* t : {&bias, &residual, &aux})
+    FL_CHECK(!*t || (*t)->device() == A.device(), "gemm operands on one device");
   FL_CHECK_BF16(A);
   FL_CHECK_BF16(B);
   FL_CHECK(A.dim() == 2 && B.dim() == 2 && out.dim() == 2, "gemm operands must be 2-D");

@@ -605,6 +605,8 @@ void add_scalar(Tensor& x, double v) {
 
 void cast_f32_bf16(const Tensor& x, Tensor& y) {
   FL_CHECK_F32(x); FL_CHECK_BF16(y);
+  FL_CHECK_CUDA(x);
+  FL_CHECK(y.device() == x.device(), "cast devices");
   FL_CHECK(x.numel() == y.numel() && x.is_contiguous() && y.is_contiguous(), "cast sizes");
   c10::cuda::CUDAGuard guard(x.device());
   FL_CUDA_OK(flodl::launch_cast_f32_bf16(ptr<float>(x), ptr<__nv_bfloat16>(y), x.numel(), cur_stream()));

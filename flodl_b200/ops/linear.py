@@ -302,10 +302,26 @@ class _CrossProjFn(torch.autograd.Function):
         return dx, dm, None, None
 
 
+def _check_projection(weight, bias, *inputs):
+    if weight.dim() != 2 or (bias is not None and tuple(bias.shape) != (weight.shape[0],)):
+        raise ValueError(f"the weight must be [rows, K] and the bias [rows] (got {tuple(weight.shape)}"
+                         f"{'' if bias is None else f' and {tuple(bias.shape)}'})")
+    for t in inputs:
+        if t.dim() < 1 or t.shape[-1] != weight.shape[1]:
+            raise ValueError(f"inputs must be [..., {weight.shape[1]}] (got {tuple(t.shape)})")
+    for t in (*inputs[1:], weight, bias):
+        if t is not None and t.device != inputs[0].device:
+            raise ValueError(f"inputs, weight and bias must be on one device (got {inputs[0].device} and "
+                             f"{t.device})")
+
+
 def cross_projection(x: torch.Tensor, memory: torch.Tensor, weight: torch.Tensor,
                      bias: Optional[torch.Tensor] = None):
     """``(queries of x, keys and values of memory)`` by a packed ``[3N, K]``
     weight's rows: ``x [..., K] -> [..., N]``, ``memory [..., K] -> [..., 2N]``."""
+    _check_projection(weight, bias, x, memory)
+    if weight.shape[0] % 3:
+        raise ValueError(f"the packed weight must be [3N, K] (got {tuple(weight.shape)})")
     n = weight.shape[0] // 3
     if use_kernels(x) and n % 8 == 0 and weight.shape[1] % 8 == 0 and weight.is_leaf:
         return _CrossProjFn.apply(x, memory, weight, bias)
@@ -321,6 +337,9 @@ def project_rows(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
                  hi: int) -> torch.Tensor:
     """``x @ weight[lo:hi]^T + bias[lo:hi]`` without gradients: one part of a
     packed projection, from the weight's cached bf16 shadow on CUDA."""
+    _check_projection(weight, bias, x)
+    if not 0 <= lo <= hi <= weight.shape[0]:
+        raise ValueError(f"rows {lo} to {hi} of {weight.shape[0]}")
     part = (lambda t: t[lo:hi] if t is not None else None)
     if not use_kernels(x):
         return F.linear(x, weight[lo:hi], part(bias))

@@ -231,6 +231,43 @@ def test_refusals():
         ops.cross_attention_packed(torch.randn(1, 2, 1, 8), torch.randn(1, 2, 1, 8))
 
 
+def projection_refusals(device, elsewhere):
+    x, mem = torch.randn(2, 3, 16, device=device), torch.randn(2, 5, 16, device=device)
+    W, b = torch.randn(24, 16, device=device), torch.randn(24, device=device)
+    q, kv = ops.cross_projection(x, mem, W, b)
+    assert q.shape == (2, 3, 8) and kv.shape == (2, 5, 16)
+    away = (lambda t: torch.empty(t.shape, device=elsewhere))
+    for args in ((x[..., :8], mem, W, b), (x, mem[..., :8], W, b), (x, mem, W[:23], b[:23]), (x, mem, W, b[:16]),
+                 (x, mem, W[0], None), (x, away(mem), W, b), (x, mem, away(W), b), (x, mem, W, away(b))):
+        with pytest.raises(ValueError):
+            ops.cross_projection(*args)
+    for args in ((x[..., :8], W, b, 0, 8), (x, W, b[:8], 0, 8), (x, W, b, 8, 25), (x, W, b, -1, 8), (x, W, b, 9, 8),
+                 (x, away(W), b, 0, 8), (x, W, away(b), 0, 8)):
+        with pytest.raises(ValueError):
+            ops.project_rows(*args)
+
+
+def test_cpu_projection_refusals():
+    projection_refusals("cpu", "meta")
+
+
+@pytest.mark.gpu
+def test_gpu_projection_refusals():
+    """Host tensors among CUDA ones are refused on the host, masks and biases too."""
+    projection_refusals("cuda", "cpu")
+    x, W, b = torch.randn(2, 16, device="cuda"), torch.randn(8, 16, device="cuda"), torch.randn(8)
+    from flodl_b200._ext import cuda_ext
+    C = cuda_ext()
+    with pytest.raises(RuntimeError):
+        C.cast_f32_bf16(b, torch.empty(8, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError):
+        C.gemm(x.bfloat16(), W.bfloat16(), torch.empty(2, 8, device="cuda"), 2, 8, 16, False, False, bias=b)
+    for heads in (1, 2):  # head sizes 64 and 32
+        qkv = torch.randn(6, 3 * 64, device="cuda").bfloat16()
+        with pytest.raises((RuntimeError, ValueError)):
+            ops.attention_packed(qkv, 2, 3, heads, False, torch.zeros(2, 3, dtype=torch.bool))
+
+
 def block(device=None, C=128, H=2):
     """A decoder block: self-attention with normed, rotated heads, then
     cross-attention to a memory, both with residuals."""
