@@ -284,7 +284,7 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
 
 // The operator: argument errors are ValueErrors. Nothing comes back where the
 // kernels do not apply (another dtype or head size, an empty input, a forward-mode
-// tangent); the caller then checks and composes.
+// tangent, tables that want gradients); the caller then checks and composes.
 optional<std::pair<Tensor, Tensor>> qk_norm_rope(const Tensor& q, const Tensor& k,
                                                  const optional<Tensor>& q_weight,
                                                  const optional<Tensor>& k_weight,
@@ -334,6 +334,7 @@ optional<std::pair<Tensor, Tensor>> qk_norm_rope(const Tensor& q, const Tensor& 
   const auto c = turn ? plain(cos) : c10::nullopt, s = turn ? plain(sin) : c10::nullopt;
   const auto pos = turn ? plain(positions) : c10::nullopt;
   auto grad = [](const optional<Tensor>& t) { return t && t->requires_grad(); };
+  if (at::GradMode::is_enabled() && (grad(c) || grad(s))) return c10::nullopt;  // learned tables
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || grad(wq) || grad(wk))) {
     auto y = QkNormRope::apply(q, k, wq, wk, c, s, pos, offset, eps);
     return std::make_pair(y[0], y[1]);

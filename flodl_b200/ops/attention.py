@@ -321,6 +321,7 @@ def attention_qk_norm(qkv: torch.Tensor, B: int, S: int, H: int, q_weight: Optio
     packed = qkv.view(B, S, 3, H, D) if qkv.is_contiguous() else qkv.reshape(B, S, 3, H, D)
     needs = any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight))
     if (torch.is_grad_enabled() and needs and _kernels_take(packed)
+            and not any(t is not None and t.requires_grad for t in (cos, sin))
             and not has_tangent(packed, q_weight, k_weight, cos, sin)):
         # the checks of both operators, on views (nothing is launched for them)
         from .norm import check_qk_norm_rope

@@ -323,7 +323,8 @@ def cross_projection(x: torch.Tensor, memory: torch.Tensor, weight: torch.Tensor
     if weight.shape[0] % 3:
         raise ValueError(f"the packed weight must be [3N, K] (got {tuple(weight.shape)})")
     n = weight.shape[0] // 3
-    if use_kernels(x) and n % 8 == 0 and weight.shape[1] % 8 == 0 and weight.is_leaf:
+    if (use_kernels(x) and n % 8 == 0 and weight.shape[1] % 8 == 0 and weight.is_leaf
+            and (bias is None or bias.is_leaf)):  # computed ones get theirs through autograd
         return _CrossProjFn.apply(x, memory, weight, bias)
     if use_kernels(x):
         x, memory, weight = x.bfloat16(), memory.bfloat16(), weight.bfloat16()

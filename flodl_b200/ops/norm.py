@@ -243,8 +243,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     is f32 and rounded once.
 
     CUDA f32, bf16 and f16 inputs with 2 <= D <= 256 run one kernel forward and one
-    backward (plus a reduction of the weight gradients); other inputs, and those with
-    forward-mode tangents, the composed form. A position outside the tables gives NaN in the rotated
+    backward (plus a reduction of the weight gradients); other inputs, those with
+    forward-mode tangents and tables that want gradients run the composed form. A position outside the tables gives NaN in the rotated
     values of its heads and records code 5 in the kernel error word on CUDA;
     on the CPU it raises.
     """

@@ -268,6 +268,42 @@ def test_gpu_projection_refusals():
             ops.attention_packed(qkv, 2, 3, heads, False, torch.zeros(2, 3, dtype=torch.bool))
 
 
+def computed_parameters(device):
+    """Biases and tables that are computed, or learned, get their gradients: against
+    the same on the CPU in 64 bits."""
+    g = torch.Generator().manual_seed(6)
+    rnd = lambda *s: torch.randn(*s, generator=g).bfloat16().float()
+    x, mem, W, b = rnd(2, 3, 16), rnd(2, 5, 16), rnd(24, 16), rnd(24)
+    qkv, cos, sin = rnd(6, 3 * 32), rnd(8, 8), rnd(8, 8)
+
+    def grads(dev, wide):
+        to = lambda t: (t.double() if wide else t.clone()).to(dev).requires_grad_()
+        a, c, d = to(b), to(cos), to(sin)
+        q, kv = ops.cross_projection(to(x), to(mem), to(W), 2 * a)
+        heads = to(qkv).view(2, 3, 3, 2, 16)
+        y = ops.qk_norm_rope(heads[:, :, 0], heads[:, :, 1], None, None, c, d)
+        (q.sum() + kv.sum() + y[0].sum() + 2 * y[1].sum()).backward()
+        first = a.grad, c.grad, d.grad
+        c.grad = d.grad = None
+        z = to(qkv) if dev == "cpu" else qkv.bfloat16().to(dev).requires_grad_()
+        ops.attention_qk_norm(z, 2, 3, 2, None, None, c, d).square().sum().backward()
+        return first + (c.grad, d.grad)
+
+    for i, (got, want) in enumerate(zip(grads(device, False), grads("cpu", True))):
+        # sums of exact ones, of f32 values, and through attention of 16-bit ones (normed
+        # heads, P, output and their gradients: six roundings)
+        close(got.cpu(), want, 6 * T if i > 2 and device != "cpu" else 64 * 2.0 ** -24, f"gradient {i}")
+
+
+def test_cpu_computed_parameters():
+    computed_parameters("cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_computed_parameters():
+    computed_parameters("cuda")
+
+
 def block(device=None, C=128, H=2):
     """A decoder block: self-attention with normed, rotated heads, then
     cross-attention to a memory, both with residuals."""
