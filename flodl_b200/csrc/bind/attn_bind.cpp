@@ -271,9 +271,13 @@ struct CrossAttn : public torch::autograd::Function<CrossAttn> {
   }
 };
 
+// Scales that the kernels take: products with powers of two up to 2^61 of the backward's
+// stay normal in f32.
+constexpr double kLeastScale = 1e-18;
+
 // Attention over a memory: argument errors are ValueErrors. Nothing comes back
 // where the kernels do not apply (another dtype or head size, an empty
-// dimension, a forward-mode tangent); the caller then checks and composes.
+// dimension, a scale far from 1, a forward-mode tangent); the caller then checks and composes.
 optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor& v,
                                  const optional<Tensor>& key_pad, bool causal, optional<double> scale) {
   if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || !q.is_cuda() ||
@@ -293,6 +297,7 @@ optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor&
                     q.size(1), " and ", k.size(1), ")");
   const double c = scale ? *scale : 1.0 / std::sqrt((double)D);
   TORCH_CHECK_VALUE(c > 0 && std::isfinite(c), "scale must be positive and finite (got ", c, ")");
+  if (c < kLeastScale || c > 1 / kLeastScale) return c10::nullopt;
   optional<Tensor> pad = key_pad;
   if (pad) pad = pad->contiguous();
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
@@ -313,6 +318,7 @@ void register_attention(py::module& m) {
         py::arg("dbias") = py::none());
   m.def("cross_attention", &cross_attention, py::arg("q"), py::arg("k"), py::arg("v"),
         py::arg("key_padding"), py::arg("causal"), py::arg("scale"));
+  m.attr("CROSS_ATTN_LEAST_SCALE") = kLeastScale;
   m.def("cross_attn_mask", &cross_attn_mask, py::arg("key_pad"));
   m.def("cross_attn_fwd",
         [](const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& key_pad,

@@ -266,7 +266,7 @@ def cross_attention_packed(q: torch.Tensor, kv: torch.Tensor,
         ok = pad is None or (pad.dtype == torch.bool and pad.shape == kv.shape[:2]
                              and pad.device == q.device)
         c = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
-        if ok and c > 0.0 and math.isfinite(c):
+        if ok and C().CROSS_ATTN_LEAST_SCALE <= c <= 1 / C().CROSS_ATTN_LEAST_SCALE:
             return _CrossPackedFn.apply(q, kv, pad.contiguous() if pad is not None else None,
                                         bool(causal), c)
     return cross_attention(q, kv[:, :, 0], kv[:, :, 1], key_padding, causal, scale)

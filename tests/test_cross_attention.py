@@ -487,6 +487,25 @@ def test_gpu_repeats_graphs_and_streams(shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1e-50, 1e-40, 1e-18, 1e-10])
+def test_gpu_tiny_scales(scale):
+    """Scores vanish: a query's output is the mean of the values (a sum of 70 rounded
+    weights and the output's rounding), however far below f32's range the scale is."""
+    for Sq in (1, 40):
+        q, k, v, do = make(2, Sq, 2, 1, 70, 64, torch.bfloat16, "cuda")
+        t = torch.finfo(torch.bfloat16).eps / 2
+        want = v.double().mean(1, keepdim=True).expand(2, Sq, 2, 64)
+        bound = 2 * t * v.double().abs().mean(1, keepdim=True).expand(2, Sq, 2, 64)
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        a = ops.cross_attention(*leaves, scale=scale)
+        b = ops.cross_attention_packed(leaves[0], torch.stack(leaves[1:], 2), scale=scale)
+        for y in (a, b):
+            within(y.detach(), want, bound, "out")
+            grads = torch.autograd.grad(y, leaves, do, retain_graph=True)
+            assert all(torch.isfinite(g).all() for g in grads)
+
+
+@pytest.mark.gpu
 def test_gpu_refusals_and_other_forms():
     from flodl_b200._ext import cuda_ext
     refusals("cuda")
