@@ -35,7 +35,7 @@
 //   384 x 256 x 512 x 64          27.1 (476)  31.5 (409)     32.9 (588)   51.5 (500)
 //   128 x 1024 x 1024 x 64        57 (603)    65 (531)       62 (830)     89 (771)
 //   64 x 2048^2 x 128, causal     79 (873)    92 (751)       113 (914)    150 (915)
-//   32 x 2048 x 8192 x 128        231 (1192)  252 (1093)     344 (1197)   520 (1060)
+//   32 x 2048 x 8192 x 128        226 (1216)  246 (1117)     347 (1189)   560 (982)
 // At head size 128 and long axes the tensor pipe is busy two thirds of the time: the
 // products of a tile and its elementwise work overlap but for the tile's round trip.
 // At head size 64 and a few tiles per item the round trip bounds it (scores, TMEM
@@ -927,12 +927,15 @@ struct Stride3 {
 //   |dP - delta| <= 2 |dO_i| max_j |V_j|   (norms; j over the visible keys; O is a mean of V)
 // so that 2^k |dS| stays within 2^15: for dQ from its row's dO, for dK, which sums rows, from
 // the largest dO of the memory head's queries. The power is folded into exponents
-// and factors that are there anyway; what it costs is a pass over V in front.
+// and factors that are there anyway; what it costs is a pass over V behind the row
+// statistics (64 x 8 heads, 256 x 256 x 64: 14.2 us for both, the statistics alone 7.4, and dQ
+// 27.3 instead of 25.6; 42 heads of 128 x 1500 x 64: 6.1 instead of 2.5).
 struct Range {
-  const float* norms;     // |dO_i|^2 [B, H, stat_pitch]
-  const uint32_t* d_max;  // [B, Hk] the largest, as bits (of numbers >= 0 in their order; NaN above)
-  const uint32_t* v_max;  // [B, Hk, parts] the largest |V_j|^2 of a range's parts
-  int parts;              // 32 at most
+  const float* norms;  // |dO_i|^2 [B, H, stat_pitch]
+  // [B, Hk, parts] the largest |dO_i|^2 and |V_j|^2 of a part of the rows, as bits (of
+  // numbers >= 0 in their order, NaN above all)
+  const uint32_t *d_max, *v_max;
+  int parts;  // kRangeParts at most: a lane each
 };
 constexpr int kRangeParts = 32;
 __device__ __forceinline__ int range_shift(float d2, float v2) {
@@ -958,9 +961,8 @@ __global__ void __launch_bounds__(256) cross_stats_kernel(const T* __restrict__ 
                                                           const T* __restrict__ dout, Stride3 ds,
                                                           const float* __restrict__ lse2,
                                                           float2* __restrict__ stats,
-                                                          float* __restrict__ norms,
-                                                          uint32_t* __restrict__ d_max, int B, int Sq,
-                                                          FastDiv by_heads, FastDiv by_group, int D) {
+                                                          float* __restrict__ norms, int B, int Sq,
+                                                          FastDiv by_heads, int D) {
   pdl_wait();
   pdl_trigger();
   constexpr int kPer = 256 / kLanes;
@@ -1001,26 +1003,24 @@ __global__ void __launch_bounds__(256) cross_stats_kernel(const T* __restrict__ 
           float n = dot8<T>(g[k], g[k]);
 #pragma unroll
           for (int x = kLanes / 2; x > 0; x >>= 1) n += __shfl_xor_sync(0xffffffffu, n, x);
-          if (part == 0 && i[k] < (uint32_t)pitch) {
-            norms[((int64_t)b * H + h[k]) * pitch + i[k]] = n;
-            uint32_t* top = d_max + (int64_t)b * by_group.div(H) + by_group.div(h[k]);
-            if (__float_as_uint(n) > *(volatile uint32_t*)top) atomicMax(top, __float_as_uint(n));
-          }
+          if (part == 0 && i[k] < (uint32_t)pitch) norms[((int64_t)b * H + h[k]) * pitch + i[k]] = n;
         }
       }
     }
 }
 
-// The largest |V_j|^2 over the visible keys of a part of each (sample, memory head), and
-// zeros to the maxima of dO that the statistics' kernel raises. kLanes lanes a row.
+// The largest |V_j|^2 over the visible keys of a part of each (sample, memory head), by
+// kLanes lanes a row, and the largest of a part of its queries' |dO_i|^2. (Raised by atomics
+// in the statistics' kernel, the second cost 20 us on 8 x 16 heads, 1024 x 1024 x 64.)
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) cross_range_kernel(const T* __restrict__ v, Stride3 vs,
                                                           const uint32_t* __restrict__ words,
                                                           const int* __restrict__ vis_end, int Sk,
                                                           FastDiv by_heads, uint32_t units, int D,
-                                                          uint32_t* __restrict__ v_max,
-                                                          uint32_t* __restrict__ d_max) {
-  __shared__ uint32_t s_top[8];
+                                                          const float* __restrict__ norms, int64_t rows,
+                                                          uint32_t* __restrict__ d_max,
+                                                          uint32_t* __restrict__ v_max) {
+  __shared__ uint2 s_top[8];
   pdl_wait();
   pdl_trigger();
   constexpr int kPer = 256 / kLanes;
@@ -1031,7 +1031,10 @@ __global__ void __launch_bounds__(256) cross_range_kernel(const T* __restrict__ 
     const uint32_t b = by_heads.div(unit), kh = unit - b * by_heads.d;
     const int end = vis_end ? __ldg(vis_end + b) : Sk;
     const T* base = v + b * vs.b + kh * vs.h + part * 8;
-    uint32_t top = 0;
+    uint2 top = make_uint2(0, 0);  // of dO, of V
+#pragma unroll 4
+    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < rows; i += gridDim.x * 256)
+      top.x = max(top.x, __float_as_uint(__ldg(norms + unit * rows + i)));
 #pragma unroll 4
     for (int j0 = blockIdx.x * kPer; j0 < end; j0 += gridDim.x * kPer) {
       const int j = j0 + sub;
@@ -1042,15 +1045,16 @@ __global__ void __launch_bounds__(256) cross_range_kernel(const T* __restrict__ 
       float n = dot8<T>(x, x);
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-      top = max(top, __float_as_uint(n));
+      top.y = max(top.y, __float_as_uint(n));
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    top.x = __reduce_max_sync(0xffffffffu, top.x);
+    top.y = __reduce_max_sync(0xffffffffu, top.y);
     if (threadIdx.x % 32 == 0) s_top[threadIdx.x / 32] = top;
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int w = 1; w < 8; ++w) top = max(top, s_top[w]);
-      v_max[(int64_t)unit * gridDim.x + blockIdx.x] = top;
-      if (blockIdx.x == 0) d_max[unit] = 0;
+      for (int w = 1; w < 8; ++w) top = make_uint2(max(top.x, s_top[w].x), max(top.y, s_top[w].y));
+      d_max[(int64_t)unit * gridDim.x + blockIdx.x] = top.x;
+      v_max[(int64_t)unit * gridDim.x + blockIdx.x] = top.y;
     }
     __syncthreads();
   }
@@ -1434,15 +1438,16 @@ __global__ void __launch_bounds__(BwdGeo<kDP, kKeys, kABufs>::kThreads, 1)
       if constexpr (Type<T>::kRanged) {
         if (x.lo >= x.hi) return 0;
         const int64_t unit = (int64_t)x.b * sh.Hk + (kKeys ? (uint32_t)x.head : sh.by_group.div(x.head));
-        const uint32_t v2 = __reduce_max_sync(
-            0xffffffffu,
-            lane < outs.range.parts ? __ldg(outs.range.v_max + unit * outs.range.parts + lane) : 0u);
+        auto most = [&](const uint32_t* of) {
+          return __uint_as_float(__reduce_max_sync(
+              0xffffffffu, lane < outs.range.parts ? __ldg(of + unit * outs.range.parts + lane) : 0u));
+        };
         float d2 = 0.f;
         if (kKeys)
-          d2 = __uint_as_float(__ldg(outs.range.d_max + unit));
+          d2 = most(outs.range.d_max);
         else if (x.row0 + r < sh.Sq)
           d2 = __ldg(outs.range.norms + ((int64_t)x.b * sh.H + x.head) * stat_pitch(sh.Sq) + x.row0 + r);
-        return range_shift(d2, __uint_as_float(v2));
+        return range_shift(d2, most(outs.range.v_max));
       }
       return 0;
     };
@@ -1858,16 +1863,16 @@ int range_parts(const CrossAttnArgs& a) {
   return (int)std::max<int64_t>(
       1, std::min<int64_t>({kRangeParts, num_sms() * 8 / units, (a.Sk + rows - 1) / rows}));
 }
-// The scratch of `stats`: the row statistics, then (f16) the norms of dO's rows, their
-// maxima and those of V's.
+// The scratch of `stats`: the row statistics, then (f16) the norms of dO's rows, the
+// maxima of their parts and those of V's.
 Range range_of(const CrossAttnArgs& a) {
   Range r{};
   if (!a.half) return r;
   const int64_t rows = (int64_t)a.B * a.H * stat_pitch(a.Sq);
   r.norms = a.stats + 2 * rows;
   r.d_max = reinterpret_cast<const uint32_t*>(r.norms + rows);
-  r.v_max = r.d_max + (int64_t)a.B * a.Hk;
   r.parts = range_parts(a);
+  r.v_max = r.d_max + (int64_t)a.B * a.Hk * r.parts;
   return r;
 }
 
@@ -1966,7 +1971,8 @@ cudaError_t run_range(const CrossAttnArgs& a, const Range& r, cudaStream_t st) {
                              Stride3{a.v_st[0], a.v_st[1], a.v_st[2]},
                              (const uint32_t*)(a.key_pad ? a.words : nullptr),
                              (const int*)(a.key_pad ? a.vis_end : nullptr), a.Sk, FastDiv((uint32_t)a.Hk),
-                             units, a.D, const_cast<uint32_t*>(r.v_max), const_cast<uint32_t*>(r.d_max));
+                             units, a.D, r.norms, (int64_t)stat_pitch(a.Sq) * (a.H / a.Hk),
+                             const_cast<uint32_t*>(r.d_max), const_cast<uint32_t*>(r.v_max));
   if (e != cudaSuccess) return e;
   note_launch();
   return cudaGetLastError();
@@ -1980,20 +1986,16 @@ cudaError_t run_stats(const CrossAttnArgs& a, cudaStream_t st) {
   const int64_t x = std::min<int64_t>((rows + per - 1) / per, num_sms() * 16ll);
   const int64_t y = std::min<int64_t>({a.B, std::max<int64_t>(1, num_sms() * 16ll / x), 65535});
   const Range r = range_of(a);
-  if constexpr (Type<T>::kRanged) {
-    const cudaError_t e = run_range<T>(a, r, st);
-    if (e != cudaSuccess) return e;
-  }
   const dim3 grid((unsigned)x, (unsigned)y);
   const Stride3 ds{a.do_st[0], a.do_st[1], a.do_st[2]};
   auto k = a.D <= 64 ? cross_stats_kernel<T, 8> : cross_stats_kernel<T, 16>;
   cudaError_t e = launch_pdl(k, grid, dim3(256), 0, st, (const T*)a.out,
                              (const T*)a.out_res, (const T*)a.dout, ds,
-                             (const float*)a.lse2, (float2*)a.stats, const_cast<float*>(r.norms),
-                             const_cast<uint32_t*>(r.d_max), a.B, a.Sq, FastDiv((uint32_t)a.H),
-                             FastDiv((uint32_t)(a.H / a.Hk)), a.D);
+                             (const float*)a.lse2, (float2*)a.stats, const_cast<float*>(r.norms), a.B,
+                             a.Sq, FastDiv((uint32_t)a.H), a.D);
   if (e != cudaSuccess) return e;
   note_launch();
+  if constexpr (Type<T>::kRanged) return run_range<T>(a, r, st);
   return cudaGetLastError();
 }
 
@@ -2034,7 +2036,7 @@ cudaError_t run_bwd(const CrossAttnArgs& a, cudaStream_t st) {
 int64_t cross_attn_stats_floats(const CrossAttnArgs& a) {
   const int64_t rows = (int64_t)a.B * a.H * stat_pitch(a.Sq);
   if (!a.half) return 2 * rows;
-  return 3 * rows + ((int64_t)a.B * a.Hk * (1 + range_parts(a)) + 3) / 4 * 4;  // (what follows is 16-byte aligned)
+  return 3 * rows + ((int64_t)a.B * a.Hk * 2 * range_parts(a) + 3) / 4 * 4;  // (what follows is 16-byte aligned)
 }
 int64_t cross_attn_fwd_partials(const CrossAttnArgs& a) {
   const CrossSplits s = cross_attn_is_few(a) ? cross_attn_few_splits(a) : fwd_splits(a);
