@@ -356,6 +356,24 @@ def test_gpu_row_tiles_that_end_inside_a_warp(rows, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Sk", [65536, 65600, 140001, 1_100_000])
+def test_gpu_few_rows_masks_of_long_memories(Sk):
+    """More mask words than one CTA holds: pieces by that limit, joined by a cluster
+    and, above sixteen, by a second kernel."""
+    for D, mask in ((64, "scattered"), (8, "right"), (128, "one")):
+        check("cuda", torch.bfloat16, 2, 1, 2, 1, Sk, D, mask=mask, grad=False)
+    check("cuda", torch.float16, 1, 3, 4, 1, Sk, 8, mask="empty", grad=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gpu_many_heads_of_one_memory_head(dtype):
+    for Sq, H, Hk, Sk in ((1, 17, 1, 300), (1, 40, 1, 1000), (5, 64, 2, 70), (1, 33, 3, 5), (130, 24, 1, 90)):
+        check("cuda", dtype, 2, Sq, H, Hk, Sk, 64)
+        check("cuda", dtype, 2, Sq, H, Hk, Sk, 96, mask="right")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("mask", ["right", "left", "scattered", "empty", "one"])
 def test_gpu_tiles_masks(mask, dtype):
