@@ -148,30 +148,35 @@ def case_flash_bert(kind):
 
 
 def case_cross(kind):
-    """Attention to a memory: the LM's heads over 256 encoder states, BERT-base
-    heads over padded ones, and a serving batch's next tokens."""
+    """Attention to a memory: the LM's heads over 256 encoder states (in f16 too),
+    BERT-base heads over padded ones, a serving batch's next tokens, causal heads of
+    128, and few heads whose axes are split over a cluster."""
     from ._ext import cuda_ext
     C = cuda_ext()
-    shapes = {"cross_fwd": (B, S, S, H), "cross_bwd": (B, S, S, H),
-              "cross_fwd_bert": (32, 256, 512, 12), "cross_step": (B, 1, 4096, H)}
-    Bc, Sq, Sk, Hc = shapes[kind]
-    d = D // H
-    q, dout = _bf(Bc, Sq, Hc, d), _bf(Bc, Sq, Hc, d)
-    k, v = _bf(Bc, Sk, 2, Hc, d).unbind(2)
+    # samples, queries, keys, heads, memory heads, head size, causal
+    lm, causal, split = (B, S, S, H, H, D // H, False), (4, 2048, 2048, 16, 16, 128, True), (
+        3, 131, 777, 6, 2, 96, False)
+    shapes = {"cross_fwd": lm, "cross_bwd": lm, "cross_bwd_f16": lm, "cross_fwd_bert": (32, 256, 512, 12, 12, 64, False),
+              "cross_step": (B, 1, 4096, H, H, D // H, False), "cross_fwd_causal": causal,
+              "cross_bwd_causal": causal, "cross_fwd_split": split, "cross_bwd_split": split}
+    Bc, Sq, Sk, Hc, Hk, d, causal = shapes[kind]
+    half = (lambda t: t.half() if kind.endswith("_f16") else t)
+    q, dout = half(_bf(Bc, Sq, Hc, d)), half(_bf(Bc, Sq, Hc, d))
+    k, v = half(_bf(Bc, Sk, 2, Hk, d)).unbind(2)
     pad = None
     if kind == "cross_fwd_bert":
         pad = torch.arange(Sk, device="cuda")[None] >= Sk - torch.arange(Bc, device="cuda")[:, None] * 8
     sc = 1.0 / math.sqrt(d)
-    flops, io = 4.0 * Bc * Hc * Sq * Sk * d, 2 * (2 * q.numel() + 2 * k.numel())
+    flops, io = 4.0 * Bc * Hc * Sq * Sk * d * (0.5 if causal else 1), 2 * (2 * q.numel() + 2 * k.numel())
     if pad is not None:
         flops *= 1 - pad.float().mean().item()
-    if kind != "cross_bwd":
-        return (lambda: C.cross_attn_fwd(q, k, v, pad, False, sc, False)), flops, io
-    out, res, lse, _ = C.cross_attn_fwd(q, k, v, None, False, sc, True)
+    if "_bwd" not in kind:
+        return (lambda: C.cross_attn_fwd(q, k, v, pad, causal, sc, False)), flops, io
+    out, res, lse, _ = C.cross_attn_fwd(q, k, v, None, causal, sc, True)
     grads = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
 
     def fn():
-        C.cross_attn_bwd(dout, q, k, v, out, res, lse, None, None, False, sc, *grads)
+        C.cross_attn_bwd(dout, q, k, v, out, res, lse, None, None, causal, sc, *grads)
     return fn, 2.5 * flops, io + 2 * (2 * q.numel() + 2 * k.numel())
 
 
@@ -389,7 +394,9 @@ CASES = {
     "flash_fwd": case_flash, "flash_bwd": case_flash,
     "flash_fwd_bert": case_flash_bert, "flash_bwd_bert": case_flash_bert,
     "cross_fwd": case_cross, "cross_bwd": case_cross, "cross_fwd_bert": case_cross,
-    "cross_step": case_cross, "qk_norm_rope_fwd": case_qk_norm_rope,
+    "cross_step": case_cross, "cross_bwd_f16": case_cross, "cross_fwd_causal": case_cross,
+    "cross_bwd_causal": case_cross, "cross_fwd_split": case_cross, "cross_bwd_split": case_cross,
+    "qk_norm_rope_fwd": case_qk_norm_rope,
     "qk_norm_rope_bwd": case_qk_norm_rope, "qk_norm_rope_long": case_qk_norm_rope,
     "ln_fwd": case_ln, "ln_bwd": case_ln, "adamw": case_adamw, "sgd": case_sgd,
     "softmax_ce": case_softmax_ce, "embed_fwd": case_embed, "embed_bwd": case_embed,

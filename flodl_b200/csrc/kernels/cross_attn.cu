@@ -41,7 +41,7 @@
 // At head size 64 and a few tiles per item the round trip bounds it (scores, TMEM
 // loads, maximum, exponentials, TMEM stores, product: a warp's tile takes about 2100
 // cycles with another CTA's warp beside it, of which 512 are exponentials): tensor
-// pipe 15 to 20% busy, exponentials 31 to 38%, instruction issue 33 to 43%, DRAM 22 to 28%.
+// pipe 14 to 21% busy, exponentials 23 to 29%, instruction issue 37 to 47%, DRAM 20 to 29%.
 // The seventh product and the statistics' pass are the price of sums in a fixed order.
 //
 // Hidden keys: a packing kernel turns the padding mask into a bit per key and

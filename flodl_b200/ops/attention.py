@@ -177,7 +177,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     copied. Up to 16 query rows per memory head (``Sq * H / Hk``; the single
     tokens of serving) take a form that streams the memory once. Scores and
     sums are f32, probabilities are rounded to the inputs' type for the
-    products, and score gradients likewise in the backward (in f16 at a power of two
+    products (for a backward pass, outputs are divided by the sum of the rounded ones, and
+    may differ from those without gradients by a rounding), and score gradients likewise in the backward (in f16 at a power of two
     that the data gives, so that small ones do not vanish nor large ones overflow; the
     gradients returned have f16's own range). Gradients are the same from run to run. Other inputs, and those with forward-mode tangents, run
     the composed form in f32 or f64.
@@ -312,7 +313,8 @@ def attention_qk_norm(qkv: torch.Tensor, B: int, S: int, H: int, q_weight: Optio
                       positions: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """Self-attention over packed ``qkv [B*S, 3C]`` whose queries and keys are
     normed per head and rotated first (:func:`qk_norm_rope`, then
-    :func:`cross_attention` over the same positions); returns ``[B*S, C]``."""
+    :func:`cross_attention` over the same positions); returns ``[B*S, C]``. On CUDA
+    other types than bf16 and f16 are cast to bf16, as :func:`attention_packed` does."""
     if qkv.dim() != 2 or qkv.shape[0] != B * S or qkv.shape[1] % (3 * H):
         raise ValueError(f"qkv must be [{B * S}, 3 * {H} * D] (got {tuple(qkv.shape)})")
     if use_kernels(qkv) and qkv.dtype not in (torch.bfloat16, torch.float16):
