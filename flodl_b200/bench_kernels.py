@@ -156,7 +156,8 @@ def case_cross(kind):
     # samples, queries, keys, heads, memory heads, head size, causal
     lm, causal, split = (B, S, S, H, H, D // H, False), (4, 2048, 2048, 16, 16, 128, True), (
         3, 131, 777, 6, 2, 96, False)
-    shapes = {"cross_fwd": lm, "cross_bwd": lm, "cross_bwd_f16": lm, "cross_fwd_bert": (32, 256, 512, 12, 12, 64, False),
+    shapes = {"cross_fwd": lm, "cross_bwd": lm, "cross_bwd_f16": lm,
+              "cross_fwd_bert": (32, 256, 512, 12, 12, 64, False),
               "cross_step": (B, 1, 4096, H, H, D // H, False), "cross_fwd_causal": causal,
               "cross_bwd_causal": causal, "cross_fwd_split": split, "cross_bwd_split": split}
     Bc, Sq, Sk, Hc, Hk, d, causal = shapes[kind]

@@ -71,9 +71,9 @@ def attention_packed(qkv: torch.Tensor, B: int, S: int, H: int, causal: bool = F
     """Self-attention over packed ``qkv [B*S, 3C]``; returns ``[B*S, C]``.
 
     ``key_padding`` (bool ``[B, S]``, True = masked key) implements the padding
-    mask used by BERT-style encoders; with ``causal`` both apply. On CUDA the flash kernel takes
-    head size 64, :func:`cross_attention` the others and empty inputs; the result
-    is bf16.
+    mask used by BERT-style encoders; with ``causal`` both apply. On CUDA the
+    flash kernel takes head size 64, :func:`cross_attention` the others and empty
+    inputs; the result is bf16.
     """
     if not use_kernels(qkv):
         D = qkv.shape[1] // (3 * H)
@@ -176,12 +176,14 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     head-major tensors transposed to this layout) are read in place, others are
     copied. Up to 16 query rows per memory head (``Sq * H / Hk``; the single
     tokens of serving) take a form that streams the memory once. Scores and
-    sums are f32, probabilities are rounded to the inputs' type for the
-    products (for a backward pass, outputs are divided by the sum of the rounded ones, and
-    may differ from those without gradients by a rounding), and score gradients likewise in the backward (in f16 at a power of two
-    that the data gives, so that small ones do not vanish nor large ones overflow; the
-    gradients returned have f16's own range). Gradients are the same from run to run. Other inputs, and those with forward-mode tangents, run
-    the composed form in f32 or f64.
+    sums are f32; probabilities are rounded to the inputs' type for the products,
+    and score gradients in the backward (in f16 at a power of two that the data
+    gives, so that small ones do not vanish nor large ones overflow; the gradients
+    returned have f16's own range). With gradients, outputs are divided by the sum
+    of the rounded probabilities and may differ by a rounding from those without.
+    Gradients are the same from run to run. Other inputs, scales below 1e-18 or
+    beyond 1e18, and inputs with forward-mode tangents run the composed form in f32
+    or f64.
     """
     if use_kernels(q):
         out = C().cross_attention(q, k, v, key_padding, causal, scale)

@@ -244,9 +244,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
 
     CUDA f32, bf16 and f16 inputs with 2 <= D <= 256 run one kernel forward and one
     backward (plus a reduction of the weight gradients); other inputs, those with
-    forward-mode tangents and tables that want gradients run the composed form. A position outside the tables gives NaN in the rotated
-    values of its heads and records code 5 in the kernel error word on CUDA;
-    on the CPU it raises.
+    forward-mode tangents and tables that want gradients run the composed form. A
+    position outside the tables gives NaN in the rotated values of its heads on
+    CUDA (the kernel records code 5 in the error word, too); on the CPU it raises.
     """
     if use_kernels(q):
         y = C().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, offset, eps)
