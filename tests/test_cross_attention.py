@@ -505,6 +505,63 @@ def test_gpu_repeats_graphs_and_streams(shape):
 
 
 @pytest.mark.gpu
+def test_gpu_f16_passes_at_once():
+    """Training passes of several shapes on streams, in threads and as graphs replayed
+    side by side give the bits of one after another."""
+    import threading
+    shapes = [(2, 130, 4, 2, 700, 64), (1, 40, 2, 2, 3000, 128), (3, 3, 4, 1, 500, 96), (8, 200, 8, 8, 200, 64)]
+    data = []
+    for i, shape in enumerate(shapes):
+        q, k, v, do = make(*shape, torch.float16, "cuda", seed=i)
+        data.append(([x.requires_grad_() for x in (q, k, v)], do * 10.0 ** (1 - i),
+                     mask_of("right", shape[0], shape[4], "cuda")))
+
+    def once(i):
+        leaves, do, pad = data[i]
+        out = ops.cross_attention(*leaves, key_padding=pad)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+    want = [once(i) for i in range(4)]
+    torch.cuda.synchronize()
+    same = lambda got: all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for turn in range(4):
+        got = [None] * 4
+        for i in range(4):
+            with torch.cuda.stream(streams[(i + turn) % 4]):
+                got[i] = once(i)
+        torch.cuda.synchronize()
+        assert same(got)
+
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(10):
+                got[i] = once(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert same(got)
+    graphs = []
+    for i in range(4):
+        with torch.cuda.stream(streams[i]):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[i], stream=streams[i]):
+                got[i] = once(i)
+    for _ in range(3):
+        for i in range(4):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    assert same(got)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("scale", [1e-50, 1e-40, 1e-18, 1e-10])
 def test_gpu_tiny_scales(scale):
     """Scores vanish: a query's output is the mean of the values (a sum of 70 rounded
